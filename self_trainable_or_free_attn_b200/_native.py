@@ -1,5 +1,5 @@
-"""ctypes binding of libechosparse_sm100.so (the C ABI declared in include/echosparse_sm100.h and
-include/echosparse_vsa_sm100.h).
+"""ctypes binding of libechosparse_sm100.so (the C ABI declared in include/echosparse_sm100.h,
+include/echosparse_vsa_sm100.h and include/echosparse_packed_sm100.h).
 
 There is no fallback: if the library is missing or a call fails, this raises. PyTorch tensors are passed as raw device
 pointers; the launch goes on torch's current CUDA stream.
@@ -73,11 +73,21 @@ SIGNATURES = {
                                _I, _I, _I, _P],
     "es_vsa_tier_rep_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "es_vsa_tier_unpool": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    "es_packed_workspace_bytes": [_I] * 6,
+    "es_packed_attn_fwd": [_P] * 7 + [_I] * 6 + [_I64] * 6 + [_F, _I, _I, _P, _P],
+    "es_packed_delta": [_P, _P, _P, _I, _I, _I, _I64, _I64, _I, _P],
+    "es_packed_attn_bwd_q": [_P] * 9 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
+    "es_packed_attn_bwd_kv": [_P] * 10 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
+    "es_prefix_workspace_bytes": [_I] * 8,
+    "es_prefix_attn": [_P] * 6 + [_I, _I, _P, _I, _P] + [_I] * 7 + [_I64] * 6 + [_F, _I, _P, _P],
+    "es_extend_tables": [_P] * 4 + [_I] * 5 + [_P] * 6,
+    "es_store_kv": [_P] * 5 + [_I] * 5 + [_I64] * 10 + [_P],
 }
 _RESTYPES = {"es_last_error": ctypes.c_char_p, "es_launch_count": ctypes.c_longlong,
              "es_dense_scratch_bytes": ctypes.c_longlong,
              "es_vsa_topk_workspace_bytes": ctypes.c_longlong, "es_vsa_split_plan_workspace_bytes": ctypes.c_longlong,
-             "es_vsa_topk_bits_offset": ctypes.c_longlong}
+             "es_vsa_topk_bits_offset": ctypes.c_longlong, "es_packed_workspace_bytes": ctypes.c_longlong,
+             "es_prefix_workspace_bytes": ctypes.c_longlong}
 
 _lib = None
 
@@ -140,7 +150,7 @@ def device_guard(fn):
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
         import torch
-        for a in args:
+        for a in (*args, *kwargs.values()):
             if isinstance(a, torch.Tensor):
                 if a.is_cuda and a.get_device() != torch._C._cuda_getDevice():
                     with torch.cuda.device(a.device):

@@ -1,0 +1,282 @@
+// A paged cache of keys and values: pages and slots of new tokens, storing them, and attention of a batch's next tokens to a shared
+// prefix and to each request's own tokens. Entry points at the end.
+#include "es_packed.cuh"
+
+namespace es {
+namespace packed {
+namespace {
+
+__device__ __forceinline__ float warp_max(float x) {
+    for (int i = 16; i; i >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
+    return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+    for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+    return x;
+}
+
+struct CacheRows {
+    int64_t page, token, head;
+};
+
+struct PrefixArgs {
+    const int *prefix_pages, *table, *lengths;
+    float* lse;
+    int prefix_len, width, B, N, H, Hk, pages, log_page;
+    float scale;
+};
+
+// A warp per query row, 32 keys at a time.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) prefix_rows_kernel(const T* q, const T* kc, CacheRows rk, const T* vc, CacheRows rv, T* o, PrefixArgs a) {
+    constexpr int C = D / 32;
+    __shared__ float rows[4][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 4 + warp;
+    if (row >= (int64_t)a.B * a.N * a.H) return;
+    const int h = (int)(row % a.H), i = (int)(row / a.H % a.N), b = (int)(row / a.H / a.N), hk = h / (a.H / a.Hk);
+    for (int c = lane; c < D; c += 32) rows[warp][c] = to_float(q[row * D + c]);
+    __syncwarp();
+    const int own = min(max(min(a.lengths[b], a.width << a.log_page) - a.N + i + 1, 0), a.width << a.log_page);
+    float top = -INFINITY, sum = 0.f, acc[C] = {};
+    for (int part = 0; part < 2; ++part) {
+        const int n = part ? own : a.prefix_len;
+        const int* list = part ? a.table + (int64_t)b * a.width : a.prefix_pages;
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            const int j = j0 + lane, page = j < n ? list[j >> a.log_page] : -1, at = j & ((1 << a.log_page) - 1);
+            const bool seen = page >= 0 && page < a.pages;
+            float x = -INFINITY;
+            if (seen) {
+                const T* kr = kc + page * rk.page + at * rk.token + hk * rk.head;
+                x = 0.f;
+                for (int c = 0; c < D; ++c) x += rows[warp][c] * to_float(kr[c]);
+                x *= a.scale * kLog2e;
+            }
+            const float next = fmaxf(top, warp_max(x)), off = next == -INFINITY ? 0.f : next, shrink = exp2f(top - off);
+            const float p = seen ? exp2f(x - off) : 0.f;
+            sum = sum * shrink + warp_sum(p);
+            top = next;
+            for (int c = 0; c < C; ++c) acc[c] *= shrink;
+            for (int jj = 0; jj < 32; ++jj) {
+                const float w = __shfl_sync(0xffffffffu, p, jj);
+                const int pg = __shfl_sync(0xffffffffu, page, jj), tk = __shfl_sync(0xffffffffu, at, jj);
+                if (pg < 0 || pg >= a.pages) continue;
+                const T* vr = vc + pg * rv.page + tk * rv.token + hk * rv.head;
+                for (int c = 0; c < C; ++c) acc[c] += w * to_float(vr[lane + 32 * c]);
+            }
+        }
+    }
+    const bool none = sum == 0.f;
+    for (int c = 0; c < C; ++c) o[row * D + lane + 32 * c] = from_float<T>(none ? 0.f : acc[c] / sum);
+    if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + i] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------------------------- pages and slots
+constexpr int PLAN_THREADS = 256, PLAN_CHUNK = 1024;          // requests that a CTA scans at a time
+constexpr int PLAN_TOKENS = 1024;                             // tokens of a CTA
+
+struct PlanArgs {
+    const int *lengths, *new_tokens, *free_pages;
+    int *table, *slots, *positions, *cu_new, *lengths_out, *taken;
+    int n_free, B, width, page, total;
+};
+
+// With len = lengths[b], n = new_tokens[b]: the request has have = ceil(len / page) pages and wants ceil((len + n) / page), at most the row's
+// width; its missing pages are free_pages[first ...], first the exclusive sum of need = wanted - held over the requests before it. Every CTA
+// makes both running sums itself (a few KB of L2 per thousand requests; a second kernel would cost a launch) and then places its own
+// share of the requests and of the tokens.
+__global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a) {
+    __shared__ int s_cu[PLAN_CHUNK + 1], s_first[PLAN_CHUNK + 1];
+    __shared__ long long s_warp[2][PLAN_THREADS / 32];
+    constexpr int PER = PLAN_CHUNK / PLAN_THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long cap = 0x7FFFFFFF;
+    long long tokens = 0, pages = 0, missing = 0;             // of the chunks before (the sums may pass 32 bits; what is stored saturates)
+    const long long t0 = (long long)blockIdx.x * PLAN_TOKENS, t1 = min(t0 + PLAN_TOKENS, (long long)a.total);
+    for (int b0 = 0; b0 < a.B; b0 += PLAN_CHUNK) {
+        const int nb = min(PLAN_CHUNK, a.B - b0);
+        long long n[PER], need[PER], sn = 0, sp = 0;
+        for (int i = 0; i < PER; ++i) {
+            const int b = b0 + tid * PER + i;
+            n[i] = need[i] = 0;
+            if (b < b0 + nb) {
+                const long long len = max(a.lengths[b], 0);
+                n[i] = max(a.new_tokens[b], 0);
+                const long long have = min((len + a.page - 1) / a.page, (long long)a.width), want = min((len + n[i] + a.page - 1) / a.page, (long long)a.width);
+                need[i] = want - have;
+            }
+            sn += n[i]; sp += need[i];
+        }
+        long long xn = sn, xp = sp;
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long yn = __shfl_up_sync(0xffffffffu, xn, d), yp = __shfl_up_sync(0xffffffffu, xp, d);
+            if (lane >= d) { xn += yn; xp += yp; }
+        }
+        if (lane == 31) { s_warp[0][warp] = xn; s_warp[1][warp] = xp; }
+        __syncthreads();
+        long long bn = tokens, bp = pages, an = tokens, ap = pages;
+        for (int w = 0; w < PLAN_THREADS / 32; ++w) {
+            if (w < warp) { bn += s_warp[0][w]; bp += s_warp[1][w]; }
+            an += s_warp[0][w]; ap += s_warp[1][w];
+        }
+        bn += xn - sn; bp += xp - sp;
+        for (int i = 0; i < PER; ++i) {
+            s_cu[tid * PER + i] = (int)min(bn, cap);
+            s_first[tid * PER + i] = (int)min(bp, cap);
+            bn += n[i]; bp += need[i];
+        }
+        if (tid == 0) { s_cu[PLAN_CHUNK] = (int)min(an, cap); s_first[PLAN_CHUNK] = (int)min(ap, cap); }
+        __syncthreads();
+        // requests: their lengths, table entries and shares of the outputs, spread over the CTAs
+        for (int r = blockIdx.x * PLAN_THREADS + tid; r < nb; r += gridDim.x * PLAN_THREADS) {
+            const int b = b0 + r, len = max(a.lengths[b], 0);
+            const long long after = (long long)len + max(a.new_tokens[b], 0);
+            const int have = (int)min(((long long)len + a.page - 1) / a.page, (long long)a.width), want = (int)min((after + a.page - 1) / a.page, (long long)a.width);
+            const int first = s_first[r], got = min(max(a.n_free - first, 0), want - have);
+            for (int j = have; j < want; ++j) a.table[(size_t)b * a.width + j] = j - have < got ? a.free_pages[first + j - have] : -1;
+            a.lengths_out[b] = max(len, (int)min(after, min((long long)(have + got) * a.page, cap)));
+            a.cu_new[b] = s_cu[r];
+        }
+        // tokens of this CTA that belong to the chunk
+        const int lo = (int)max(t0, (long long)s_cu[0]), hi = (int)min(t1, (long long)s_cu[nb == PLAN_CHUNK ? PLAN_CHUNK : nb]);
+        for (int t = lo + tid; t < hi; t += PLAN_THREADS) {
+            int x = 0, y = nb;                                // the last request of the chunk that starts at or before t
+            while (x + 1 < y) {
+                const int m = (x + y) >> 1;
+                if (s_cu[m] <= t) x = m; else y = m;
+            }
+            const int b = b0 + x, len = max(a.lengths[b], 0);
+            const long long pos = (long long)len + (t - s_cu[x]), col = pos / a.page;
+            const int have = (int)min(((long long)len + a.page - 1) / a.page, (long long)a.width);
+            int p = -1;
+            if (col < have) p = a.table[(size_t)b * a.width + col];       // (held before the call: nobody writes it)
+            else if (col < a.width && s_first[x] + (col - have) < a.n_free) p = a.free_pages[s_first[x] + (col - have)];
+            const long long slot = (long long)p * a.page + pos % a.page;
+            a.slots[t] = p >= 0 && slot <= cap ? (int)slot : -1;
+            a.positions[t] = (int)min(pos, cap);
+        }
+        if (blockIdx.x == 0)
+            for (int r = tid; r < nb; r += PLAN_THREADS) {    // pages needed and not there
+                const int b = b0 + r, len = max(a.lengths[b], 0);
+                const long long held = ((long long)len + a.page - 1) / a.page, wanted = ((long long)len + max(a.new_tokens[b], 0) + a.page - 1) / a.page;
+                const long long have = min(held, (long long)a.width), want = min(wanted, (long long)a.width);
+                missing += (wanted - held) - min(max((long long)a.n_free - s_first[r], 0ll), want - have);
+            }
+        tokens = an; pages = ap;
+        __syncthreads();
+    }
+    for (long long t = max(t0, tokens) + tid; t < t1; t += PLAN_THREADS) a.slots[t] = a.positions[t] = -1;
+    if (blockIdx.x == 0) {
+        for (int d = 16; d; d >>= 1) missing += __shfl_xor_sync(0xffffffffu, missing, d);
+        if (lane == 0) s_warp[0][warp] = missing;
+        __syncthreads();
+        if (tid == 0) {
+            missing = 0;
+            for (int w = 0; w < PLAN_THREADS / 32; ++w) missing += s_warp[0][w];
+            a.cu_new[a.B] = (int)min(tokens, cap);
+            a.taken[0] = (int)min(pages, (long long)a.n_free);
+            a.taken[1] = (int)min(missing, cap);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- storing
+struct StoreArgs {
+    const uint4 *k, *v;
+    uint4 *kc, *vc;
+    const int* slots;
+    Rows rk, rv;                     // strides here in 16-byte chunks
+    CacheRows rkc, rvc;
+    int total, Hk, pages, page;
+};
+
+// A thread per 16 bytes: consecutive threads take the chunks of a row of K, then of V.
+template <int D> __global__ void __launch_bounds__(256) store_kv_kernel(StoreArgs a) {
+    constexpr int CH = D / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int c = (int)(i % CH);
+    const int64_t row = i / CH;
+    const int64_t th = row >> 1;
+    const int h = (int)(th % a.Hk);
+    const int64_t t = th / a.Hk;
+    if (t >= a.total) return;
+    const int slot = a.slots[t];
+    if (slot < 0 || slot / a.page >= a.pages) return;
+    const int page = slot / a.page, at = slot % a.page;
+    if (row & 1) a.vc[page * a.rvc.page + at * a.rvc.token + h * a.rvc.head + c] = a.v[t * a.rv.token + h * a.rv.head + c];
+    else a.kc[page * a.rkc.page + at * a.rkc.token + h * a.rkc.head + c] = a.k[t * a.rk.token + h * a.rk.head + c];
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace es
+
+using namespace es;
+using namespace es::packed;
+
+extern "C" long long es_prefix_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+
+extern "C" int es_prefix_attn(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse, const int32_t* prefix_pages,
+                              int32_t n_prefix_pages, int32_t prefix_len, const int32_t* table, int32_t table_width, const int32_t* lengths,
+                              int32_t batch, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t D, int32_t pages, int32_t page_size,
+                              int64_t k_page, int64_t k_token, int64_t k_head, int64_t v_page, int64_t v_token, int64_t v_head, float scale,
+                              int32_t dtype, void* workspace, void* stream) {
+    (void)workspace;
+    if (int rc = check_sizes("es_prefix_attn", batch, tokens, prefix_len, heads, kv_heads, D, dtype)) return rc;
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+        return set_error(-1, "es_prefix_attn: page_size must be 16, 32, 64, 128 or 256");
+    if (pages < 0 || table_width < 0 || n_prefix_pages < 0 || (int64_t)table_width * page_size > 0x7FFFFFFF || (int64_t)pages * page_size > 0x7FFFFFFF ||
+        (int64_t)n_prefix_pages * page_size < prefix_len || (int64_t)batch * tokens * heads > 0x7FFFFFFF)
+        return set_error(-1, "es_prefix_attn: sizes out of range");
+    if (batch == 0 || tokens == 0) return 0;
+    if (!q || !o || !lse || !lengths || (prefix_len && !prefix_pages) || (table_width && !table) || (pages && (!k_cache || !v_cache)))
+        return set_error(-1, "es_prefix_attn: null pointer");
+    if (!aligned(16, q, k_cache, v_cache, o)) return set_error(-1, "es_prefix_attn: q, k_cache, v_cache, o must be 16-byte aligned");
+    if (!whole_chunks(k_page, k_token, k_head, v_page, v_token, v_head)) return set_error(-1, "es_prefix_attn: strides must be multiples of 8 elements");
+    PrefixArgs a{prefix_pages, table, lengths, lse, prefix_len, table_width, batch, tokens, heads, kv_heads, pages, 0, scale};
+    while ((1 << a.log_page) < page_size) ++a.log_page;
+    const unsigned grid = (unsigned)(((int64_t)batch * tokens * heads + 3) / 4);
+    auto go = [&](auto t, auto d) {
+        using T = decltype(t);
+        prefix_rows_kernel<T, d><<<grid, 128, 0, (cudaStream_t)stream>>>((const T*)q, (const T*)k_cache, {k_page, k_token, k_head}, (const T*)v_cache,
+                                                                         {v_page, v_token, v_head}, (T*)o, a);
+        ES_CHECK_LAUNCH("prefix_rows_kernel");
+        return 0;
+    };
+    if (dtype == 0) return D == 64 ? go(__nv_bfloat16{}, std::integral_constant<int, 64>{}) : go(__nv_bfloat16{}, std::integral_constant<int, 128>{});
+    return D == 64 ? go(__half{}, std::integral_constant<int, 64>{}) : go(__half{}, std::integral_constant<int, 128>{});
+}
+
+extern "C" int es_extend_tables(const int32_t* lengths, const int32_t* new_tokens, int32_t* table, const int32_t* free_pages, int32_t n_free,
+                                int32_t batch, int32_t table_width, int32_t page_size, int32_t total, int32_t* slots, int32_t* positions,
+                                int32_t* cu_new, int32_t* lengths_out, int32_t* taken, void* stream) {
+    if (n_free < 0 || batch < 0 || table_width < 0 || page_size < 1 || total < 0) return set_error(-1, "es_extend_tables: sizes out of range");
+    if (!cu_new || !taken || (batch && (!lengths || !new_tokens || !lengths_out)) || (batch && table_width && !table) || (n_free && !free_pages) ||
+        (total && (!slots || !positions)))
+        return set_error(-1, "es_extend_tables: null pointer");
+    const PlanArgs a{lengths, new_tokens, free_pages, table, slots, positions, cu_new, lengths_out, taken, n_free, batch, table_width, page_size, total};
+    const unsigned grid = (unsigned)std::max<int64_t>(1, ((int64_t)total + PLAN_TOKENS - 1) / PLAN_TOKENS);
+    extend_tables_kernel<<<grid, PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
+    ES_CHECK_LAUNCH("extend_tables_kernel");
+    return 0;
+}
+
+extern "C" int es_store_kv(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* slots, int32_t total, int32_t kv_heads,
+                           int32_t D, int32_t pages, int32_t page_size, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                           int64_t kc_page, int64_t kc_token, int64_t kc_head, int64_t vc_page, int64_t vc_token, int64_t vc_head, void* stream) {
+    if (int rc = check_sizes("es_store_kv", 0, total, 0, kv_heads, kv_heads, D, 0)) return rc;
+    if (pages < 0 || page_size < 1 || (int64_t)pages * page_size > 0x7FFFFFFF) return set_error(-1, "es_store_kv: sizes out of range");
+    if (total == 0 || pages == 0) return 0;
+    if (!k || !v || !k_cache || !v_cache || !slots) return set_error(-1, "es_store_kv: null pointer");
+    if (!aligned(16, k, v, k_cache, v_cache)) return set_error(-1, "es_store_kv: k, v, k_cache, v_cache must be 16-byte aligned");
+    if (!whole_chunks(k_token, k_head, v_token, v_head, kc_page, kc_token, kc_head, vc_page, vc_token, vc_head))
+        return set_error(-1, "es_store_kv: strides must be multiples of 8 elements");
+    const StoreArgs a{(const uint4*)k, (const uint4*)v, (uint4*)k_cache, (uint4*)v_cache, slots, {k_token / 8, k_head / 8}, {v_token / 8, v_head / 8},
+                      {kc_page / 8, kc_token / 8, kc_head / 8}, {vc_page / 8, vc_token / 8, vc_head / 8}, total, kv_heads, pages, page_size};
+    const int64_t n = (int64_t)total * kv_heads * 2 * (D / 8);
+    const unsigned grid = (unsigned)((n + 255) / 256);
+    if (D == 64) store_kv_kernel<64><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+    else store_kv_kernel<128><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+    ES_CHECK_LAUNCH("store_kv_kernel");
+    return 0;
+}

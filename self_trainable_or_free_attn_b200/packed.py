@@ -1,0 +1,166 @@
+"""Attention over packed sequences: the tokens of a batch lie behind one another, without padding between them.
+
+`packed_attention` is exact softmax attention of every sequence to its own keys, with gradients: causal or full, with as many
+query heads to a key head as the model has, from sequences of one token to long ones. It stands beside the block-sparse operators of
+`vsa`, which take sequences of one length: the same kernels' conventions (bf16 or fp16, head dim 64 or 128, fp32 softmax and LSE, one owner
+per gradient row: reproducible bit for bit).
+
+  q        [tokens, heads, D]; k, v [tokens, kv_heads, D], heads a multiple of kv_heads; any token and head strides (the thirds
+           of a fused projection, say); what the kernels' loads cannot take (a last dimension with a stride, rows off 16 bytes) is copied
+  cu_q     int32 [batch + 1] on the device, not decreasing: sequence b has the tokens cu_q[b] .. cu_q[b + 1] - 1
+  cu_k     the same for the keys where they are more than the queries (a prompt's next chunk behind what is there)
+
+Tokens of no sequence (behind the last, say) get output 0, LSE -inf and gradient 0, and what they hold reaches no other row; the same
+is true of keys that the causal mask hides.
+"""
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as N
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+DIMS = (64, 128)
+
+
+def usable(t):
+    """Whether the kernels' 16-byte loads can take t [..., D] as it lies: its rows in one piece, no two rows the same memory."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(n == 1 or (s % 8 == 0 and t.shape[-1] <= s < 2 ** 39) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
+
+
+def rows(t):
+    """t itself where the kernels can read it, else a copy."""
+    return t if usable(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def strides(t):
+    """Element strides of all but the last dimension; those of dimensions of one entry, which nothing uses, as if contiguous."""
+    whole, out = t.shape[-1], []
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        out.append(s if n > 1 else whole)
+        whole = max(whole, out[-1] * n)
+    return tuple(reversed(out))
+
+
+def softmax_scale(scale, D):
+    if scale is None:
+        return 1.0 / math.sqrt(D)
+    scale = float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale must be a finite number above 0, got {scale}")
+    return scale
+
+
+def check_heads(q_heads, kv_heads, D):
+    if D not in DIMS:
+        raise RuntimeError(f"the head dim must be one of {DIMS}, got {D}")
+    if kv_heads < 1 or q_heads < 1 or q_heads % kv_heads:
+        raise RuntimeError(f"the query heads ({q_heads}) must be a multiple of the key heads ({kv_heads})")
+
+
+def check_tokens(ref, **tensors):
+    """Every tensor on the CUDA device of `ref` and in its dtype, bf16 or fp16."""
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be a CUDA tensor: this operator has no CPU path")
+        if t.device != ref.device:
+            raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
+        if t.dtype not in _DTYPES or t.dtype != ref.dtype:
+            raise RuntimeError("all of them must share the dtype bfloat16 or float16: " + ", ".join(tensors))
+
+
+def check_ints(ref, **tensors):
+    """Device tensors of whole numbers as int32, contiguous."""
+    out = []
+    for name, t in tensors.items():
+        if t.device != ref.device:
+            raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
+        if t.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"{name} must be int32, got {t.dtype}")
+        out.append(t.to(torch.int32).contiguous())
+    return out
+
+
+def _call(name, *args):
+    N.check(getattr(N.load(), name)(*args), name)
+
+
+def _fwd(q, k, v, cu_q, cu_k, scale, causal):
+    T, H, D = q.shape
+    o = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(H, T, device=q.device, dtype=torch.float32)
+    B, Hk = cu_q.numel() - 1, k.shape[1]
+    n = int(N.load().es_packed_workspace_bytes(B, T, k.shape[0], H, Hk, D))
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    _call("es_packed_attn_fwd", N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(o), N.ptr(lse), N.ptr(cu_q), N.ptr(cu_k), B, T, k.shape[0], H, Hk, D,
+          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
+    return o, lse
+
+
+class _Function(torch.autograd.Function):
+    @staticmethod
+    @N.device_guard
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
+        o, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        ctx.scale, ctx.causal = scale, causal
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    @N.device_guard
+    def backward(ctx, dout, dlse):
+        if dout is None:
+            return (None,) * 7
+        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        dout = rows(dout)
+        (T, H, D), (Tk, Hk, _) = q.shape, k.shape
+        delta = torch.empty_like(lse)
+        dt, st = _DTYPES[q.dtype], N.stream_ptr()
+        _call("es_packed_delta", N.ptr(o), N.ptr(dout), N.ptr(delta), T, H, D, *strides(dout), dt, st)
+        sizes = (cu_q.numel() - 1, T, Tk, H, Hk, D, *strides(q), *strides(k), *strides(v), *strides(dout), ctx.scale, ctx.causal, dt, st)
+        ins = [N.ptr(t) for t in (q, k, v, dout, lse, delta)]
+        cus = (N.ptr(cu_q), N.ptr(cu_k))
+        dq = dk = dv = None
+        if ctx.needs_input_grad[0]:
+            dq = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
+            _call("es_packed_attn_bwd_q", *ins, N.ptr(dq), *cus, *sizes)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dk, dv = (torch.empty(Tk, Hk, D, device=q.device, dtype=q.dtype) for _ in range(2))
+            _call("es_packed_attn_bwd_kv", *ins, N.ptr(dk), N.ptr(dv), *cus, *sizes)
+        return dq, dk, dv, None, None, None, None
+
+
+@N.device_guard
+def packed_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, return_lse=False):
+    """Softmax attention of every sequence of a packed batch to its own keys: [tokens, heads, D], and with return_lse also the
+    natural-log LSE [heads, tokens] in fp32 (no gradient flows through it).
+
+    `causal`: query i of nq sees the keys j <= i + nk - nq of its sequence's nk (the last query sees all); a row that sees none is 0 with
+    LSE -inf. `scale`: factor of q k^T, 1 / sqrt(D) by default. cu_q, cu_k are read on the GPU only: nothing synchronises, and a
+    captured call follows them when they change."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise RuntimeError(f"{name} must be [tokens, heads, D], got {tuple(t.shape)}")
+    check_tokens(q, q=q, k=k, v=v)
+    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise RuntimeError("k and v must have one shape, and the head dim of q")
+    check_heads(q.shape[1], k.shape[1], q.shape[2])
+    if cu_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise RuntimeError(f"without cu_k there are as many keys as queries, got {k.shape[0]} and {q.shape[0]}")
+        cu_q, = check_ints(q, cu_q=cu_q)
+        cu_k = cu_q
+    else:
+        cu_q, cu_k = check_ints(q, cu_q=cu_q, cu_k=cu_k)
+    if cu_q.dim() != 1 or cu_q.numel() < 1 or cu_k.shape != cu_q.shape:
+        raise RuntimeError("cu_q and cu_k must be [batch + 1]")
+    if max(q.shape[0], k.shape[0]) >= 2 ** 31 - 256:
+        raise RuntimeError("at most 2**31 - 257 tokens")
+    scale = softmax_scale(scale, q.shape[2])
+    o, lse = _Function.apply(rows(q), rows(k), rows(v), cu_q, cu_k, scale, int(bool(causal)))
+    return (o, lse) if return_lse else o
