@@ -8,6 +8,10 @@
 
 namespace es {
 namespace packed {
+
+int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, float* lse, const Batch& b, int D, int dtype, void* ws,
+                  cudaStream_t st);
+
 namespace {
 
 template <typename T, int D> __device__ __forceinline__ float dot_row(const float* a, const T* b) {
@@ -21,53 +25,12 @@ template <typename T, int D> __device__ __forceinline__ float dot_row(const floa
     return s;
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-    for (int i = 16; i; i >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
-    return x;
-}
 __device__ __forceinline__ float warp_sum(float x) {
     for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
     return x;
 }
 
 constexpr int WARPS = 8;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * WARPS) fwd_rows_kernel(const T* q, Rows rq, const T* k, Rows rk, const T* v, Rows rv, T* o, float* lse, Batch b) {
-    constexpr int C = D / 32;
-    __shared__ float rows[WARPS][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * WARPS + warp;
-    if (row >= (int64_t)b.Tq * b.H) return;
-    const int t = (int)(row / b.H), h = (int)(row % b.H), hk = h / b.G;
-    const int s = sequence_of(b.cu_q, b.B, t);
-    int n = 0, k0 = 0;
-    if (s >= 0) {
-        const int q0 = b.q_at(s), nq = b.q_at(s + 1) - q0, nk = max(b.k_at(s + 1) - b.k_at(s), 0);
-        k0 = b.k_at(s);
-        n = b.causal ? min(max(t - q0 + 1 + nk - nq, 0), nk) : nk;
-    }
-    for (int c = lane; c < D; c += 32) rows[warp][c] = to_float(q[t * rq.token + h * rq.head + c]);
-    __syncwarp();
-    float top = -INFINITY, sum = 0.f, acc[C] = {};
-    for (int j0 = 0; j0 < n; j0 += 32) {
-        const int j = j0 + lane;
-        float x = -INFINITY;
-        if (j < n) x = dot_row<T, D>(rows[warp], k + (int64_t)(k0 + j) * rk.token + hk * rk.head) * (b.scale * kLog2e);
-        const float next = fmaxf(top, warp_max(x)), off = next == -INFINITY ? 0.f : next, shrink = exp2f(top - off);
-        const float p = j < n ? exp2f(x - off) : 0.f;
-        sum = sum * shrink + warp_sum(p);
-        top = next;
-        for (int i = 0; i < C; ++i) acc[i] *= shrink;
-        for (int jj = 0; jj < min(32, n - j0); ++jj) {
-            const float w = __shfl_sync(0xffffffffu, p, jj);
-            const T* vr = v + (int64_t)(k0 + j0 + jj) * rv.token + hk * rv.head;
-            for (int i = 0; i < C; ++i) acc[i] += w * to_float(vr[lane + 32 * i]);
-        }
-    }
-    for (int i = 0; i < C; ++i) o[((int64_t)t * b.H + h) * D + lane + 32 * i] = from_float<T>(n > 0 ? acc[i] / sum : 0.f);
-    if (lane == 0) lse[(int64_t)h * b.Tq + t] = n > 0 ? (top + log2f(sum)) * kLn2 : -INFINITY;
-}
 
 template <typename T, int D> __global__ void __launch_bounds__(256) delta_kernel(const T* o, const T* dout, Rows rdo, float* delta, int Tq, int H) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -187,20 +150,13 @@ extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, v
                                   int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D,
                                   int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
                                   float scale, int32_t causal, int32_t dtype, void* workspace, void* stream) {
-    (void)workspace;
     if (int rc = check_sizes("es_packed_attn_fwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
     if (total_q == 0) return 0;
     if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v))) return set_error(-1, "es_packed_attn_fwd: null pointer");
     if (!aligned(16, q, k, v, o)) return set_error(-1, "es_packed_attn_fwd: q, k, v, o must be 16-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head)) return set_error(-1, "es_packed_attn_fwd: strides must be multiples of 8 elements");
     const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
-    return with_type(dtype, D, [&](auto t, auto d) {
-        using T = decltype(t);
-        fwd_rows_kernel<T, d><<<blocks((int64_t)total_q * heads), 32 * WARPS, 0, (cudaStream_t)stream>>>(
-            (const T*)q, {q_token, q_head}, (const T*)k, {k_token, k_head}, (const T*)v, {v_token, v_head}, (T*)o, lse, b);
-        ES_CHECK_LAUNCH("fwd_rows_kernel");
-        return 0;
-    });
+    return packed_fwd_tc(q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, o, lse, b, D, dtype, workspace, (cudaStream_t)stream);
 }
 
 extern "C" int es_packed_delta(const void* o, const void* dout, float* delta, int32_t total_q, int32_t heads, int32_t D, int64_t do_token,

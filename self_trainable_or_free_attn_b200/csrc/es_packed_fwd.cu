@@ -1,0 +1,544 @@
+// Forward attention of packed sequences, and of new tokens to a paged cache, on the 5th-generation tensor cores: one pass over the keys
+// with the running maximum and sum of the softmax.
+//
+//   S = scale Q K^T, P = exp(S - m), l = sum P, O = P V / l, LSE = m + log l
+//
+// A CTA has two tiles of 128 query rows and walks the keys 128 at a time. The rows of a tile are (token, head) pairs, the `pack` query heads
+// of a key head next to one another: all of them read the same K and V, a tile covers 128 / pack tokens, and the causal diagonal
+// wastes that much less. One new token of a request still fills `pack` rows.
+//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, a thread per row
+//   warp 8          issues the MMAs; warp 9 issues the TMA loads
+// Tensor memory: S of tile 0, of tile 1 (128 columns each; P overwrites the first 64 of its S as 16-bit pairs and is the MMA's A operand from
+// there), O of tile 0, of tile 1 (D columns each). The MMAs of an iteration are P V of tile 0, Q K^T of tile 0 for the next keys, the same two of
+// tile 1: while one tile's softmax runs the tensor cores work for the other. K and V go through one ring in the order of use.
+//
+// A row's reference m is raised only when its maximum has grown by more than a factor 2^8 since (P stays below 2^8, rounded relative to
+// itself): O, in tensor memory, is then rescaled by the row's own thread.
+//
+// What is hidden must not reach the row, but P = 0 times NaN or infinity is NaN. In the iterations that a mask cuts (the diagonal, the end of the
+// keys) the softmax warps therefore look through V in shared memory; what is not finite is set to 0 there and added at the end, from global
+// memory, to the rows that do see it.
+#include "es_packed.cuh"
+#include "es_vsa_tc.cuh"
+
+namespace es {
+namespace packed {
+
+namespace {
+using vsa::pack2;
+using vsa::umma_idesc;
+using vsa::kNaN16x2;
+using vsa::kNaN32;
+
+constexpr int TM = 128, TN = 128, THREADS = 384;
+// Registers per thread: 168 at launch (three warps to a quarter of the SM), shared out anew: 224 + 224 + 56 = 3 * 168.
+constexpr int REGS_SOFTMAX = 224, REGS_REST = 56;
+constexpr uint32_t HALF = TM * 128;                          // 128 rows x 64 d, one swizzled box
+constexpr float RAISE = 8.f;                                 // log2 of the factor
+
+template <int D> struct Cfg {
+    static constexpr uint32_t TILE = TM * D * 2;             // [d half][128 rows][128 B]
+    static constexpr int NSLOT = D == 128 ? 5 : 10;
+    static constexpr uint32_t Q = 0, RING = 2 * TILE, CTL = RING + NSLOT * TILE, BYTES = CTL + 512;
+};
+struct Ctl {
+    uint64_t qfull[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain;
+    uint32_t tmem_base;
+    int abort, not_finite;
+    uint32_t seen[10];                                       // paged: a bit per page of the slot's tile that is one of the cache
+};
+static_assert(sizeof(Ctl) <= 512, "control block");
+
+struct FwdArgs {
+    Batch b;
+    int pack, tokens, splits;                                // heads per row group, tokens per 128 rows, CTAs that share a tile's keys
+    int vheads;                                              // kv_heads * (G / pack)
+    void* o;
+    float* lse;
+    float *part_o, *part_lse;                                // [split][token][head][D], log2-domain [split][token][head] (splits > 1)
+    const void* v;                                           // for what is not finite
+    Rows rv;
+    int* status;
+};
+
+// What a CTA does.
+struct Work {
+    int q0, n_tok;       // first token, tokens (up to two tiles)
+    int base, nk;        // token t sees keys 0 .. base + t (causal), 0 .. nk - 1
+    int k0;              // first key row
+    int i0, i1;          // its key tiles
+};
+
+__device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
+}  // namespace
+
+// The tile of grid slot x: pieces of the batch are what lies before the first sequence, the sequences, and what lies behind the last; piece i
+// starts at slot floor(start / span) + i, which leaves each piece at least ceil(length / span) slots without a sum over the lengths.
+// A warp searches 32 pieces at a time.
+__device__ __forceinline__ Work find_work(const FwdArgs& a, int x, int span, int lane) {
+    const int pieces = a.b.B + 2;
+    auto start = [&](int i) { return i == 0 ? 0 : a.b.q_at(i - 1); };
+    int lo = 0, n = pieces;
+    while (n > 1) {
+        const int step = (n + 31) >> 5, i = lo + lane * step;
+        const bool at = lane * step < n && start(i) / span + i <= x;
+        const int c = max(__popc(__ballot_sync(0xffffffffu, at)), 1) - 1;
+        n = min(step, n - c * step);
+        lo += c * step;
+    }
+    Work w{};
+    const int s = start(lo), e = lo + 1 < pieces ? start(lo + 1) : a.b.Tq, t = (x - (s / span + lo)) * span;
+    w.q0 = s + t;
+    w.n_tok = min(span, e - s - t);
+    if (lo >= 1 && lo <= a.b.B) {
+        w.k0 = a.b.k_at(lo - 1);
+        w.nk = max(a.b.k_at(lo) - w.k0, 0);
+        w.base = t + w.nk - (e - s);
+    }
+    return w;
+}
+
+template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {       // either of two packed values
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    return (w & E) == E || ((w >> 16) & E) == E;
+}
+template <typename T> __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    if ((w & E) == E) w &= 0xFFFF0000u;
+    if (((w >> 16) & E) == E) w &= 0xFFFFu;
+    return w;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ FwdArgs a) {
+    using C = Cfg<D>;
+    constexpr uint32_t O_COL = 256;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int wide = a.vheads * a.splits, hs = blockIdx.x % wide, vh = hs % a.vheads, split = hs / a.vheads, span = 2 * a.tokens;
+    const int per_kv = a.b.G / a.pack, kh = vh / per_kv, head0 = vh * a.pack;
+    Work w = find_work(a, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);       // the last tiles of a causal sequence see the most keys
+    if (w.n_tok <= 0) return;
+    // key tiles of the two row tiles
+    int n[2];
+    for (int s = 0; s < 2; ++s) {
+        const int last = min((s + 1) * a.tokens, w.n_tok) - 1;
+        n[s] = last >= s * a.tokens ? (seen_by(a, w, last) + TN - 1) / TN : 0;
+    }
+    const int all = max(n[0], n[1]);
+    w.i0 = (int)((int64_t)all * split / a.splits);
+    w.i1 = (int)((int64_t)all * (split + 1) / a.splits);
+    const int nt = w.i1 - w.i0;
+    const uint32_t base = smem_u32(smem);
+    Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
+    volatile int* abort_flag = &ctl->abort;
+    if (tid == 0) {
+        const int earlier = *reinterpret_cast<volatile int*>(a.status);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ctl->qfull[i]), 1);
+            mbar_init(smem_u32(&ctl->sfull[i]), 1);
+            mbar_init(smem_u32(&ctl->pfull[i]), 128);
+            mbar_init(smem_u32(&ctl->ofull[i]), 1);
+        }
+        for (int i = 0; i < C::NSLOT; ++i) {
+            mbar_init(smem_u32(&ctl->full[i]), 1);
+            mbar_init(smem_u32(&ctl->empty[i]), 1);
+        }
+        mbar_init(smem_u32(&ctl->drain), 1);
+        ctl->not_finite = 0;
+        ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
+        if (base & 1023u) atomicCAS(a.status, 0, 910);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
+    // iterations of tile s: i0 .. end(s) - 1
+    const int end0 = min(max(n[0], w.i0), w.i1), end1 = min(max(n[1], w.i0), w.i1);
+    uint32_t issued = 0;
+
+    if (warp >= 8) {
+    reg_dec<REGS_REST>();
+    if (warp == 9) {
+        // ------------------------------------------------------------ loads: Q, then K(i), V(i) for every i
+        bool ok = *abort_flag == 0;
+        if (lane == 0 && ok && nt > 0) {
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            const uint32_t qbytes = (uint32_t)(a.tokens * a.pack * D * 2);
+            for (int s = 0; s < 2; ++s) {
+                if ((s ? end1 : end0) <= w.i0) continue;     // nobody would wait for it
+                mbar_arrive_expect_tx(smem_u32(&ctl->qfull[s]), qbytes);
+                for (int d = 0; d < D / 64; ++d)
+                    tma_load_3d(base + C::Q + s * C::TILE + d * HALF, &tmQ, smem_u32(&ctl->qfull[s]), 64 * d, head0, w.q0 + s * a.tokens);
+            }
+            uint32_t slot = 0, par = 1;
+            for (int i = w.i0; i < w.i1 && ok; ++i)
+                for (int x = 0; x < 2 && ok; ++x) {
+                    ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 601);
+                    if (!ok) break;
+                    const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                    mbar_arrive_expect_tx(bar, C::TILE);
+                    for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.k0 + i * TN);
+                    ++issued;
+                    if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+                }
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------------------ MMAs
+        constexpr uint32_t ID_QK = umma_idesc<T>(128, TN, 0, 0), ID_PV = umma_idesc<T>(128, D, 0, 1);
+        const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dv0 = umma_desc_sw128(0, HALF, 1024);
+        const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, v_hi = (uint32_t)(dv0 >> 32), v_lo = (uint32_t)dv0;
+        bool ok = *abort_flag == 0;
+        auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
+        auto take = [&](int seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 603); };
+        auto issue_qk = [&](int s, int seq) {
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t qa = k_lo + ((base + C::Q + s * C::TILE) >> 4), kb = k_lo + ((base + C::RING + slot_of(seq) * C::TILE) >> 4);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                    umma_ss_lohi(tmem + s * 128, qa + off, k_hi, kb + off, k_hi, ID_QK, ks > 0);
+                }
+                umma_commit(smem_u32(&ctl->sfull[s]));
+            }
+            __syncwarp();
+        };
+        auto release = [&](int seq) {
+            if (elect_one()) umma_commit(empty0 + 8 * slot_of(seq));
+            __syncwarp();
+        };
+        const int end[2] = {end0, end1};
+        if (nt > 0 && ok) {
+            take(0);
+            for (int s = 0; s < 2; ++s)
+                if (end[s] > w.i0) {
+                    ok = ok && mbar_wait_warp(smem_u32(&ctl->qfull[s]), 0, abort_flag, a.status, 602);
+                    if (ok) issue_qk(s, 0);
+                }
+            if (ok) release(0);
+        }
+        for (int i = 0; i < nt && ok; ++i) {
+            const int vseq = 2 * i + 1, kseq = 2 * i + 2;
+            bool v_in = false, k_in = false;
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s) {
+                if (w.i0 + i >= end[s]) continue;
+                if (!v_in) { take(vseq); v_in = true; }
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->pfull[s]), i & 1, abort_flag, a.status, 604);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t vb = v_lo + ((base + C::RING + slot_of(vseq) * C::TILE) >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_ts_lohi(tmem + O_COL + s * D, tmem + s * 128 + ks * 8, vb + ((ks * 2048) >> 4), v_hi, ID_PV, (i > 0 || ks > 0) ? 1u : 0u);
+                    if (w.i0 + i + 1 == end[s]) umma_commit(smem_u32(&ctl->ofull[s]));
+                }
+                __syncwarp();
+                if (w.i0 + i + 1 < end[s]) {
+                    if (!k_in) { take(kseq); k_in = true; }
+                    if (!ok) break;
+                    issue_qk(s, kseq);                       // P of this tile has been read by then: MMAs run in their order
+                }
+            }
+            if (!ok) break;
+            release(vseq);
+            if (i + 1 < nt) release(kseq);
+        }
+        // every MMA issued above has finished before tensor memory is freed
+        if (elect_one()) umma_commit(smem_u32(&ctl->drain));
+        __syncwarp();
+        mbar_wait(smem_u32(&ctl->drain), 0, abort_flag, a.status, 606);
+    }
+    } else {
+        // ------------------------------------------------------------ softmax and epilogue
+        reg_inc<REGS_SOFTMAX>();
+        const int s = warp >> 2, r = tid & 127;
+        const int tok = s * a.tokens + r / a.pack, head = head0 + r % a.pack;
+        const bool valid = r / a.pack < a.tokens && tok < w.n_tok;
+        const int vis = valid ? seen_by(a, w, tok) : 0;
+        const int whole = seen_by(a, w, s * a.tokens) / TN;  // tiles before this one are seen by every row (its first sees the fewest keys)
+        const int end = s ? end1 : end0;
+        const uint32_t scol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + s * 128, ocol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + O_COL + s * D;
+        const float c = a.b.scale * kLog2e;
+        float m = -INFINITY, l = 0.f;
+        bool ok = *abort_flag == 0;
+        for (int i = w.i0; i < end && ok; ++i) {
+            const int it = i - w.i0;
+            ok = mbar_wait_warp(smem_u32(&ctl->sfull[s]), it & 1, abort_flag, a.status, 607);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t x[128];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_ld32(scol + 32 * j, x + 32 * j);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_wait_ld_regs(x + 32 * j);
+            if (i >= whole) {
+                const int lim = vis - i * TN;
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    if (j >= lim) x[j] = 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < TN; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[j]));
+            const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+            const bool raise = m == -INFINITY ? y > -INFINITY : y > m + RAISE;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float next = raise ? y : m, shrink = raise ? (m == -INFINITY ? 0.f : ex2_approx(m - next)) : 1.f;
+                m = next;
+                l *= shrink;
+                if (it > 0) {
+                    // (P V of the iteration before was issued before this S: it has written O)
+#pragma unroll 1
+                    for (int h = 0; h < D / 32; ++h) {
+                        uint32_t o[32];
+                        tmem_ld32(ocol + 32 * h, o);
+                        tmem_wait_ld_regs(o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                        tmem_st32(ocol + 32 * h, o);
+                    }
+                }
+            }
+            const float off = m == -INFINITY ? 0.f : -m;
+            const float2 cc = make_float2(c, c), oo = make_float2(off, off);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t p[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), cc, oo);
+                    const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                    sum = __fadd2_rn(sum, e);
+                    p[j] = pack2<T>(e.x, e.y);
+                }
+                tmem_st32(scol + 32 * h, p);
+            }
+            l += sum.x + sum.y;
+            if (i >= whole) {
+                // V rows that some rows of the tile may not see
+                const int vseq = 2 * it + 1;
+                const uint32_t slot = (uint32_t)vseq % C::NSLOT;
+                ok = mbar_wait_warp(full0 + 8 * slot, ((uint32_t)vseq / C::NSLOT) & 1, abort_flag, a.status, 608);
+                if (!ok) break;
+                uint8_t* row = smem + C::RING + slot * C::TILE + r * 128;
+                bool any = false;
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+                    for (int ch = 0; ch < 8; ++ch) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(row + d * HALF + 16 * (ch ^ (r & 7)));
+                        any |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+                    }
+                if (any) {
+                    for (int d = 0; d < D / 64; ++d)
+                        for (int ch = 0; ch < 8; ++ch) {
+                            uint4* v = reinterpret_cast<uint4*>(row + d * HALF + 16 * ch);
+                            *v = make_uint4(finite_only<T>(v->x), finite_only<T>(v->y), finite_only<T>(v->z), finite_only<T>(v->w));
+                        }
+                    *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
+                }
+                fence_proxy_async_smem();
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctl->pfull[s]));
+        }
+        if (end > w.i0) ok = ok && mbar_wait_warp(smem_u32(&ctl->ofull[s]), 0, abort_flag, a.status, 609);
+        if (ok) {
+            tc_fence_after();
+            const bool any = end > w.i0;
+            const float inv = l != 0.f ? 1.f / l : 0.f;      // 0: a row without a key; NaN stays NaN
+            const bool fix = any && *reinterpret_cast<volatile int*>(&ctl->not_finite) != 0;
+            const int64_t row = (int64_t)(w.q0 + tok) * a.b.H + head;
+            const int from = max(w.i0, min(seen_by(a, w, 0), seen_by(a, w, min(a.tokens, w.n_tok - 1))) / TN) * TN, to = min(vis, w.i1 * TN);
+#pragma unroll 1
+            for (int h = 0; h < D / 32; ++h) {
+                uint32_t o[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = 0;
+                if (any) {
+                    tmem_ld32(ocol + 32 * h, o);
+                    tmem_wait_ld_regs(o);
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l != 0.f ? __uint_as_float(o[j]) * inv : 0.f);
+                if (fix && valid) {
+                    for (int k = from; k < to; ++k) {
+                        const T* vr = static_cast<const T*>(a.v) + (int64_t)(w.k0 + k) * a.rv.token + (int64_t)kh * a.rv.head + 32 * h;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float e = to_float(vr[j]);
+                            if (!(fabsf(e) < INFINITY)) o[j] = __float_as_uint(__uint_as_float(o[j]) + e);
+                        }
+                    }
+                }
+                if (!valid) continue;
+                if (a.splits > 1) {
+                    float4* dst = reinterpret_cast<float4*>(a.part_o + ((int64_t)split * a.b.Tq * a.b.H + row) * D + 32 * h);
+                    if (any)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D + 32 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        dst[j] = make_uint4(pack2<T>(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1])), pack2<T>(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3])),
+                                            pack2<T>(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5])), pack2<T>(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7])));
+                }
+            }
+            if (valid) {
+                const float z = l != 0.f ? m + log2f(l) : -INFINITY;
+                if (a.splits > 1) a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = z;
+                else a.lse[(int64_t)head * a.b.Tq + w.q0 + tok] = z * kLn2;
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    if (warp == 9 && lane == 0 && *abort_flag) {
+        // a wait gave up: give the loads a moment (100 us in all) to land before shared memory goes away
+        const uint64_t t_end = global_timer_ns() + 100000ull;
+        for (int s = 0; s < 2; ++s)
+            while (issued && (s ? end1 : end0) > w.i0 && !mbar_try_wait(smem_u32(&ctl->qfull[s]), 0) && global_timer_ns() < t_end) {}
+        for (uint32_t back = 1; back <= (uint32_t)C::NSLOT && back <= issued; ++back) {
+            const uint32_t sq = issued - back;
+            while (!mbar_try_wait(full0 + 8 * (sq % C::NSLOT), (sq / C::NSLOT) & 1) && global_timer_ns() < t_end) {}
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (*abort_flag) {
+        // NaN in all that the CTA owns: the caller's memory is not initialised
+        for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
+            const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head0 + e % a.pack;
+            if (a.splits > 1) {
+                a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = __uint_as_float(kNaN32);
+                for (int d = 0; d < D; ++d) a.part_o[((int64_t)split * a.b.Tq * a.b.H + row) * D + d] = __uint_as_float(kNaN32);
+            } else {
+                a.lse[(int64_t)(head0 + e % a.pack) * a.b.Tq + w.q0 + e / a.pack] = __uint_as_float(kNaN32);
+                for (int d = 0; d < D / 2; ++d) reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D)[d] = kNaN16x2;
+            }
+        }
+    }
+}
+
+// o = sum_p 2^(z_p - M) o_p / sum_p 2^(z_p - M), a warp per row; parts without a key (z = -inf) were not written and are not read.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) merge_kernel(const float* part_o, const float* part_lse, T* o, float* lse, int parts, int Tq, int H) {
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = (int64_t)Tq * H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    float top = -INFINITY;
+    bool nan = false;
+    for (int p = lane; p < parts; p += 32) {
+        const float z = part_lse[p * rows + row];
+        nan |= z != z;
+        top = fmaxf(top, z);
+    }
+    for (int i = 16; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    constexpr int C = D / 32;
+    float acc[C] = {}, sum = 0.f;
+    for (int p = 0; p < parts; ++p) {
+        const float z = part_lse[p * rows + row];
+        if (z == -INFINITY) continue;
+        const float w = exp2f(z - top);
+        sum += w;
+        const float* src = part_o + (p * rows + row) * D + C * lane;
+        if constexpr (C == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            acc[0] += w * v.x; acc[1] += w * v.y; acc[2] += w * v.z; acc[3] += w * v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            acc[0] += w * v.x; acc[1] += w * v.y;
+        }
+    }
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c)
+        reinterpret_cast<uint32_t*>(o + row * D + C * lane)[c] = pack2<T>(sum != 0.f ? acc[2 * c] * inv : 0.f, sum != 0.f ? acc[2 * c + 1] * inv : 0.f);
+    if (lane == 0) lse[(row % H) * Tq + row / H] = sum != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+// Query heads that share a tile's rows: the most heads of a group (a divisor of it) that still fill 15 of 16 rows. More heads make the tile
+// shorter in tokens; the rows lost are computed for nothing.
+int rows_pack(int G) {
+    for (int d = min(G, TM); d > 1; --d)
+        if (G % d == 0 && TM / d * d >= TM - TM / 16) return d;
+    return 1;
+}
+
+template <typename T> static int make_rows_map(CUtensorMap* m, const void* ptr, int D, int heads, long long tokens, Rows r, int box_heads, int box_tokens) {
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens};
+    cuuint64_t str[2] = {(cuuint64_t)r.head * 2, (cuuint64_t)r.token * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return encode_tensor_map(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                             const_cast<void*>(ptr), dims, str, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int D>
+static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, FwdArgs a, cudaStream_t st) {
+    CUtensorMap tq, tk, tv;
+    // (a batch without keys loads none, but a map needs an extent)
+    const long long tk_rows = a.b.Tk ? a.b.Tk : a.b.Tq;
+    if (!a.b.Tk) { k = v = q; rk = rv = rq; }
+    if (int rc = make_rows_map<T>(&tq, q, D, a.b.H, a.b.Tq, rq, a.pack, a.tokens)) return rc;
+    if (int rc = make_rows_map<T>(&tk, k, D, a.b.Hk, tk_rows, rk, 1, TN)) return rc;
+    if (int rc = make_rows_map<T>(&tv, v, D, a.b.Hk, tk_rows, rv, 1, TN)) return rc;
+    auto kern = packed_fwd_kernel<T, D>;
+    if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
+    const int64_t grid = (int64_t)a.vheads * a.splits * (a.b.Tq / (2 * a.tokens) + a.b.B + 2);
+    if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_fwd: too many tiles");
+    kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
+    ES_CHECK_LAUNCH("packed_fwd_kernel");
+    if (a.splits > 1) {
+        merge_kernel<T, D><<<(unsigned)(((int64_t)a.b.Tq * a.b.H + 7) / 8), 256, 0, st>>>(a.part_o, a.part_lse, static_cast<T*>(a.o), a.lse, a.splits, a.b.Tq, a.b.H);
+        ES_CHECK_LAUNCH("merge_kernel");
+    }
+    return 0;
+}
+
+// The caller has checked sizes and pointers.
+int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, float* lse, const Batch& b, int D, int dtype, void* ws,
+                  cudaStream_t st) {
+    (void)ws;
+    FwdArgs a{};
+    a.b = b;
+    a.pack = rows_pack(b.G);
+    a.tokens = TM / a.pack;
+    a.splits = 1;
+    a.vheads = b.H / a.pack;
+    a.o = o;
+    a.lse = lse;
+    a.v = v;
+    a.rv = rv;
+    a.status = device_status_ptr();
+    if (!a.status) return set_error(-2, "es_packed_attn_fwd: the device status word is not available on this device");
+    if (D == 64)
+        return dtype == 0 ? launch<__nv_bfloat16, 64>(q, rq, k, rk, v, rv, a, st) : launch<__half, 64>(q, rq, k, rk, v, rv, a, st);
+    return dtype == 0 ? launch<__nv_bfloat16, 128>(q, rq, k, rk, v, rv, a, st) : launch<__half, 128>(q, rq, k, rk, v, rv, a, st);
+}
+
+}  // namespace packed
+}  // namespace es

@@ -131,6 +131,11 @@ __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
+// ---------------------------------------------------------------- registers of a warpgroup
+// What the inc's of a block's warpgroups take must be what its dec's gave, of the registers the block was launched with.
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---------------------------------------------------------------- programmatic dependent launch
 // A kernel started with launch_dependent (es_api_internal.h) may begin while the one before it on the stream still runs; past this
 // wait the earlier kernel, and all that it wrote, is complete.
