@@ -74,8 +74,8 @@ SIGNATURES = {
     "es_vsa_tier_rep_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "es_vsa_tier_unpool": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "es_packed_workspace_bytes": [_I] * 6,
-    "es_packed_attn_fwd": [_P] * 7 + [_I] * 6 + [_I64] * 6 + [_F, _I, _I, _P, _P],
-    "es_packed_delta": [_P, _P, _P, _I, _I, _I, _I64, _I64, _I, _P],
+    "es_packed_attn_fwd": [_P] * 8 + [_I] * 6 + [_I64] * 6 + [_F, _I, _I, _P, _P],
+    "es_packed_delta": [_P, _P, _P, _P, _I, _I, _I, _I64, _I64, _I, _P],
     "es_packed_attn_bwd_q": [_P] * 9 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
     "es_packed_attn_bwd_kv": [_P] * 10 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
     "es_prefix_workspace_bytes": [_I] * 8,

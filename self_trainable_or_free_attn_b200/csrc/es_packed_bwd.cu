@@ -1,0 +1,663 @@
+// Backward attention of packed sequences on the 5th-generation tensor cores, in two passes with one owner per output row: no atomics, the
+// same inputs give the same bits.
+//
+//   P = exp(scale Q K^T - LSE), dS = P o (dO V^T - delta)
+//   dK / dV pass: a CTA owns 128 keys and walks the query rows that see them, 128 (token, head) rows of all heads of the key's group at a time:
+//                 S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   dQ pass:      a CTA owns 128 (token, head) rows and walks their keys, 128 at a time: S = Q K^T, dP = dO V^T, dQ += dS K
+// P and dS are written over S and dP in tensor memory, as 16-bit pairs, and are the A operands of the second products from there. (One
+// pass instead would save two of seven products, S and dP again, and need dQ added with atomics in the order in which CTAs happen to run.)
+//
+//   warps 0-7  P and dS: a thread has row 32 (warp % 4) + lane and 64 columns, those of warps 4-7 the upper half
+//   warp 8     issues the MMAs; warp 9 issues the TMA loads; warp 10 (dK / dV) brings LSE and delta of the walked rows
+//
+// What a mask hides, or what lies in the walked tile behind the sequence, has P = dS = 0, and 0 times NaN or infinity would be NaN: in tiles
+// that a mask cuts, values of the walked tiles that are not finite are set to 0 in shared memory once S and dP are there. dS is NaN already
+// where they are seen; dV alone gets what is not finite in dO at the end, from global memory.
+#include "es_packed_tc.cuh"
+
+namespace es {
+namespace packed {
+
+namespace {
+template <int D> struct Cfg {
+    static constexpr uint32_t TILE = TM * D * 2;             // [d half][128 rows][128 B]
+    static constexpr int NSLOT = D == 128 ? 5 : 10;
+    static constexpr uint32_t Y1 = 0, Y2 = TILE, RING = 2 * TILE, ROWS = RING + NSLOT * TILE;
+    static constexpr int NROW = 2;                           // stages of LSE and delta
+    static constexpr uint32_t CTL = ROWS + NROW * 2 * TM * 4, BYTES = CTL + 512;
+};
+static_assert(Cfg<128>::BYTES <= 232448, "shared memory");
+struct Ctl {
+    uint64_t yfull, full[10], empty[10], sfull[2], dpfull, pfull, dsfull, rfull[2], rempty[2], gfull, drain;
+    uint32_t tmem_base;
+    int abort, not_finite;
+};
+static_assert(sizeof(Ctl) <= 512, "control block");
+
+struct BwdArgs {
+    Batch b;
+    int pack, tokens;                                        // heads per row group, tokens per 128 rows
+    const float *lse, *delta;
+    void *d0, *d1;                                           // dQ, or dK and dV
+    const void* dout;                                        // for what is not finite
+    Rows rdo;
+    int* status;
+};
+
+// Row r of the tile at `tile`, its values that are not finite set to 0; whether there were any.
+template <typename T, int D> __device__ __forceinline__ bool clean_row(uint8_t* tile, int r) {
+    uint8_t* row = tile + r * 128;
+    bool any = false;
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + d * HALF + 16 * (ch ^ (r & 7)));
+            any |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
+        }
+    if (any) {
+        for (int d = 0; d < D / 64; ++d)
+            for (int ch = 0; ch < 8; ++ch) {
+                uint4* v = reinterpret_cast<uint4*>(row + d * HALF + 16 * ch);
+                *v = make_uint4(finite_only<T>(v->x), finite_only<T>(v->y), finite_only<T>(v->z), finite_only<T>(v->w));
+            }
+    }
+    return any;
+}
+
+template <typename T, int D> __device__ __forceinline__ void store_row(T* dst, uint32_t tcol, int from, int to, bool any, bool valid, float factor) {
+#pragma unroll 1
+    for (int h = from; h < to; ++h) {
+        uint32_t g[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) g[j] = 0;
+        if (any) {
+            tmem_ld32(tcol + 32 * h, g);
+            tmem_wait_ld_regs(g);
+        }
+        if (!valid) continue;
+        uint4* out = reinterpret_cast<uint4*>(dst + 32 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t p[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) p[x] = pack2<T>(__uint_as_float(g[8 * j + 2 * x]) * factor, __uint_as_float(g[8 * j + 2 * x + 1]) * factor);
+            out[j] = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+    }
+}
+
+// The wait of a CTA that gives up for the loads in flight (100 us in all), before shared memory goes away.
+template <int NSLOT> __device__ __forceinline__ void land(Ctl* ctl, uint32_t issued) {
+    const uint64_t t_end = global_timer_ns() + 100000ull;
+    while (issued && !mbar_try_wait(smem_u32(&ctl->yfull), 0) && global_timer_ns() < t_end) {}
+    for (uint32_t back = 1; back <= (uint32_t)NSLOT && back <= issued; ++back) {
+        const uint32_t sq = issued - back;
+        while (!mbar_try_wait(smem_u32(&ctl->full[sq % NSLOT]), (sq / NSLOT) & 1) && global_timer_ns() < t_end) {}
+    }
+}
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------- dK, dV
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ BwdArgs a) {
+    using C = Cfg<D>;
+    constexpr uint32_t DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int kh = blockIdx.x % a.b.Hk;
+    // (the first keys of a causal sequence are seen by the most queries)
+    const Piece at = find_piece(a.b.cu_k, a.b.B, a.b.Tk, blockIdx.x / a.b.Hk, TN, lane);
+    if (at.n <= 0) return;
+    int q0 = 0, nq = 0, diag = 0, first = 0;                 // diag: query t sees the owner's keys 0 .. t + diag
+    if (at.seq >= 0) {
+        q0 = a.b.q_at(at.seq);
+        nq = max(a.b.q_at(at.seq + 1) - q0, 0);
+        diag = a.b.causal ? at.length - nq - at.offset : TN;
+        first = min(max(-diag, 0), nq);                      // the first query that sees one of them
+    }
+    const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens, nt = subs * per;
+    const uint32_t base = smem_u32(smem);
+    Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
+    volatile int* abort_flag = &ctl->abort;
+    if (tid == 0) {
+        const int earlier = *reinterpret_cast<volatile int*>(a.status);
+        mbar_init(smem_u32(&ctl->yfull), 1);
+        for (int i = 0; i < C::NSLOT; ++i) {
+            mbar_init(smem_u32(&ctl->full[i]), 1);
+            mbar_init(smem_u32(&ctl->empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ctl->sfull[i]), 1);
+            mbar_init(smem_u32(&ctl->rfull[i]), 32);
+            mbar_init(smem_u32(&ctl->rempty[i]), 256);
+        }
+        mbar_init(smem_u32(&ctl->dpfull), 1);
+        mbar_init(smem_u32(&ctl->pfull), 256);
+        mbar_init(smem_u32(&ctl->dsfull), 256);
+        mbar_init(smem_u32(&ctl->gfull), 1);
+        mbar_init(smem_u32(&ctl->drain), 1);
+        ctl->not_finite = 0;
+        ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
+        if (base & 1023u) atomicCAS(a.status, 0, 911);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    // rows of the ring's tiles that no load writes (128 is not a multiple of the heads) take part in the products, times 0
+    const int loaded = a.tokens * a.pack;
+    if (loaded < TM) {
+        const int chunks = (TM - loaded) * 8, all = chunks * (D / 64) * C::NSLOT;
+        for (int e = tid; e < all; e += THREADS) {
+            const int t = e / chunks, c = e % chunks;        // t: (slot, d half)
+            *reinterpret_cast<uint4*>(smem + C::RING + t * HALF + loaded * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
+    float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then delta
+    float* row_delta = row_lse + C::NROW * TM;
+    uint32_t issued = 0;
+    // walked tile i: query heads head0 .., first token
+    auto head_of = [&](int i) { return kh * a.b.G + (i / per) * a.pack; };
+    auto token_of = [&](int i) { return first + (i % per) * a.tokens; };
+
+    if (warp >= 8) {
+        reg_dec<REGS_REST>();
+        bool ok = *abort_flag == 0;
+        if (warp == 9) {
+            // -------------------------------------------------------- loads: K, V, then Q(i), dO(i)
+            if (lane == 0 && ok && nt > 0) {
+                mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * C::TILE);
+                for (int d = 0; d < D / 64; ++d) {
+                    tma_load_3d(base + C::Y1 + d * HALF, &tmK, smem_u32(&ctl->yfull), 64 * d, kh, at.first);
+                    tma_load_3d(base + C::Y2 + d * HALF, &tmV, smem_u32(&ctl->yfull), 64 * d, kh, at.first);
+                }
+                const uint32_t bytes = (uint32_t)(loaded * D * 2);
+                uint32_t slot = 0, par = 1;
+                for (int i = 0; i < nt && ok; ++i)
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 621);
+                        if (!ok) break;
+                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                        mbar_arrive_expect_tx(bar, bytes);
+                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmDO : &tmQ, bar, 64 * d, head_of(i), q0 + token_of(i));
+                        ++issued;
+                        if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+                    }
+            }
+        } else if (warp == 10) {
+            // -------------------------------------------------------- LSE and delta of tile i, once tile i - 2's have been read
+            for (int i = 0; i < nt && ok; ++i) {
+                float l[4], d[4];
+                const int h0 = head_of(i), t0 = token_of(i);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = lane + 32 * x, t = t0 + r / a.pack;
+                    const bool valid = r < loaded && t < nq;
+                    const int64_t g = (int64_t)(h0 + r % a.pack) * a.b.Tq + q0 + t;
+                    const float z = valid ? __ldg(a.lse + g) : -INFINITY;
+                    l[x] = z == -INFINITY ? -INFINITY : -z * kLog2e;       // (added to the logit: P of a row without keys, or of none, is 0)
+                    d[x] = valid ? __ldg(a.delta + g) : 0.f;
+                }
+                ok = mbar_wait_warp(smem_u32(&ctl->rempty[i % C::NROW]), ((i / C::NROW) & 1) ^ 1, abort_flag, a.status, 622);
+                if (!ok) break;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    row_lse[(i % C::NROW) * TM + lane + 32 * x] = l[x];
+                    row_delta[(i % C::NROW) * TM + lane + 32 * x] = d[x];
+                }
+                mbar_arrive(smem_u32(&ctl->rfull[i % C::NROW]));
+            }
+        } else if (warp == 8) {
+            // -------------------------------------------------------- MMAs
+            constexpr uint32_t ID_S = umma_idesc<T>(128, TM, 0, 0), ID_G = umma_idesc<T>(128, D, 0, 1);
+            const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dx0 = umma_desc_sw128(0, HALF, 1024);
+            const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, x_hi = (uint32_t)(dx0 >> 32), x_lo = (uint32_t)dx0;
+            auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
+            auto take = [&](int seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 623); };
+            auto first_product = [&](int x, int i) {         // x = 0: S(i) = K Q^T, x = 1: dP(i) = V dO^T
+                take(2 * i + x);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t ya = k_lo + ((base + (x ? C::Y2 : C::Y1)) >> 4), xb = k_lo + ((base + C::RING + slot_of(2 * i + x) * C::TILE) >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                        umma_ss_lohi(tmem + x * DP_COL, ya + off, k_hi, xb + off, k_hi, ID_S, ks > 0);
+                    }
+                    umma_commit(x ? smem_u32(&ctl->dpfull) : smem_u32(&ctl->sfull[0]));
+                }
+                __syncwarp();
+            };
+            auto second_product = [&](int x, int i) {        // x = 0: dK += dS^T Q, x = 1: dV += P^T dO
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * i + x) * C::TILE) >> 4), p = tmem + (x ? 0u : DP_COL);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_ts_lohi(tmem + (x ? DV_COL : DK_COL), p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G,
+                                     (i > 0 || ks > 0) ? 1u : 0u);
+                    umma_commit(empty0 + 8 * slot_of(2 * i + x));
+                }
+                __syncwarp();
+            };
+            if (nt > 0) {
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), 0, abort_flag, a.status, 624);
+                if (ok) first_product(0, 0);
+                if (ok) first_product(1, 0);
+            }
+            for (int i = 0; i < nt && ok; ++i) {
+                ok = mbar_wait_warp(smem_u32(&ctl->pfull), i & 1, abort_flag, a.status, 625);
+                if (!ok) break;
+                second_product(1, i);
+                if (i + 1 < nt) first_product(0, i + 1);     // (over P, which dV has read: MMAs run in their order)
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), i & 1, abort_flag, a.status, 626);
+                if (!ok) break;
+                second_product(0, i);
+                if (i + 1 < nt) first_product(1, i + 1);
+            }
+            if (ok && nt > 0 && elect_one()) umma_commit(smem_u32(&ctl->gfull));
+            __syncwarp();
+            // every MMA issued above has finished before tensor memory is freed
+            if (elect_one()) umma_commit(smem_u32(&ctl->drain));
+            __syncwarp();
+            mbar_wait(smem_u32(&ctl->drain), 0, abort_flag, a.status, 627);
+        }
+    } else {
+        // ------------------------------------------------------------ P, dS and epilogue
+        reg_inc<REGS_MATH>();
+        const int r = tid & 127, ch = warp >> 2;             // key row, half of the columns
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16), scol = tl + 64 * ch, dpcol = tl + DP_COL + 64 * ch;
+        const float c = a.b.scale * kLog2e;
+        bool ok = *abort_flag == 0;
+        for (int i = 0; i < nt && ok; ++i) {
+            const int t0 = token_of(i);
+            // the first of the tile's tokens sees the fewest keys; the rows behind the last token are of other sequences
+            const bool cut = t0 + diag < at.n - 1, masked = cut || t0 + a.tokens > nq;
+            ok = mbar_wait_warp(smem_u32(&ctl->rfull[i % C::NROW]), (i / C::NROW) & 1, abort_flag, a.status, 628) &&
+                 mbar_wait_warp(smem_u32(&ctl->sfull[0]), i & 1, abort_flag, a.status, 629);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t x[64];
+            tmem_ld32(scol, x);
+            tmem_ld32(scol + 32, x + 32);
+            tmem_wait_ld_regs(x);
+            tmem_wait_ld_regs(x + 32);
+            const float4* rl = reinterpret_cast<const float4*>(row_lse + (i % C::NROW) * TM + 64 * ch);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float4 z = rl[j];
+                x[4 * j] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j]), c, z.x)));
+                x[4 * j + 1] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 1]), c, z.y)));
+                x[4 * j + 2] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 2]), c, z.z)));
+                x[4 * j + 3] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 3]), c, z.w)));
+            }
+            const int lim = cut ? max(r - diag - t0, 0) * a.pack - 64 * ch : 0;      // columns before it do not see the key
+            if (masked) {
+                // columns that are not rows of the sequence have an offset of -inf: P is 0 unless their logit is not finite
+                const int end = min(loaded, (nq - t0) * a.pack) - 64 * ch;
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                    if (j < lim || j >= end) x[j] = 0;
+            }
+            {
+                uint32_t p[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) p[j] = pack2<T>(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                tmem_st32(scol, p);
+            }
+            if (masked) {
+                // dP of this tile is there too: from here on its Q and dO are read by the second products only
+                ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 630);
+                if (!ok) break;
+                const uint32_t slot = (uint32_t)(2 * i + ch) % C::NSLOT;             // half of the threads Q, half dO
+                if (clean_row<T, D>(smem + C::RING + slot * C::TILE, r)) *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
+                fence_proxy_async_smem();
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctl->pfull));
+            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 631);
+            if (!ok) break;
+            tc_fence_after();
+            const float4* rd = reinterpret_cast<const float4*>(row_delta + (i % C::NROW) * TM + 64 * ch);
+            uint32_t ds[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t y[32];
+                tmem_ld32(dpcol + 32 * h, y);
+                tmem_wait_ld_regs(y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float4 z = rd[8 * h + j];
+                    const uint32_t* xp = x + 32 * h + 4 * j;
+                    float g0 = __uint_as_float(xp[0]) * (__uint_as_float(y[4 * j]) - z.x), g1 = __uint_as_float(xp[1]) * (__uint_as_float(y[4 * j + 1]) - z.y);
+                    float g2 = __uint_as_float(xp[2]) * (__uint_as_float(y[4 * j + 2]) - z.z), g3 = __uint_as_float(xp[3]) * (__uint_as_float(y[4 * j + 3]) - z.w);
+                    if (masked) {                            // (0 times what a hidden row holds)
+                        const int k = 32 * h + 4 * j, end = min(loaded, (nq - t0) * a.pack) - 64 * ch;
+                        if (k < lim || k >= end) g0 = 0.f;
+                        if (k + 1 < lim || k + 1 >= end) g1 = 0.f;
+                        if (k + 2 < lim || k + 2 >= end) g2 = 0.f;
+                        if (k + 3 < lim || k + 3 >= end) g3 = 0.f;
+                    }
+                    ds[16 * h + 2 * j] = pack2<T>(g0, g1);
+                    ds[16 * h + 2 * j + 1] = pack2<T>(g2, g3);
+                }
+            }
+            mbar_arrive(smem_u32(&ctl->rempty[i % C::NROW]));
+            tmem_st32(dpcol, ds);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctl->dsfull));
+        }
+        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 632);
+        if (ok) {
+            tc_fence_after();
+            const int64_t row = (int64_t)(at.first + r) * a.b.Hk + kh;
+            const bool valid = r < at.n;
+            // warps 0-3 write dV, warps 4-7 dK
+            T* dst = static_cast<T*>(ch ? a.d0 : a.d1) + row * D;
+            store_row<T, D>(dst, tl + (ch ? DK_COL : DV_COL), 0, D / 32, nt > 0, valid, ch ? a.b.scale : 1.f);
+            if (ch == 0 && valid && nt > 0 && *reinterpret_cast<volatile int*>(&ctl->not_finite)) {
+                // what is not finite in dO of the rows of cut tiles that see this key
+                for (int i = 0; i < nt; ++i) {
+                    const int t0 = token_of(i);
+                    if (!(t0 + diag < at.n - 1 || t0 + a.tokens > nq)) continue;
+                    for (int t = max(t0, r - diag); t < min(t0 + a.tokens, nq); ++t)
+                        for (int h = head_of(i); h < head_of(i) + a.pack; ++h) {
+                            const T* src = static_cast<const T*>(a.dout) + (int64_t)(q0 + t) * a.rdo.token + (int64_t)h * a.rdo.head;
+                            for (int d = 0; d < D; ++d) {
+                                const float e = to_float(src[d]);
+                                if (!(fabsf(e) < INFINITY)) dst[d] = from_float<T>(to_float(dst[d]) + e);
+                            }
+                        }
+                }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, issued);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (*abort_flag)
+        for (int e = tid; e < at.n * (D / 2); e += THREADS) {
+            const int64_t w = ((int64_t)(at.first + e / (D / 2)) * a.b.Hk + kh) * (D / 2) + e % (D / 2);
+            static_cast<uint32_t*>(a.d0)[w] = static_cast<uint32_t*>(a.d1)[w] = kNaN16x2;
+        }
+}
+
+// ---------------------------------------------------------------------------------------------- dQ
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ BwdArgs a) {
+    using C = Cfg<D>;
+    constexpr uint32_t DP_COL = 256, DQ_COL = 384;           // S of even and of odd tiles: columns 0 and 128
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int vheads = a.b.H / a.pack, vh = blockIdx.x % vheads, head0 = vh * a.pack, kh = head0 / a.b.G;
+    const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / vheads - 1 - blockIdx.x / vheads, a.tokens, lane);
+    if (at.n <= 0) return;
+    int k0 = 0, nk = 0, diag = 0;                            // token t of the span sees keys 0 .. t + diag
+    if (at.seq >= 0) {
+        k0 = a.b.k_at(at.seq);
+        nk = max(a.b.k_at(at.seq + 1) - k0, 0);
+        diag = nk - at.length + at.offset;
+    }
+    auto seen_by = [&](int t) { return a.b.causal ? min(max(t + diag + 1, 0), nk) : nk; };
+    const int nt = (seen_by(at.n - 1) + TN - 1) / TN, whole = seen_by(0) / TN;
+    const uint32_t base = smem_u32(smem);
+    Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
+    volatile int* abort_flag = &ctl->abort;
+    if (tid == 0) {
+        const int earlier = *reinterpret_cast<volatile int*>(a.status);
+        mbar_init(smem_u32(&ctl->yfull), 1);
+        for (int i = 0; i < C::NSLOT; ++i) {
+            mbar_init(smem_u32(&ctl->full[i]), 1);
+            mbar_init(smem_u32(&ctl->empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctl->sfull[i]), 1);
+        mbar_init(smem_u32(&ctl->dpfull), 1);
+        mbar_init(smem_u32(&ctl->dsfull), 256);
+        mbar_init(smem_u32(&ctl->gfull), 1);
+        mbar_init(smem_u32(&ctl->drain), 1);
+        ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
+        if (base & 1023u) atomicCAS(a.status, 0, 912);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), 512);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
+    uint32_t issued = 0;
+
+    if (warp >= 8) {
+        reg_dec<REGS_REST>();
+        bool ok = *abort_flag == 0;
+        if (warp == 9) {
+            // -------------------------------------------------------- loads: Q, dO, then K(i), V(i)
+            if (lane == 0 && ok && nt > 0) {
+                const uint32_t bytes = (uint32_t)(a.tokens * a.pack * D * 2);
+                mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * bytes);
+                for (int d = 0; d < D / 64; ++d) {
+                    tma_load_3d(base + C::Y1 + d * HALF, &tmQ, smem_u32(&ctl->yfull), 64 * d, head0, at.first);
+                    tma_load_3d(base + C::Y2 + d * HALF, &tmDO, smem_u32(&ctl->yfull), 64 * d, head0, at.first);
+                }
+                uint32_t slot = 0, par = 1;
+                for (int i = 0; i < nt && ok; ++i)
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 641);
+                        if (!ok) break;
+                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                        mbar_arrive_expect_tx(bar, C::TILE);
+                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, k0 + i * TN);
+                        ++issued;
+                        if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+                    }
+            }
+        } else if (warp == 8) {
+            // -------------------------------------------------------- MMAs
+            constexpr uint32_t ID_S = umma_idesc<T>(128, TN, 0, 0), ID_G = umma_idesc<T>(128, D, 0, 1);
+            const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dx0 = umma_desc_sw128(0, HALF, 1024);
+            const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, x_hi = (uint32_t)(dx0 >> 32), x_lo = (uint32_t)dx0;
+            auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
+            auto first_product = [&](int x, int i) {         // x = 0: S(i) = Q K^T, x = 1: dP(i) = dO V^T
+                const int seq = 2 * i + x;
+                ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 643);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t ya = k_lo + ((base + (x ? C::Y2 : C::Y1)) >> 4), xb = k_lo + ((base + C::RING + slot_of(seq) * C::TILE) >> 4);
+                    const uint32_t d = tmem + (x ? DP_COL : (uint32_t)(i & 1) * 128);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                        umma_ss_lohi(d, ya + off, k_hi, xb + off, k_hi, ID_S, ks > 0);
+                    }
+                    umma_commit(x ? smem_u32(&ctl->dpfull) : smem_u32(&ctl->sfull[i & 1]));
+                    if (x) umma_commit(empty0 + 8 * slot_of(seq));       // V is needed no more
+                }
+                __syncwarp();
+            };
+            if (nt > 0) {
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), 0, abort_flag, a.status, 644);
+                if (ok) first_product(0, 0);
+                if (ok) first_product(1, 0);
+            }
+            for (int i = 0; i < nt && ok; ++i) {
+                if (i + 1 < nt) first_product(0, i + 1);     // (over dS of tile i - 1, which dQ has read: MMAs run in their order)
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), i & 1, abort_flag, a.status, 646);
+                if (!ok) break;
+                if (i + 1 < nt) first_product(1, i + 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * i) * C::TILE) >> 4), p = tmem + (uint32_t)(i & 1) * 128;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_ts_lohi(tmem + DQ_COL, p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, (i > 0 || ks > 0) ? 1u : 0u);
+                    umma_commit(empty0 + 8 * slot_of(2 * i));
+                    if (i + 1 == nt) umma_commit(smem_u32(&ctl->gfull));
+                }
+                __syncwarp();
+            }
+            // every MMA issued above has finished before tensor memory is freed
+            if (elect_one()) umma_commit(smem_u32(&ctl->drain));
+            __syncwarp();
+            mbar_wait(smem_u32(&ctl->drain), 0, abort_flag, a.status, 647);
+        }
+    } else {
+        // ------------------------------------------------------------ P, dS and epilogue
+        reg_inc<REGS_MATH>();
+        const int r = tid & 127, ch = warp >> 2;
+        const int tok = r / a.pack, head = head0 + r % a.pack;
+        const bool valid = tok < a.tokens && tok < at.n;
+        const int vis = valid ? seen_by(tok) : 0;
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16), dpcol = tl + DP_COL + 64 * ch;
+        const float c = a.b.scale * kLog2e;
+        const int64_t g = (int64_t)head * a.b.Tq + at.first + tok;
+        const float z = valid ? a.lse[g] : -INFINITY, off = z == -INFINITY ? -INFINITY : -z * kLog2e, delta = valid ? a.delta[g] : 0.f;
+        bool ok = *abort_flag == 0;
+        for (int i = 0; i < nt && ok; ++i) {
+            const uint32_t scol = tl + (uint32_t)(i & 1) * 128 + 64 * ch;
+            ok = mbar_wait_warp(smem_u32(&ctl->sfull[i & 1]), (i >> 1) & 1, abort_flag, a.status, 649);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t x[64];
+            tmem_ld32(scol, x);
+            tmem_ld32(scol + 32, x + 32);
+            tmem_wait_ld_regs(x);
+            tmem_wait_ld_regs(x + 32);
+            const float2 cc = make_float2(c, c), oo = make_float2(off, off);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), cc, oo);
+                x[2 * j] = __float_as_uint(ex2_approx(y.x));
+                x[2 * j + 1] = __float_as_uint(ex2_approx(y.y));
+            }
+            const bool masked = i >= whole;
+            const int lim = vis - i * TN - 64 * ch;
+            if (masked) {
+                // S has read K by now; what is left is dQ, where hidden keys have dS = 0. A half of d for each half of the threads
+                uint8_t* tile = smem + C::RING + (uint32_t)(2 * i) % C::NSLOT * C::TILE;
+                if (64 * ch < D) clean_row<T, 64>(tile + ch * HALF, r);
+                fence_proxy_async_smem();
+            }
+            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 651);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t ds[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t y[32];
+                tmem_ld32(dpcol + 32 * h, y);
+                tmem_wait_ld_regs(y);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int k = 32 * h + 2 * j;
+                    float g0 = __uint_as_float(x[k]) * (__uint_as_float(y[2 * j]) - delta), g1 = __uint_as_float(x[k + 1]) * (__uint_as_float(y[2 * j + 1]) - delta);
+                    if (masked) {
+                        if (k >= lim) g0 = 0.f;
+                        if (k + 1 >= lim) g1 = 0.f;
+                    }
+                    ds[16 * h + j] = pack2<T>(g0, g1);
+                }
+            }
+            tmem_st32(scol, ds);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&ctl->dsfull));
+        }
+        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 652);
+        if (ok) {
+            tc_fence_after();
+            T* dst = static_cast<T*>(a.d0) + ((int64_t)(at.first + tok) * a.b.H + head) * D;
+            store_row<T, D>(dst, tl + DQ_COL, ch * (D / 64), (ch + 1) * (D / 64), nt > 0, valid, a.b.scale);
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    __syncwarp();
+    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, issued);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (*abort_flag)
+        for (int e = tid; e < at.n * a.pack * (D / 2); e += THREADS) {
+            const int row = e / (D / 2);
+            static_cast<uint32_t*>(a.d0)[((int64_t)(at.first + row / a.pack) * a.b.H + head0 + row % a.pack) * (D / 2) + e % (D / 2)] = kNaN16x2;
+        }
+}
+
+template <typename T, int D>
+static int launch(bool kv, const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const BwdArgs& a, cudaStream_t st) {
+    CUtensorMap tq, tk, tv, tdo;
+    // (a batch without queries or without keys loads none, but a map needs an extent)
+    long long nq = a.b.Tq, nk = a.b.Tk;
+    if (!nq) { q = dout = k; rq = rdo = rk; nq = nk; }
+    if (!nk) { k = v = q; rk = rv = rq; nk = nq; }
+    const int qh = a.b.Tq ? a.b.H : a.b.Hk, qbox = a.b.Tq ? a.pack : 1, kvh = a.b.Tk ? a.b.Hk : 1;
+    if (int rc = make_rows_map<T>(&tq, q, D, qh, nq, rq, qbox, a.tokens)) return rc;
+    if (int rc = make_rows_map<T>(&tdo, dout, D, qh, nq, rdo, qbox, a.tokens)) return rc;
+    if (int rc = make_rows_map<T>(&tk, k, D, kvh, nk, rk, 1, TN)) return rc;
+    if (int rc = make_rows_map<T>(&tv, v, D, kvh, nk, rv, 1, TN)) return rc;
+    const int64_t grid = kv ? a.b.Hk * piece_slots(a.b.Tk, TN, a.b.B) : a.b.H / a.pack * piece_slots(a.b.Tq, a.tokens, a.b.B);
+    if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many tiles");
+    auto kern = kv ? packed_bwd_kv_kernel<T, D> : packed_bwd_q_kernel<T, D>;
+    if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
+    kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, tdo, a);
+    ES_CHECK_LAUNCH("packed_bwd_kernel");
+    return 0;
+}
+
+// The caller has checked sizes and pointers. kv: d0 = dK, d1 = dV; else d0 = dQ.
+int packed_bwd_tc(bool kv, const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const float* lse, const float* delta,
+                  void* d0, void* d1, const Batch& b, int D, int dtype, cudaStream_t st) {
+    BwdArgs a{};
+    a.b = b;
+    a.pack = rows_pack(b.G);
+    a.tokens = TM / a.pack;
+    a.lse = lse;
+    a.delta = delta;
+    a.d0 = d0;
+    a.d1 = d1;
+    a.dout = dout;
+    a.rdo = rdo;
+    a.status = device_status_ptr();
+    if (!a.status) return set_error(-2, "es_packed_attn_bwd: the device status word is not available on this device");
+    if (D == 64)
+        return dtype == 0 ? launch<__nv_bfloat16, 64>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st) : launch<__half, 64>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st);
+    return dtype == 0 ? launch<__nv_bfloat16, 128>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st) : launch<__half, 128>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st);
+}
+
+}  // namespace packed
+}  // namespace es

@@ -18,22 +18,12 @@
 // What is hidden must not reach the row, but P = 0 times NaN or infinity is NaN. In the iterations that a mask cuts (the diagonal, the end of the
 // keys) the softmax warps therefore look through V in shared memory; what is not finite is set to 0 there and added at the end, from global
 // memory, to the rows that do see it.
-#include "es_packed.cuh"
-#include "es_vsa_tc.cuh"
+#include "es_packed_tc.cuh"
 
 namespace es {
 namespace packed {
 
 namespace {
-using vsa::pack2;
-using vsa::umma_idesc;
-using vsa::kNaN16x2;
-using vsa::kNaN32;
-
-constexpr int TM = 128, TN = 128, THREADS = 384;
-// Registers per thread: 168 at launch (three warps to a quarter of the SM), shared out anew: 224 + 224 + 56 = 3 * 168.
-constexpr int REGS_SOFTMAX = 224, REGS_REST = 56;
-constexpr uint32_t HALF = TM * 128;                          // 128 rows x 64 d, one swizzled box
 constexpr float RAISE = 8.f;                                 // log2 of the factor
 
 template <int D> struct Cfg {
@@ -56,6 +46,7 @@ struct FwdArgs {
     void* o;
     float* lse;
     float *part_o, *part_lse;                                // [split][token][head][D], log2-domain [split][token][head] (splits > 1)
+    void* o_rest;                                            // what rounding O left, for the backward's delta; may be null
     const void* v;                                           // for what is not finite
     Rows rv;
     int* status;
@@ -72,43 +63,6 @@ struct Work {
 __device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
 }  // namespace
 
-// The tile of grid slot x: pieces of the batch are what lies before the first sequence, the sequences, and what lies behind the last; piece i
-// starts at slot floor(start / span) + i, which leaves each piece at least ceil(length / span) slots without a sum over the lengths.
-// A warp searches 32 pieces at a time.
-__device__ __forceinline__ Work find_work(const FwdArgs& a, int x, int span, int lane) {
-    const int pieces = a.b.B + 2;
-    auto start = [&](int i) { return i == 0 ? 0 : a.b.q_at(i - 1); };
-    int lo = 0, n = pieces;
-    while (n > 1) {
-        const int step = (n + 31) >> 5, i = lo + lane * step;
-        const bool at = lane * step < n && start(i) / span + i <= x;
-        const int c = max(__popc(__ballot_sync(0xffffffffu, at)), 1) - 1;
-        n = min(step, n - c * step);
-        lo += c * step;
-    }
-    Work w{};
-    const int s = start(lo), e = lo + 1 < pieces ? start(lo + 1) : a.b.Tq, t = (x - (s / span + lo)) * span;
-    w.q0 = s + t;
-    w.n_tok = min(span, e - s - t);
-    if (lo >= 1 && lo <= a.b.B) {
-        w.k0 = a.b.k_at(lo - 1);
-        w.nk = max(a.b.k_at(lo) - w.k0, 0);
-        w.base = t + w.nk - (e - s);
-    }
-    return w;
-}
-
-template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {       // either of two packed values
-    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-    return (w & E) == E || ((w >> 16) & E) == E;
-}
-template <typename T> __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-    if ((w & E) == E) w &= 0xFFFF0000u;
-    if (((w >> 16) & E) == E) w &= 0xFFFFu;
-    return w;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -119,8 +73,17 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wide = a.vheads * a.splits, hs = blockIdx.x % wide, vh = hs % a.vheads, split = hs / a.vheads, span = 2 * a.tokens;
     const int per_kv = a.b.G / a.pack, kh = vh / per_kv, head0 = vh * a.pack;
-    Work w = find_work(a, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);       // the last tiles of a causal sequence see the most keys
-    if (w.n_tok <= 0) return;
+    // the last tiles of a causal sequence see the most keys: they go first
+    const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);
+    Work w{};
+    w.q0 = at.first;
+    w.n_tok = at.n;
+    if (at.n <= 0) return;
+    if (at.seq >= 0) {
+        w.k0 = a.b.k_at(at.seq);
+        w.nk = max(a.b.k_at(at.seq + 1) - w.k0, 0);
+        w.base = at.offset + w.nk - at.length;
+    }
     // key tiles of the two row tiles
     int n[2];
     for (int s = 0; s < 2; ++s) {
@@ -263,7 +226,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     } else {
         // ------------------------------------------------------------ softmax and epilogue
-        reg_inc<REGS_SOFTMAX>();
+        reg_inc<REGS_MATH>();
         const int s = warp >> 2, r = tid & 127;
         const int tok = s * a.tokens + r / a.pack, head = head0 + r % a.pack;
         const bool valid = r / a.pack < a.tokens && tok < w.n_tok;
@@ -394,11 +357,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         for (int j = 0; j < 8; ++j)
                             dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
                 } else {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) p[j] = pack2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
                     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D + 32 * h);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        dst[j] = make_uint4(pack2<T>(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1])), pack2<T>(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3])),
-                                            pack2<T>(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5])), pack2<T>(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7])));
+                    for (int j = 0; j < 4; ++j) dst[j] = make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+                    if (a.o_rest) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) p[j] = rest2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]), p[j]);
+                        dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o_rest) + row * D + 32 * h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) dst[j] = make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+                    }
                 }
             }
             if (valid) {
@@ -445,7 +416,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
 // o = sum_p 2^(z_p - M) o_p / sum_p 2^(z_p - M), a warp per row; parts without a key (z = -inf) were not written and are not read.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) merge_kernel(const float* part_o, const float* part_lse, T* o, float* lse, int parts, int Tq, int H) {
+__global__ void __launch_bounds__(256) merge_kernel(const float* part_o, const float* part_lse, T* o, T* o_rest, float* lse, int parts, int Tq, int H) {
     const int lane = threadIdx.x & 31;
     const int64_t rows = (int64_t)Tq * H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
@@ -475,26 +446,13 @@ __global__ void __launch_bounds__(256) merge_kernel(const float* part_o, const f
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-    for (int c = 0; c < C / 2; ++c)
-        reinterpret_cast<uint32_t*>(o + row * D + C * lane)[c] = pack2<T>(sum != 0.f ? acc[2 * c] * inv : 0.f, sum != 0.f ? acc[2 * c + 1] * inv : 0.f);
+    for (int c = 0; c < C / 2; ++c) {
+        const float x = sum != 0.f ? acc[2 * c] * inv : 0.f, y = sum != 0.f ? acc[2 * c + 1] * inv : 0.f;
+        const uint32_t p = pack2<T>(x, y);
+        reinterpret_cast<uint32_t*>(o + row * D + C * lane)[c] = p;
+        if (o_rest) reinterpret_cast<uint32_t*>(o_rest + row * D + C * lane)[c] = rest2<T>(x, y, p);
+    }
     if (lane == 0) lse[(row % H) * Tq + row / H] = sum != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
-}
-
-// Query heads that share a tile's rows: the most heads of a group (a divisor of it) that still fill 15 of 16 rows. More heads make the tile
-// shorter in tokens; the rows lost are computed for nothing.
-int rows_pack(int G) {
-    for (int d = min(G, TM); d > 1; --d)
-        if (G % d == 0 && TM / d * d >= TM - TM / 16) return d;
-    return 1;
-}
-
-template <typename T> static int make_rows_map(CUtensorMap* m, const void* ptr, int D, int heads, long long tokens, Rows r, int box_heads, int box_tokens) {
-    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens};
-    cuuint64_t str[2] = {(cuuint64_t)r.head * 2, (cuuint64_t)r.token * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
-    cuuint32_t estr[3] = {1, 1, 1};
-    return encode_tensor_map(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                             const_cast<void*>(ptr), dims, str, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <typename T, int D>
@@ -513,15 +471,15 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
     ES_CHECK_LAUNCH("packed_fwd_kernel");
     if (a.splits > 1) {
-        merge_kernel<T, D><<<(unsigned)(((int64_t)a.b.Tq * a.b.H + 7) / 8), 256, 0, st>>>(a.part_o, a.part_lse, static_cast<T*>(a.o), a.lse, a.splits, a.b.Tq, a.b.H);
+        merge_kernel<T, D><<<(unsigned)(((int64_t)a.b.Tq * a.b.H + 7) / 8), 256, 0, st>>>(a.part_o, a.part_lse, static_cast<T*>(a.o), static_cast<T*>(a.o_rest), a.lse, a.splits, a.b.Tq, a.b.H);
         ES_CHECK_LAUNCH("merge_kernel");
     }
     return 0;
 }
 
 // The caller has checked sizes and pointers.
-int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, float* lse, const Batch& b, int D, int dtype, void* ws,
-                  cudaStream_t st) {
+int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, void* o_rest,
+                  float* lse, const Batch& b, int D, int dtype, void* ws, cudaStream_t st) {
     (void)ws;
     FwdArgs a{};
     a.b = b;
@@ -530,6 +488,7 @@ int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     a.splits = 1;
     a.vheads = b.H / a.pack;
     a.o = o;
+    a.o_rest = o_rest;
     a.lse = lse;
     a.v = v;
     a.rv = rv;

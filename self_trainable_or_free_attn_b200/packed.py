@@ -87,24 +87,25 @@ def _call(name, *args):
     N.check(getattr(N.load(), name)(*args), name)
 
 
-def _fwd(q, k, v, cu_q, cu_k, scale, causal):
+def _fwd(q, k, v, cu_q, cu_k, scale, causal, with_rest):
     T, H, D = q.shape
     o = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
+    rest = torch.empty_like(o) if with_rest else None
     lse = torch.empty(H, T, device=q.device, dtype=torch.float32)
     B, Hk = cu_q.numel() - 1, k.shape[1]
     n = int(N.load().es_packed_workspace_bytes(B, T, k.shape[0], H, Hk, D))
     ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-    _call("es_packed_attn_fwd", N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(o), N.ptr(lse), N.ptr(cu_q), N.ptr(cu_k), B, T, k.shape[0], H, Hk, D,
-          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
-    return o, lse
+    _call("es_packed_attn_fwd", N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(o), N.ptr(rest), N.ptr(lse), N.ptr(cu_q), N.ptr(cu_k), B, T, k.shape[0], H,
+          Hk, D, *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
+    return o, rest, lse
 
 
 class _Function(torch.autograd.Function):
     @staticmethod
     @N.device_guard
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
-        o, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal)
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        o, rest, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, rest, lse, cu_q, cu_k)
         ctx.scale, ctx.causal = scale, causal
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -116,12 +117,12 @@ class _Function(torch.autograd.Function):
     def backward(ctx, dout, dlse):
         if dout is None:
             return (None,) * 7
-        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, o, rest, lse, cu_q, cu_k = ctx.saved_tensors
         dout = rows(dout)
         (T, H, D), (Tk, Hk, _) = q.shape, k.shape
         delta = torch.empty_like(lse)
         dt, st = _DTYPES[q.dtype], N.stream_ptr()
-        _call("es_packed_delta", N.ptr(o), N.ptr(dout), N.ptr(delta), T, H, D, *strides(dout), dt, st)
+        _call("es_packed_delta", N.ptr(o), N.ptr(rest), N.ptr(dout), N.ptr(delta), T, H, D, *strides(dout), dt, st)
         sizes = (cu_q.numel() - 1, T, Tk, H, Hk, D, *strides(q), *strides(k), *strides(v), *strides(dout), ctx.scale, ctx.causal, dt, st)
         ins = [N.ptr(t) for t in (q, k, v, dout, lse, delta)]
         cus = (N.ptr(cu_q), N.ptr(cu_k))

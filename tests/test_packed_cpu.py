@@ -9,7 +9,7 @@ BIG = 0x10000
 
 
 def _fwd(**over):
-    a = dict(q=BIG, k=2 * BIG, v=3 * BIG, o=4 * BIG, lse=5 * BIG, cu_q=6 * BIG, cu_k=7 * BIG, B=2, Tq=10, Tk=12, H=4, Hk=2, D=64,
+    a = dict(q=BIG, k=2 * BIG, v=3 * BIG, o=4 * BIG, rest=8 * BIG, lse=5 * BIG, cu_q=6 * BIG, cu_k=7 * BIG, B=2, Tq=10, Tk=12, H=4, Hk=2, D=64,
              qt=256, qh=64, kt=128, kh=64, vt=128, vh=64, scale=0.1, causal=1, dtype=0, ws=None, st=None)
     a.update(over)
     return a
@@ -26,7 +26,7 @@ def _bwd(kv, **over):
 
 
 def _delta(**over):
-    a = dict(o=BIG, do=2 * BIG, delta=3 * BIG, T=10, H=4, D=64, dt=256, dh=64, dtype=0, st=None)
+    a = dict(o=BIG, rest=None, do=2 * BIG, delta=3 * BIG, T=10, H=4, D=64, dt=256, dh=64, dtype=0, st=None)
     a.update(over)
     return a
 
@@ -55,7 +55,7 @@ def _store(**over):
 SIZES = [dict(B=-1), dict(Tq=-1), dict(Tk=-1), dict(Tq=0x7FFFFF00), dict(H=0), dict(H=3), dict(Hk=0), dict(D=96), dict(dtype=2)]
 REFUSED = (
     [("es_packed_attn_fwd", _fwd, x) for x in SIZES + [dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(lse=None), dict(cu_q=None), dict(cu_k=None),
-                                                       dict(q=BIG + 8), dict(k=BIG + 8), dict(v=BIG + 2), dict(o=BIG + 8), dict(qt=257), dict(kh=60), dict(vt=4)]]
+                                                       dict(q=BIG + 8), dict(k=BIG + 8), dict(v=BIG + 2), dict(o=BIG + 8), dict(rest=BIG + 8), dict(qt=257), dict(kh=60), dict(vt=4)]]
     + [(f"es_packed_attn_bwd_{n}", lambda kv=kv, **o: _bwd(kv, **o), x) for n, kv in (("q", False), ("kv", True))
        for x in SIZES + [dict(q=None), dict(do=None), dict(lse=None), dict(delta=None), dict(d0=None), dict(cu_q=None), dict(do=BIG + 8), dict(d0=BIG + 8), dict(dt=4),
                          dict(qh=65)]]
