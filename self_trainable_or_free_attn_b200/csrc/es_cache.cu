@@ -1,75 +1,9 @@
-// A paged cache of keys and values: pages and slots of new tokens, storing them, and attention of a batch's next tokens to a shared
-// prefix and to each request's own tokens. Entry points at the end.
+// A paged cache of keys and values: pages and slots of new tokens, and storing them. (Attention to it: es_prefix.cu.)
 #include "es_packed.cuh"
 
 namespace es {
 namespace packed {
 namespace {
-
-__device__ __forceinline__ float warp_max(float x) {
-    for (int i = 16; i; i >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
-    return x;
-}
-__device__ __forceinline__ float warp_sum(float x) {
-    for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-    return x;
-}
-
-struct CacheRows {
-    int64_t page, token, head;
-};
-
-struct PrefixArgs {
-    const int *prefix_pages, *table, *lengths;
-    float* lse;
-    int prefix_len, width, B, N, H, Hk, pages, log_page;
-    float scale;
-};
-
-// A warp per query row, 32 keys at a time.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) prefix_rows_kernel(const T* q, const T* kc, CacheRows rk, const T* vc, CacheRows rv, T* o, PrefixArgs a) {
-    constexpr int C = D / 32;
-    __shared__ float rows[4][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + warp;
-    if (row >= (int64_t)a.B * a.N * a.H) return;
-    const int h = (int)(row % a.H), i = (int)(row / a.H % a.N), b = (int)(row / a.H / a.N), hk = h / (a.H / a.Hk);
-    for (int c = lane; c < D; c += 32) rows[warp][c] = to_float(q[row * D + c]);
-    __syncwarp();
-    const int own = min(max(min(a.lengths[b], a.width << a.log_page) - a.N + i + 1, 0), a.width << a.log_page);
-    float top = -INFINITY, sum = 0.f, acc[C] = {};
-    for (int part = 0; part < 2; ++part) {
-        const int n = part ? own : a.prefix_len;
-        const int* list = part ? a.table + (int64_t)b * a.width : a.prefix_pages;
-        for (int j0 = 0; j0 < n; j0 += 32) {
-            const int j = j0 + lane, page = j < n ? list[j >> a.log_page] : -1, at = j & ((1 << a.log_page) - 1);
-            const bool seen = page >= 0 && page < a.pages;
-            float x = -INFINITY;
-            if (seen) {
-                const T* kr = kc + page * rk.page + at * rk.token + hk * rk.head;
-                x = 0.f;
-                for (int c = 0; c < D; ++c) x += rows[warp][c] * to_float(kr[c]);
-                x *= a.scale * kLog2e;
-            }
-            const float next = fmaxf(top, warp_max(x)), off = next == -INFINITY ? 0.f : next, shrink = exp2f(top - off);
-            const float p = seen ? exp2f(x - off) : 0.f;
-            sum = sum * shrink + warp_sum(p);
-            top = next;
-            for (int c = 0; c < C; ++c) acc[c] *= shrink;
-            for (int jj = 0; jj < 32; ++jj) {
-                const float w = __shfl_sync(0xffffffffu, p, jj);
-                const int pg = __shfl_sync(0xffffffffu, page, jj), tk = __shfl_sync(0xffffffffu, at, jj);
-                if (pg < 0 || pg >= a.pages) continue;
-                const T* vr = vc + pg * rv.page + tk * rv.token + hk * rv.head;
-                for (int c = 0; c < C; ++c) acc[c] += w * to_float(vr[lane + 32 * c]);
-            }
-        }
-    }
-    const bool none = sum == 0.f;
-    for (int c = 0; c < C; ++c) o[row * D + lane + 32 * c] = from_float<T>(none ? 0.f : acc[c] / sum);
-    if (lane == 0) a.lse[((int64_t)b * a.H + h) * a.N + i] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
-}
 
 // ---------------------------------------------------------------------------------------------- pages and slots
 constexpr int PLAN_THREADS = 256, PLAN_CHUNK = 1024;          // requests that a CTA scans at a time
@@ -213,39 +147,6 @@ template <int D> __global__ void __launch_bounds__(256) store_kv_kernel(StoreArg
 
 using namespace es;
 using namespace es::packed;
-
-extern "C" long long es_prefix_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
-
-extern "C" int es_prefix_attn(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse, const int32_t* prefix_pages,
-                              int32_t n_prefix_pages, int32_t prefix_len, const int32_t* table, int32_t table_width, const int32_t* lengths,
-                              int32_t batch, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t D, int32_t pages, int32_t page_size,
-                              int64_t k_page, int64_t k_token, int64_t k_head, int64_t v_page, int64_t v_token, int64_t v_head, float scale,
-                              int32_t dtype, void* workspace, void* stream) {
-    (void)workspace;
-    if (int rc = check_sizes("es_prefix_attn", batch, tokens, prefix_len, heads, kv_heads, D, dtype)) return rc;
-    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
-        return set_error(-1, "es_prefix_attn: page_size must be 16, 32, 64, 128 or 256");
-    if (pages < 0 || table_width < 0 || n_prefix_pages < 0 || (int64_t)table_width * page_size > 0x7FFFFFFF || (int64_t)pages * page_size > 0x7FFFFFFF ||
-        (int64_t)n_prefix_pages * page_size < prefix_len || (int64_t)batch * tokens * heads > 0x7FFFFFFF)
-        return set_error(-1, "es_prefix_attn: sizes out of range");
-    if (batch == 0 || tokens == 0) return 0;
-    if (!q || !o || !lse || !lengths || (prefix_len && !prefix_pages) || (table_width && !table) || (pages && (!k_cache || !v_cache)))
-        return set_error(-1, "es_prefix_attn: null pointer");
-    if (!aligned(16, q, k_cache, v_cache, o)) return set_error(-1, "es_prefix_attn: q, k_cache, v_cache, o must be 16-byte aligned");
-    if (!whole_chunks(k_page, k_token, k_head, v_page, v_token, v_head)) return set_error(-1, "es_prefix_attn: strides must be multiples of 8 elements");
-    PrefixArgs a{prefix_pages, table, lengths, lse, prefix_len, table_width, batch, tokens, heads, kv_heads, pages, 0, scale};
-    while ((1 << a.log_page) < page_size) ++a.log_page;
-    const unsigned grid = (unsigned)(((int64_t)batch * tokens * heads + 3) / 4);
-    auto go = [&](auto t, auto d) {
-        using T = decltype(t);
-        prefix_rows_kernel<T, d><<<grid, 128, 0, (cudaStream_t)stream>>>((const T*)q, (const T*)k_cache, {k_page, k_token, k_head}, (const T*)v_cache,
-                                                                         {v_page, v_token, v_head}, (T*)o, a);
-        ES_CHECK_LAUNCH("prefix_rows_kernel");
-        return 0;
-    };
-    if (dtype == 0) return D == 64 ? go(__nv_bfloat16{}, std::integral_constant<int, 64>{}) : go(__nv_bfloat16{}, std::integral_constant<int, 128>{});
-    return D == 64 ? go(__half{}, std::integral_constant<int, 64>{}) : go(__half{}, std::integral_constant<int, 128>{});
-}
 
 extern "C" int es_extend_tables(const int32_t* lengths, const int32_t* new_tokens, int32_t* table, const int32_t* free_pages, int32_t n_free,
                                 int32_t batch, int32_t table_width, int32_t page_size, int32_t total, int32_t* slots, int32_t* positions,

@@ -20,6 +20,11 @@ struct Rows {
     int64_t token, head;
 };
 
+// A page, a token and a head stride, in elements.
+struct CacheRows {
+    int64_t page, token, head;
+};
+
 // What the kernels of a packed batch have in common.
 struct Batch {
     const int *cu_q, *cu_k;

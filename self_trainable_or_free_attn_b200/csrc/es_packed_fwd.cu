@@ -35,7 +35,6 @@ struct Ctl {
     uint64_t qfull[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain;
     uint32_t tmem_base;
     int abort, not_finite;
-    uint32_t seen[10];                                       // paged: a bit per page of the slot's tile that is one of the cache
 };
 static_assert(sizeof(Ctl) <= 512, "control block");
 
@@ -50,6 +49,10 @@ struct FwdArgs {
     const void* v;                                           // for what is not finite
     Rows rv;
     int* status;
+    // paged keys: all queries see the first nk tokens of the pages in `list`
+    const int* list;
+    int nk, pages, log_page;
+    int64_t v_page;
 };
 
 // What a CTA does.
@@ -63,7 +66,7 @@ struct Work {
 __device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
 }  // namespace
 
-template <typename T, int D>
+template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ FwdArgs a) {
@@ -73,16 +76,22 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wide = a.vheads * a.splits, hs = blockIdx.x % wide, vh = hs % a.vheads, split = hs / a.vheads, span = 2 * a.tokens;
     const int per_kv = a.b.G / a.pack, kh = vh / per_kv, head0 = vh * a.pack;
-    // the last tiles of a causal sequence see the most keys: they go first
-    const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);
     Work w{};
-    w.q0 = at.first;
-    w.n_tok = at.n;
-    if (at.n <= 0) return;
-    if (at.seq >= 0) {
-        w.k0 = a.b.k_at(at.seq);
-        w.nk = max(a.b.k_at(at.seq + 1) - w.k0, 0);
-        w.base = at.offset + w.nk - at.length;
+    if (PAGED) {
+        w.q0 = blockIdx.x / wide * span;
+        w.n_tok = min(span, a.b.Tq - w.q0);
+        w.nk = a.nk;
+    } else {
+        // the last tiles of a causal sequence see the most keys: they go first
+        const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);
+        w.q0 = at.first;
+        w.n_tok = at.n;
+        if (at.n <= 0) return;
+        if (at.seq >= 0) {
+            w.k0 = a.b.k_at(at.seq);
+            w.nk = max(a.b.k_at(at.seq + 1) - w.k0, 0);
+            w.base = at.offset + w.nk - at.length;
+        }
     }
     // key tiles of the two row tiles
     int n[2];
@@ -134,27 +143,45 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp == 9) {
         // ------------------------------------------------------------ loads: Q, then K(i), V(i) for every i
         bool ok = *abort_flag == 0;
-        if (lane == 0 && ok && nt > 0) {
-            tma_prefetch_desc(&tmK);
-            tma_prefetch_desc(&tmV);
-            const uint32_t qbytes = (uint32_t)(a.tokens * a.pack * D * 2);
-            for (int s = 0; s < 2; ++s) {
-                if ((s ? end1 : end0) <= w.i0) continue;     // nobody would wait for it
-                mbar_arrive_expect_tx(smem_u32(&ctl->qfull[s]), qbytes);
-                for (int d = 0; d < D / 64; ++d)
-                    tma_load_3d(base + C::Q + s * C::TILE + d * HALF, &tmQ, smem_u32(&ctl->qfull[s]), 64 * d, head0, w.q0 + s * a.tokens);
+        const int box = min(TN, PAGED ? 1 << a.log_page : TN), boxes = TN / box;
+        if (ok && nt > 0 && (PAGED || lane == 0)) {
+            if (lane == 0) {
+                tma_prefetch_desc(&tmK);
+                tma_prefetch_desc(&tmV);
+                const uint32_t qbytes = (uint32_t)(a.tokens * a.pack * D * 2);
+                for (int s = 0; s < 2; ++s) {
+                    if ((s ? end1 : end0) <= w.i0) continue; // nobody would wait for it
+                    mbar_arrive_expect_tx(smem_u32(&ctl->qfull[s]), qbytes);
+                    for (int d = 0; d < D / 64; ++d)
+                        tma_load_3d(base + C::Q + s * C::TILE + d * HALF, &tmQ, smem_u32(&ctl->qfull[s]), 64 * d, head0, w.q0 + s * a.tokens);
+                }
             }
             uint32_t slot = 0, par = 1;
-            for (int i = w.i0; i < w.i1 && ok; ++i)
+            for (int i = w.i0; i < w.i1 && ok; ++i) {
+                // paged: a lane per box; a page that is not of the cache, or behind the keys, is loaded as zeros
+                int page = a.pages;
+                if (PAGED && lane < boxes && i * TN + lane * box < w.nk) {
+                    const int p = __ldg(a.list + ((i * TN + lane * box) >> a.log_page));
+                    if (p >= 0 && p < a.pages) page = p;
+                }
                 for (int x = 0; x < 2 && ok; ++x) {
-                    ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 601);
+                    ok = PAGED ? mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 601) : mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 601);
                     if (!ok) break;
                     const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
-                    mbar_arrive_expect_tx(bar, C::TILE);
-                    for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.k0 + i * TN);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+                    if (PAGED) {
+                        __syncwarp();
+                        if (lane < boxes)
+                            for (int d = 0; d < D / 64; ++d)
+                                tma_load_4d(dst + d * HALF + lane * box * 128, x ? &tmV : &tmK, bar, 64 * d, kh, (i * TN) & ((1 << a.log_page) - 1), page);
+                        __syncwarp();
+                    } else {
+                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.k0 + i * TN);
+                    }
                     ++issued;
                     if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                 }
+            }
         }
     } else if (warp == 8) {
         // ------------------------------------------------------------ MMAs
@@ -237,8 +264,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float c = a.b.scale * kLog2e;
         float m = -INFINITY, l = 0.f;
         bool ok = *abort_flag == 0;
+        const int box = min(TN, PAGED ? 1 << a.log_page : TN);
+        // paged: a bit per box of tile i whose page is not of the cache; looked up a tile ahead
+        auto bad_pages = [&](int i) -> uint32_t {
+            const int k = i * TN + lane * box;
+            const int p = lane * box < TN && k < w.nk ? __ldg(a.list + (k >> a.log_page)) : 0;
+            return __ballot_sync(0xffffffffu, p < 0 || p >= a.pages);
+        };
+        uint32_t bad = 0, bad_next = PAGED && w.i0 < end ? bad_pages(w.i0) : 0u;
         for (int i = w.i0; i < end && ok; ++i) {
             const int it = i - w.i0;
+            if (PAGED) {
+                bad = bad_next;
+                if (i + 1 < end) bad_next = bad_pages(i + 1);
+            }
             ok = mbar_wait_warp(smem_u32(&ctl->sfull[s]), it & 1, abort_flag, a.status, 607);
             if (!ok) break;
             tc_fence_after();
@@ -252,6 +291,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
                     if (j >= lim) x[j] = 0xff800000u;
+            }
+            if (PAGED && bad) {
+                // (their keys and values are zeros: nothing of them can reach the row but the logit 0)
+                const int shift = min(a.log_page, 7);
+#pragma unroll
+                for (int j = 0; j < TN; j += 16)
+                    if ((bad >> (j >> shift)) & 1)
+#pragma unroll
+                        for (int jj = 0; jj < 16; ++jj) x[j + jj] = 0xff800000u;
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -341,7 +389,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l != 0.f ? __uint_as_float(o[j]) * inv : 0.f);
                 if (fix && valid) {
                     for (int k = from; k < to; ++k) {
-                        const T* vr = static_cast<const T*>(a.v) + (int64_t)(w.k0 + k) * a.rv.token + (int64_t)kh * a.rv.head + 32 * h;
+                        const T* vr = static_cast<const T*>(a.v) + (int64_t)kh * a.rv.head + 32 * h;
+                        if (PAGED) {
+                            const int p = __ldg(a.list + (k >> a.log_page));
+                            if (p < 0 || p >= a.pages) continue;
+                            vr += p * a.v_page + (int64_t)(k & ((1 << a.log_page) - 1)) * a.rv.token;
+                        } else {
+                            vr += (int64_t)(w.k0 + k) * a.rv.token;
+                        }
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             const float e = to_float(vr[j]);
@@ -350,7 +405,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     }
                 }
                 if (!valid) continue;
-                if (a.splits > 1) {
+                if (PAGED || a.splits > 1) {
                     float4* dst = reinterpret_cast<float4*>(a.part_o + ((int64_t)split * a.b.Tq * a.b.H + row) * D + 32 * h);
                     if (any)
 #pragma unroll
@@ -374,7 +429,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
             if (valid) {
                 const float z = l != 0.f ? m + log2f(l) : -INFINITY;
-                if (a.splits > 1) a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = z;
+                if (PAGED || a.splits > 1) a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = z;
                 else a.lse[(int64_t)head * a.b.Tq + w.q0 + tok] = z * kLn2;
             }
         }
@@ -403,7 +458,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // NaN in all that the CTA owns: the caller's memory is not initialised
         for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
             const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head0 + e % a.pack;
-            if (a.splits > 1) {
+            if (PAGED || a.splits > 1) {
                 a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = __uint_as_float(kNaN32);
                 for (int d = 0; d < D; ++d) a.part_o[((int64_t)split * a.b.Tq * a.b.H + row) * D + d] = __uint_as_float(kNaN32);
             } else {
@@ -464,9 +519,9 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     if (int rc = make_rows_map<T>(&tq, q, D, a.b.H, a.b.Tq, rq, a.pack, a.tokens)) return rc;
     if (int rc = make_rows_map<T>(&tk, k, D, a.b.Hk, tk_rows, rk, 1, TN)) return rc;
     if (int rc = make_rows_map<T>(&tv, v, D, a.b.Hk, tk_rows, rv, 1, TN)) return rc;
-    auto kern = packed_fwd_kernel<T, D>;
+    auto kern = packed_fwd_kernel<T, D, false>;
     if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
-    const int64_t grid = (int64_t)a.vheads * a.splits * (a.b.Tq / (2 * a.tokens) + a.b.B + 2);
+    const int64_t grid = (int64_t)a.vheads * a.splits * piece_slots(a.b.Tq, 2 * a.tokens, a.b.B);
     if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_fwd: too many tiles");
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
     ES_CHECK_LAUNCH("packed_fwd_kernel");
@@ -497,6 +552,47 @@ int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     if (D == 64)
         return dtype == 0 ? launch<__nv_bfloat16, 64>(q, rq, k, rk, v, rv, a, st) : launch<__half, 64>(q, rq, k, rk, v, rv, a, st);
     return dtype == 0 ? launch<__nv_bfloat16, 128>(q, rq, k, rk, v, rv, a, st) : launch<__half, 128>(q, rq, k, rk, v, rv, a, st);
+}
+
+// The part of a batch's new tokens that sees a prefix in pages: `parts` fp32 partial results and log2-domain LSEs, [part][token][head]. The caller has
+// checked sizes and pointers.
+template <typename T, int D>
+static int launch_prefix(const void* q, const void* k, CacheRows rk, const void* v, CacheRows rv, const FwdArgs& a, cudaStream_t st) {
+    CUtensorMap tq, tk, tv;
+    if (int rc = make_rows_map<T>(&tq, q, D, a.b.H, a.b.Tq, {(int64_t)a.b.H * D, D}, a.pack, a.tokens)) return rc;
+    if (int rc = make_pages_map<T>(&tk, k, D, a.b.Hk, 1 << a.log_page, a.pages, rk, TN)) return rc;
+    if (int rc = make_pages_map<T>(&tv, v, D, a.b.Hk, 1 << a.log_page, a.pages, rv, TN)) return rc;
+    const int64_t grid = (int64_t)a.vheads * a.splits * ((a.b.Tq + 2 * a.tokens - 1) / (2 * a.tokens));
+    if (grid > 0x7FFFFFFF) return set_error(-1, "es_prefix_attn: too many tiles");
+    auto kern = packed_fwd_kernel<T, D, true>;
+    if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
+    kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
+    ES_CHECK_LAUNCH("packed_fwd_kernel (paged)");
+    return 0;
+}
+
+int prefix_fwd_tc(const void* q, const void* k, CacheRows rk, const void* v, CacheRows rv, float* part_o, float* part_lse, int parts, const int* list, int prefix_len,
+                  int tokens, int H, int Hk, int pages, int log_page, float scale, int D, int dtype, cudaStream_t st) {
+    FwdArgs a{};
+    a.b = Batch{nullptr, nullptr, 0, tokens, 0, H, Hk, H / Hk, scale, 0};
+    a.pack = rows_pack(a.b.G);
+    a.tokens = TM / a.pack;
+    a.splits = parts;
+    a.vheads = H / a.pack;
+    a.part_o = part_o;
+    a.part_lse = part_lse;
+    a.v = v;
+    a.rv = Rows{rv.token, rv.head};
+    a.v_page = rv.page;
+    a.list = list;
+    a.nk = prefix_len;
+    a.pages = pages;
+    a.log_page = log_page;
+    a.status = device_status_ptr();
+    if (!a.status) return set_error(-2, "es_prefix_attn: the device status word is not available on this device");
+    if (D == 64)
+        return dtype == 0 ? launch_prefix<__nv_bfloat16, 64>(q, k, rk, v, rv, a, st) : launch_prefix<__half, 64>(q, k, rk, v, rv, a, st);
+    return dtype == 0 ? launch_prefix<__nv_bfloat16, 128>(q, k, rk, v, rv, a, st) : launch_prefix<__half, 128>(q, k, rk, v, rv, a, st);
 }
 
 }  // namespace packed

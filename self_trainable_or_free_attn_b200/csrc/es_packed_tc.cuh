@@ -82,5 +82,15 @@ template <typename T> int make_rows_map(CUtensorMap* m, const void* ptr, int D, 
                              const_cast<void*>(ptr), dims, str, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// A cache in pages [pages][page][heads][D] in boxes of up to `rows` tokens of one page.
+template <typename T> int make_pages_map(CUtensorMap* m, const void* ptr, int D, int heads, int page, int pages, CacheRows r, int rows) {
+    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)page, (cuuint64_t)pages};
+    cuuint64_t str[3] = {(cuuint64_t)r.head * 2, (cuuint64_t)r.token * 2, (cuuint64_t)r.page * 2};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)(page < rows ? page : rows), 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return encode_tensor_map(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                             const_cast<void*>(ptr), dims, str, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 }  // namespace packed
 }  // namespace es
