@@ -76,6 +76,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wide = a.vheads * a.splits, hs = blockIdx.x % wide, vh = hs % a.vheads, split = hs / a.vheads, span = 2 * a.tokens;
     const int per_kv = a.b.G / a.pack, kh = vh / per_kv, head0 = vh * a.pack;
+    if (PAGED) launch_dependents();                          // the requests' own tokens may go ahead where an SM is free
     Work w{};
     if (PAGED) {
         w.q0 = blockIdx.x / wide * span;

@@ -7,9 +7,10 @@
 //   own tokens   `own_kernel`: tokens x heads of a group rows against each request's pages. Every key is read once and multiplied with a few
 //                rows: bound by HBM. Warps with m16n8k16 MMAs, 64 keys at a time, scores and P in registers: the tensor cores are idle most of the
 //                time at any shape (16 FLOP a byte; tcgen05 with its 128 rows would compute eight times as much for the same bytes).
-// Work of own_kernel: the (request, heads, block of new tokens) items, each a run of 64-key units, one behind the other; CTA c of C takes the
-// units c W / C .. (c + 1) W / C of W whatever the lengths are. An item's first share is stored by its rows (part A), one that starts inside an
-// item by its CTA (part B; a CTA has at most one). The merge finds them by the same arithmetic.
+// Work of own_kernel: the (request, heads, block of new tokens) items, each ITEM + its 64-key units long, one behind the other; CTA c of C has
+// the stretch c W / C .. (c + 1) W / C of W whatever the lengths are. (ITEM: what starting and storing an item costs, in units.) An item's first
+// share is stored by its rows (part A), one that starts inside an item by its CTA (part B; a CTA has at most one). The join finds them by
+// the same arithmetic.
 #include "es_packed_tc.cuh"
 #include "es_vsa_mma.cuh"
 
@@ -21,12 +22,15 @@ int prefix_fwd_tc(const void* q, const void* k, CacheRows rk, const void* v, Cac
 
 namespace {
 constexpr int UNIT = 64, WARPS = 4, OWN_THREADS = 32 * (WARPS + 1), ROWS = 64;
-constexpr int GROUPS = 1024;                                  // requests (or groups of them) whose running sums a CTA keeps
+constexpr int ITEM = 2;
 
 __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
 }
-__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 
 struct PrefixArgs {
     const int *prefix_pages, *table, *lengths;
@@ -42,176 +46,197 @@ struct PrefixArgs {
     float *p_o, *p_lse;              // of the prefix: parts [part][token][head][D], or part A of its item
     int p_parts;
     float *b_o, *b_lse;              // part B [cta][ROWS][D], [cta][ROWS]
-    long long* first;                // [B + 1] first unit of each request: written by CTA 0
+    long long* first;                // [B + 1] where each request starts: written by CTA 0
     int* status;
 };
 
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) { return min(max(__ldg(a.lengths + b), 0), a.width << a.log_page); }
-__device__ __forceinline__ long long prefix_units(const PrefixArgs& a) {
-    return a.prefix_item ? (long long)(a.prefix_len + UNIT - 1) / UNIT * a.vheads : 0;
-}
+__device__ __forceinline__ int units_of(int keys) { return (int)(((long long)keys + UNIT - 1) / UNIT); }
+// The stretch of a set of keys: of all its items.
+__device__ __forceinline__ long long stretch(int keys, int items) { return keys > 0 ? (long long)(units_of(keys) + ITEM) * items : 0; }
+__device__ __forceinline__ long long prefix_stretch(const PrefixArgs& a) { return a.prefix_item ? stretch(a.prefix_len, a.vheads) : 0; }
 
-template <int D> struct Own {
+template <int D, int MT> struct Own {
     static constexpr uint32_t HALF = UNIT * 128, TILE = UNIT * D * 2;
-    static constexpr int NSLOT = D == 128 ? 5 : 8;             // two CTAs per SM
-    static constexpr uint32_t RING = 0, SUM = NSLOT * TILE, CTL = SUM + 2 * 16 * D * 4, SCAN = CTL + 512, BYTES = SCAN + (GROUPS + 1) * 8;
+    static constexpr int NSLOT = D == 64 ? 8 : MT == 2 ? 3 : 4;        // two CTAs per SM
+    static constexpr uint32_t QPITCH = D * 2 + 16, QTILE = 16 * MT * QPITCH;
+    static constexpr uint32_t RING = 0, Q = NSLOT * TILE, SUM = Q + 2 * QTILE, CTL = SUM + (MT < 4 ? WARPS * 16 * D * 4 : 0), BYTES = CTL + 1536;
 };
-struct OwnCtl {
-    uint64_t full[8], empty[8];
-    int abort, not_finite;
-    float ml[2][32];                 // maxima and sums of the warps that are joined with others
-    long long warp_sum[WARPS + 1];
-};
-static_assert(sizeof(OwnCtl) <= 512, "control block");
-
-// One share of an item: rows of one request (or of the batch, for the prefix) against its units from .. to.
-struct Share {
+// A unit as the load warp hands it to the others.
+struct UnitDesc {
+    int k0;              // first key in its set, -1: no more units
+    int n;               // keys of the set
     int b;               // request, -1: the prefix
-    int head0, t0, rows; // first head, first new token of the item (in the batch), rows
-    int u0, u1;          // units of the item
-    bool starts;         // from the item's first unit
-    int n;               // keys of the item
+    int head0, t0, tq;   // first head, first new token of the item: in the batch, in the request
+    int rows;
+    int flags;           // FIRST, LAST unit of the CTA's share of the item; STARTS: the item's first share
+    uint32_t bad;        // a bit per box whose page is not of the cache
 };
-
-// Finds the item of unit u: which request, heads and block of tokens, and the unit's number in it.
-struct Finder {
-    const PrefixArgs& a;
-    const long long* sums;           // units before group g of requests
-    int group;                       // requests in a group
-    __device__ __forceinline__ Share at(long long u, long long end) const {
-        Share s;
-        const long long pu = prefix_units(a);
-        long long per;
-        long long x;
-        if (u < pu) {
-            s.b = -1;
-            s.n = a.prefix_len;
-            x = u;
-        } else {
-            int lo = 0, hi = (a.B + group - 1) / group;
-            while (lo + 1 < hi) {
-                const int m = (lo + hi) >> 1;
-                if (sums[m] <= u) lo = m; else hi = m;
-            }
-            int b = lo * group;
-            long long f = sums[lo], w;
-            while (f + (w = units(b)) <= u) { f += w; ++b; }
-            s.b = b;
-            s.n = own_length(a, b);
-            x = u - f;
-        }
-        per = (s.n + UNIT - 1) / UNIT;
-        const int item = (int)(x / per);
-        s.u0 = (int)(x - item * per);
-        s.u1 = (int)min(per, s.u0 + (end - u));
-        s.starts = s.u0 == 0;
-        s.head0 = item % a.vheads * a.pack;
-        const int blk = s.b < 0 ? 0 : item / a.vheads, tokens = s.b < 0 ? a.B * a.N : min(a.per_block, a.N - blk * a.per_block);
-        s.t0 = s.b < 0 ? 0 : s.b * a.N + blk * a.per_block;
-        s.rows = tokens * a.pack;
-        return s;
-    }
-    __device__ __forceinline__ long long units(int b) const { return (long long)((own_length(a, b) + UNIT - 1) / UNIT) * a.vheads * a.blocks; }
+enum { FIRST = 1, LAST = 2, STARTS = 4 };
+struct OwnCtl {
+    uint64_t full[8], empty[8], qfull[2], qempty[2], joined;
+    int abort, not_finite, first_b;
+    long long first_x, warp_sum[WARPS + 1];
+    UnitDesc desc[4];
+    float ml[WARPS][32];             // maxima and sums of warps that are joined
 };
+static_assert(sizeof(OwnCtl) <= 1536, "control block");
 
 // MT: 16-row tiles of an item. One: every warp has them and a quarter of a unit's keys; two: two warps each and half; four: all keys.
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(OWN_THREADS, 2)
 own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PrefixArgs a) {
-    using C = Own<D>;
+    using C = Own<D, MT>;
     using E = vsa::Elt<T>;
     constexpr int WK = WARPS / MT, KW = UNIT / WK;            // warps that share a row tile, keys of a warp in a unit
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(smem);
     OwnCtl* ctl = reinterpret_cast<OwnCtl*>(smem + C::CTL);
-    long long* sums = reinterpret_cast<long long*>(smem + C::SCAN);
     volatile int* abort_flag = &ctl->abort;
+    launch_dependents();
     if (tid == 0) {
         const int earlier = *reinterpret_cast<volatile int*>(a.status);
         for (int i = 0; i < C::NSLOT; ++i) {
             mbar_init(smem_u32(&ctl->full[i]), 1);
             mbar_init(smem_u32(&ctl->empty[i]), WARPS);
         }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ctl->qfull[i]), 1);
+            mbar_init(smem_u32(&ctl->qempty[i]), WARPS);
+        }
+        mbar_init(smem_u32(&ctl->joined), WARPS);
         ctl->not_finite = 0;
+        ctl->first_b = -1;
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 913);
         mbar_fence_init();
         fence_proxy_async_smem();
     }
-    // running sums of the units over groups of requests
-    const Finder find{a, sums, max(1, (a.B + GROUPS - 1) / GROUPS)};
-    const int groups = (a.B + find.group - 1) / find.group, per = (groups + OWN_THREADS - 1) / OWN_THREADS;
+    // where the requests start: a running sum over all of them, a run of requests to a thread
+    const int items = a.vheads * a.blocks, run = (a.B + OWN_THREADS - 1) / OWN_THREADS, b0 = min(a.B, tid * run), b1 = min(a.B, b0 + run);
     long long mine = 0;
-    for (int g = tid * per; g < min(groups, (tid + 1) * per); ++g)
-        for (int b = g * find.group; b < min(a.B, (g + 1) * find.group); ++b) mine += find.units(b);
-    long long run = mine;
+    for (int b = b0; b < b1; ++b) mine += stretch(own_length(a, b), items);
+    long long x = mine;
     for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += y;
+        const long long y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
     }
-    if (lane == 31) ctl->warp_sum[warp] = run;
+    if (lane == 31) ctl->warp_sum[warp] = x;
     __syncthreads();
-    long long W = prefix_units(a);
-    run += W - mine;
+    long long W = prefix_stretch(a);
+    x += W - mine;
     for (int w = 0; w <= WARPS; ++w) {
-        if (w < warp) run += ctl->warp_sum[w];
+        if (w < warp) x += ctl->warp_sum[w];
         W += ctl->warp_sum[w];
     }
-    for (int g = tid * per; g < min(groups, (tid + 1) * per); ++g) {
-        sums[g] = run;
-        for (int b = g * find.group; b < min(a.B, (g + 1) * find.group); ++b) {
-            if (blockIdx.x == 0) a.first[b] = run;
-            run += find.units(b);
+    // (a CTA's stretch is never empty: no more CTAs than W)
+    const long long ctas = min((long long)a.ctas, W);
+    const bool busy = blockIdx.x < ctas;
+    const long long beg = busy ? W * blockIdx.x / ctas : 0, end = busy ? W * (blockIdx.x + 1) / ctas : 0;
+    if (blockIdx.x == 0 || (busy && x <= beg && beg < x + mine))
+        for (int b = b0; b < b1; ++b) {
+            const long long w = stretch(own_length(a, b), items);
+            if (blockIdx.x == 0) a.first[b] = x;
+            if (busy && x <= beg && beg < x + w) { ctl->first_b = b; ctl->first_x = beg - x; }
+            x += w;
         }
-    }
     if (blockIdx.x == 0 && tid == 0) a.first[a.B] = W;
     __syncthreads();
-    // (no more CTAs than units: each has one at least)
-    const long long ctas = min((long long)a.ctas, W);
-    const long long beg = blockIdx.x < ctas ? W * blockIdx.x / ctas : 0, end = blockIdx.x < ctas ? W * (blockIdx.x + 1) / ctas : 0;
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     bool ok = *abort_flag == 0;
 
     if (warp == WARPS) {
-        // ------------------------------------------------------------ loads: K and V of every unit, a lane per box
+        // ------------------------------------------------------------ loads: Q of every item, K and V of every unit, a lane per row or box
         const int box = min(UNIT, 1 << a.log_page), boxes = UNIT / box;
-        uint32_t slot = 0, par = 1, issued = 0;
+        uint32_t slot = 0, par = 1, issued = 0, unit = 0, item_no = 0;
         if (lane == 0) {
             tma_prefetch_desc(&tmK);
             tma_prefetch_desc(&tmV);
         }
-        for (long long u = beg; u < end && ok;) {
-            const Share s = find.at(u, end);
-            const int* list = s.b < 0 ? a.prefix_pages : a.table + (size_t)s.b * a.width;
-            const int kh = s.head0 / (a.H / a.Hk);
-            for (int i = s.u0; i < s.u1 && ok; ++i) {
-                const int k = i * UNIT + lane * box;
-                int page = a.pages;                           // a page that is not of the cache, or behind the keys, is loaded as zeros
-                if (lane < boxes && k < s.n) {
-                    const int p = __ldg(list + (k >> a.log_page));
-                    if (p >= 0 && p < a.pages) page = p;
-                }
-                for (int x = 0; x < 2 && ok; ++x) {
-                    ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 661);
-                    if (!ok) break;
-                    const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
-                    if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
-                    __syncwarp();
-                    if (lane < boxes)
-                        for (int d = 0; d < D / 64; ++d)
-                            tma_load_4d(dst + d * C::HALF + lane * box * 128, x ? &tmV : &tmK, bar, 64 * d, kh, (i * UNIT) & ((1 << a.log_page) - 1), page);
-                    __syncwarp();
-                    ++issued;
-                    if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+        long long left = end - beg;
+        int b = ctl->first_b;                                 // -1: in the prefix
+        int n = b < 0 ? a.prefix_len : own_length(a, b), units = units_of(n), item, y;
+        {
+            const long long at = b < 0 ? beg : ctl->first_x;
+            item = left > 0 ? (int)(at / (units + ITEM)) : 0;
+            y = left > 0 ? (int)(at - (long long)item * (units + ITEM)) : 0;
+        }
+        while (left > 0 && ok) {
+            const int y1 = (int)min((long long)units + ITEM, y + left), u0 = max(0, y - ITEM), u1 = max(0, y1 - ITEM);
+            if (u1 > u0) {
+                const int blk = b < 0 ? 0 : item / a.vheads, head0 = (item - blk * a.vheads) * a.pack;
+                const int tq = blk * a.per_block, t0 = b < 0 ? 0 : b * a.N + tq;
+                const int rows = (b < 0 ? a.B * a.N : min(a.per_block, a.N - tq)) * a.pack;
+                const int* list = b < 0 ? a.prefix_pages : a.table + (size_t)b * a.width;
+                const int kh = head0 / (a.H / a.Hk), qs = item_no & 1;
+                ok = mbar_wait_warp(smem_u32(&ctl->qempty[qs]), ((item_no >> 1) & 1) ^ 1, abort_flag, a.status, 664);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&ctl->qfull[qs]), (uint32_t)(rows * D * 2));
+                __syncwarp();
+                for (int r = lane; r < rows; r += 32)
+                    bulk_load(base + C::Q + qs * C::QTILE + r * C::QPITCH, static_cast<const T*>(a.q) + ((int64_t)(t0 + r / a.pack) * a.H + head0 + r % a.pack) * D,
+                              D * 2, smem_u32(&ctl->qfull[qs]));
+                ++item_no;
+                int win = 0, wbase = -1;                      // pages of the next 32 boxes
+                for (int i = u0; i < u1 && ok; ++i) {
+                    const int bx = i * boxes, w = bx & ~31;   // (8, 4, 2 or 1 boxes to a unit: a unit's are in one window)
+                    if (w != wbase) {
+                        wbase = w;
+                        const long long k = (long long)(w + lane) * box;
+                        win = k < n ? __ldg(list + (k >> a.log_page)) : -1;
+                    }
+                    const int p = __shfl_sync(0xffffffffu, win, (bx & 31) + (lane & (boxes - 1)));
+                    const bool good = p >= 0 && p < a.pages, needed = (long long)(bx + lane) * box < n;
+                    // a page that is not of the cache, or behind the keys, is loaded as zeros
+                    const int page = lane < boxes && needed && good ? p : a.pages;
+                    const uint32_t bad = __ballot_sync(0xffffffffu, lane < boxes && needed && !good);
+                    for (int x_ = 0; x_ < 2 && ok; ++x_) {
+                        ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 661);
+                        if (!ok) break;
+                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                        if (lane == 0) {
+                            // (the slot's last tenant was at least NSLOT tiles ago, its unit's copy of the descriptor long taken)
+                            if (x_ == 0)
+                                ctl->desc[unit & 3] = UnitDesc{i * UNIT, n, b, head0, t0, tq, rows, (i == u0 ? FIRST : 0) | (i + 1 == u1 ? LAST : 0) | (u0 == 0 ? STARTS : 0), bad};
+                            mbar_arrive_expect_tx(bar, C::TILE);
+                        }
+                        __syncwarp();
+                        if (lane < boxes)
+                            for (int d = 0; d < D / 64; ++d)
+                                tma_load_4d(dst + d * C::HALF + lane * box * 128, x_ ? &tmV : &tmK, bar, 64 * d, kh, (i * UNIT) & ((1 << a.log_page) - 1), page);
+                        __syncwarp();
+                        ++issued;
+                        if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+                    }
+                    ++unit;
                 }
             }
-            u += s.u1 - s.u0;
+            left -= y1 - y;
+            y = 0;
+            if (++item == (b < 0 ? a.vheads : items)) {
+                item = 0;
+                do {
+                    ++b;
+                    n = b < a.B ? own_length(a, b) : 0;
+                } while (b < a.B && n == 0);
+                if (b >= a.B) break;
+                units = units_of(n);
+            }
+        }
+        if (ok) ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 665);
+        if (ok && lane == 0) {
+            ctl->desc[unit & 3].k0 = -1;
+            mbar_arrive(full0 + 8 * slot);
         }
         __syncwarp();
         if (lane == 0 && *abort_flag) {
             // a wait gave up: give the loads a moment (100 us in all) to land before shared memory goes away
             const uint64_t t_end = global_timer_ns() + 100000ull;
+            for (uint32_t q = 0; q < 2 && q < item_no; ++q) {
+                const uint32_t it = item_no - 1 - q;
+                while (!mbar_try_wait(smem_u32(&ctl->qfull[it & 1]), (it >> 1) & 1) && global_timer_ns() < t_end) {}
+            }
             for (uint32_t back = 1; back <= (uint32_t)C::NSLOT && back <= issued; ++back) {
                 const uint32_t sq = issued - back;
                 while (!mbar_try_wait(full0 + 8 * (sq % C::NSLOT), (sq / C::NSLOT) & 1) && global_timer_ns() < t_end) {}
@@ -221,259 +246,305 @@ own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUte
         const int mt = warp / WK, wk = warp % WK;             // row tile, share of the keys
         const int r0 = 16 * mt + (lane >> 2), r1 = r0 + 8;
         const float c = a.scale * kLog2e;
-        uint32_t seq = 0;
-        for (long long u = beg; u < end;) {
-            const Share s = find.at(u, end);
-            const int* list = s.b < 0 ? a.prefix_pages : a.table + (size_t)s.b * a.width;
+        const int box = min(UNIT, 1 << a.log_page), box_log = 31 - __clz(box);
+        uint32_t slot = 0, par = 0, unit = 0, item_no = 0;
+        uint32_t qf[D / 16][4];
+        float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        int from = 0;                                         // first unit's first key of the share
+        uint32_t join_par = 0;
+        // a barrier of the four warps whose wait is bounded: one that gave up elsewhere comes no more
+        auto together = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->joined));
+            ok = mbar_wait_warp(smem_u32(&ctl->joined), join_par, abort_flag, a.status, 667);
+            join_par ^= 1;
+            return ok;
+        };
+        while (ok) {
+            ok = mbar_wait_warp(full0 + 8 * slot, par, abort_flag, a.status, 662);
+            if (!ok) break;
+            const UnitDesc u = ctl->desc[unit++ & 3];
+            if (u.k0 < 0) break;
             // keys that the thread's two rows see, and the fewest and most that any row of the item sees
-            auto seen = [&](int row) {
-                if (s.b < 0) return s.n;
-                const int t = s.t0 - s.b * a.N + row / a.pack;
-                return max(s.n - a.N + t + 1, 0);
-            };
-            const int v0 = r0 < s.rows ? seen(r0) : 0, v1 = r1 < s.rows ? seen(r1) : 0, least = seen(0), most = seen(s.rows - 1);
-            uint32_t qf[D / 16][4];
-            const T* q = static_cast<const T*>(a.q);
-            auto q_at = [&](int row) { return q + ((int64_t)(s.t0 + row / a.pack) * a.H + s.head0 + row % a.pack) * D + 2 * (lane & 3); };
+            auto seen = [&](int row) { return u.b < 0 ? u.n : max(u.n - a.N + u.tq + row / a.pack + 1, 0); };
+            const int v0 = r0 < u.rows ? seen(r0) : 0, v1 = r1 < u.rows ? seen(r1) : 0, least = seen(0);
+            if (u.flags & FIRST) {
+                const int qs = item_no & 1;
+                ok = mbar_wait_warp(smem_u32(&ctl->qfull[qs]), (item_no >> 1) & 1, abort_flag, a.status, 666);
+                if (!ok) break;
+                // 16 rows x 16 d: lanes 0-15 rows 0-15 of d 0-7, lanes 16-31 of d 8-15
+                const uint32_t qa = base + C::Q + qs * C::QTILE + (16 * mt + (lane & 15)) * C::QPITCH + (lane >> 4) * 16;
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                qf[ks][0] = r0 < s.rows ? *reinterpret_cast<const uint32_t*>(q_at(r0) + 16 * ks) : 0u;
-                qf[ks][1] = r1 < s.rows ? *reinterpret_cast<const uint32_t*>(q_at(r1) + 16 * ks) : 0u;
-                qf[ks][2] = r0 < s.rows ? *reinterpret_cast<const uint32_t*>(q_at(r0) + 16 * ks + 8) : 0u;
-                qf[ks][3] = r1 < s.rows ? *reinterpret_cast<const uint32_t*>(q_at(r1) + 16 * ks + 8) : 0u;
+                for (int ks = 0; ks < D / 16; ++ks) vsa::ldsm4(qa + 32 * ks, qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->qempty[qs]));
+                ++item_no;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+                m0 = m1 = -INFINITY;
+                l0 = l1 = 0.f;
+                from = u.k0;
             }
-            float o[D / 8][4];
+            const int k0 = u.k0 + wk * KW;                    // this warp's keys k0 .. k0 + KW - 1
+            float x[KW / 8][4];
+            const uint32_t kb = base + C::RING + slot * C::TILE;
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-            for (int i = s.u0; i < s.u1; ++i) {
-                const int k0 = i * UNIT + wk * KW;            // this warp's keys k0 .. k0 + KW - 1
-                uint32_t slot = seq % C::NSLOT;
-                ok = ok && mbar_wait_warp(full0 + 8 * slot, (seq / C::NSLOT) & 1, abort_flag, a.status, 662);
-                ++seq;
-                float x[KW / 8][4];
-                if (ok) {
-                    const uint32_t kb = base + C::RING + slot * C::TILE;
+            for (int j = 0; j < KW / 8; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < KW / 8; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+            for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks)
+                for (int j = 0; j < KW / 16; ++j) {
+                    // 16 keys x 16 d: lanes 0-7, 8-15 keys 0-7 (d 0-7, 8-15), lanes 16-31 keys 8-15
+                    const int row = wk * KW + 16 * j + (lane & 7) + ((lane >> 4) << 3), ch = 2 * (ks & 3) + ((lane >> 3) & 1);
+                    uint32_t f0, f1, f2, f3;
+                    vsa::ldsm4(kb + (ks >> 2) * C::HALF + row * 128 + ((ch ^ (row & 7)) << 4), f0, f1, f2, f3);
+                    E::mma(x[2 * j], qf[ks], f0, f1);
+                    E::mma(x[2 * j + 1], qf[ks], f2, f3);
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * slot);
+            if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+            if (u.k0 + UNIT > least) {
 #pragma unroll
-                        for (int j = 0; j < KW / 16; ++j) {
-                            // 16 keys x 16 d: lanes 0-7, 8-15 rows 0-7 (d 0-7, 8-15), lanes 16-31 rows 8-15
-                            const int row = wk * KW + 16 * j + (lane & 7) + ((lane >> 4) << 3), ch = 2 * (ks & 3) + ((lane >> 3) & 1);
-                            uint32_t b0, b1, b2, b3;
-                            vsa::ldsm4(kb + (ks >> 2) * C::HALF + row * 128 + ((ch ^ (row & 7)) << 4), b0, b1, b2, b3);
-                            E::mma(x[2 * j], qf[ks], b0, b1);
-                            E::mma(x[2 * j + 1], qf[ks], b2, b3);
-                        }
-                    // a page that is not of the cache: its keys are not attended to
-                    if (i * UNIT + UNIT > least) {
+                for (int j = 0; j < KW / 8; ++j) {
+                    const int k = k0 + 8 * j + 2 * (lane & 3);
+                    if (k >= v0) x[j][0] = -INFINITY;
+                    if (k + 1 >= v0) x[j][1] = -INFINITY;
+                    if (k >= v1) x[j][2] = -INFINITY;
+                    if (k + 1 >= v1) x[j][3] = -INFINITY;
+                }
+            }
+            if (u.bad)
 #pragma unroll
-                        for (int j = 0; j < KW / 8; ++j) {
-                            const int k = k0 + 8 * j + 2 * (lane & 3);
-                            if (k >= v0) x[j][0] = -INFINITY;
-                            if (k + 1 >= v0) x[j][1] = -INFINITY;
-                            if (k >= v1) x[j][2] = -INFINITY;
-                            if (k + 1 >= v1) x[j][3] = -INFINITY;
-                        }
-                    }
-                    const int kp = k0 + 16 * lane;             // (pages hold 16 keys at least)
-                    const int pg = 16 * lane < KW && kp < s.n ? __ldg(list + (kp >> a.log_page)) : 0;
-                    const uint32_t bad = __ballot_sync(0xffffffffu, pg < 0 || pg >= a.pages);
-                    if (bad)
+                for (int j = 0; j < KW / 8; ++j)
+                    if ((u.bad >> ((wk * KW + 8 * j) >> box_log)) & 1) x[j][0] = x[j][1] = x[j][2] = x[j][3] = -INFINITY;
+            float y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < KW / 8; ++j)
-                            if ((bad >> (j / 2)) & 1) x[j][0] = x[j][1] = x[j][2] = x[j][3] = -INFINITY;
-                    float y0 = -INFINITY, y1 = -INFINITY;
+            for (int j = 0; j < KW / 8; ++j) {
+                y0 = fmaxf(y0, fmaxf(x[j][0], x[j][1]));
+                y1 = fmaxf(y1, fmaxf(x[j][2], x[j][3]));
+            }
+            y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 1));
+            y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 1));
+            y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 2)) * c;
+            y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2)) * c;
+            if (__any_sync(0xffffffffu, y0 > m0 || y1 > m1)) {
+                const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+                const float f0 = n0 == -INFINITY ? 1.f : ex2_approx(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2_approx(m1 - n1);
+                m0 = n0; m1 = n1;
+                l0 *= f0; l1 *= f1;
 #pragma unroll
-                    for (int j = 0; j < KW / 8; ++j) {
-                        y0 = fmaxf(y0, fmaxf(x[j][0], x[j][1]));
-                        y1 = fmaxf(y1, fmaxf(x[j][2], x[j][3]));
-                    }
-                    y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 1));
-                    y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 1));
-                    y0 = fmaxf(y0, __shfl_xor_sync(0xffffffffu, y0, 2)) * c;
-                    y1 = fmaxf(y1, __shfl_xor_sync(0xffffffffu, y1, 2)) * c;
-                    if (__any_sync(0xffffffffu, y0 > m0 || y1 > m1)) {
-                        const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
-                        const float f0 = n0 == -INFINITY ? 1.f : ex2_approx(m0 - n0), f1 = n1 == -INFINITY ? 1.f : ex2_approx(m1 - n1);
-                        m0 = n0; m1 = n1;
-                        l0 *= f0; l1 *= f1;
+                for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+            }
+            const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
 #pragma unroll
-                        for (int j = 0; j < D / 8; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
-                    }
-                    const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
-#pragma unroll
-                    for (int j = 0; j < KW / 8; ++j) {
-                        x[j][0] = ex2_approx(fmaf(x[j][0], c, z0));
-                        x[j][1] = ex2_approx(fmaf(x[j][1], c, z0));
-                        x[j][2] = ex2_approx(fmaf(x[j][2], c, z1));
-                        x[j][3] = ex2_approx(fmaf(x[j][3], c, z1));
-                        l0 += x[j][0] + x[j][1];
-                        l1 += x[j][2] + x[j][3];
+            for (int j = 0; j < KW / 8; ++j) {
+                x[j][0] = ex2_approx(fmaf(x[j][0], c, z0));
+                x[j][1] = ex2_approx(fmaf(x[j][1], c, z0));
+                x[j][2] = ex2_approx(fmaf(x[j][2], c, z1));
+                x[j][3] = ex2_approx(fmaf(x[j][3], c, z1));
+                l0 += x[j][0] + x[j][1];
+                l1 += x[j][2] + x[j][3];
+            }
+            ok = mbar_wait_warp(full0 + 8 * slot, par, abort_flag, a.status, 663);
+            if (!ok) break;
+            if (k0 + KW > least) {
+                // V rows that some row does not see: what is not finite there is set to 0 (0 times it would be NaN), and given at the end to the
+                // rows that do see it
+                for (int e = lane; e < KW * (D / 8); e += 32) {
+                    const int row = wk * KW + e / (D / 8), ch = e % (D / 8);
+                    uint4* p = reinterpret_cast<uint4*>(smem + C::RING + slot * C::TILE + (ch >> 3) * C::HALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+                    const uint4 w = *p;
+                    if (u.k0 + row >= least && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w))) {
+                        if (u.k0 + row < u.n) *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
+                        *p = make_uint4(finite_only<T>(w.x), finite_only<T>(w.y), finite_only<T>(w.z), finite_only<T>(w.w));
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(empty0 + 8 * slot);
-                slot = seq % C::NSLOT;
-                ok = ok && mbar_wait_warp(full0 + 8 * slot, (seq / C::NSLOT) & 1, abort_flag, a.status, 663);
-                ++seq;
-                if (ok) {
-                    const uint32_t vb = base + C::RING + slot * C::TILE;
-                    if (k0 + KW > least) {
-                        // V rows that some row does not see: what is not finite there is set to 0 (0 times it would be NaN), and given at the end to
-                        // the rows that do see it
-                        for (int e = lane; e < KW * (D / 8); e += 32) {
-                            const int row = wk * KW + e / (D / 8), ch = e % (D / 8);
-                            uint4* p = reinterpret_cast<uint4*>(smem + C::RING + slot * C::TILE + (ch >> 3) * C::HALF + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-                            const uint4 w = *p;
-                            if (i * UNIT + row >= least && (not_finite<T>(w.x) || not_finite<T>(w.y) || not_finite<T>(w.z) || not_finite<T>(w.w))) {
-                                if (i * UNIT + row < most) *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
-                                *p = make_uint4(finite_only<T>(w.x), finite_only<T>(w.y), finite_only<T>(w.z), finite_only<T>(w.w));
-                            }
-                        }
-                        __syncwarp();
-                        fence_proxy_async_smem();
-                    }
-#pragma unroll
-                    for (int j = 0; j < KW / 16; ++j) {
-                        const uint32_t p[4] = {pack2<T>(x[2 * j][0], x[2 * j][1]), pack2<T>(x[2 * j][2], x[2 * j][3]), pack2<T>(x[2 * j + 1][0], x[2 * j + 1][1]),
-                                               pack2<T>(x[2 * j + 1][2], x[2 * j + 1][3])};
-#pragma unroll
-                        for (int d = 0; d < D / 16; ++d) {
-                            // 16 keys x 16 d, transposed: lanes 0-15 keys 0-15 of d 0-7, lanes 16-31 of d 8-15
-                            const int row = wk * KW + 16 * j + (lane & 15), ch = 2 * (d & 3) + (lane >> 4);
-                            uint32_t b0, b1, b2, b3;
-                            ldsm4_trans(vb + (d >> 2) * C::HALF + row * 128 + ((ch ^ (row & 7)) << 4), b0, b1, b2, b3);
-                            E::mma(o[2 * d], p, b0, b1);
-                            E::mma(o[2 * d + 1], p, b2, b3);
-                        }
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty0 + 8 * slot);
+                fence_proxy_async_smem();
             }
+            const uint32_t vb = base + C::RING + slot * C::TILE;
+#pragma unroll
+            for (int j = 0; j < KW / 16; ++j) {
+                const uint32_t p[4] = {pack2<T>(x[2 * j][0], x[2 * j][1]), pack2<T>(x[2 * j][2], x[2 * j][3]), pack2<T>(x[2 * j + 1][0], x[2 * j + 1][1]),
+                                       pack2<T>(x[2 * j + 1][2], x[2 * j + 1][3])};
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    // 16 keys x 16 d, transposed: lanes 0-15 keys 0-15 of d 0-7, lanes 16-31 of d 8-15
+                    const int row = wk * KW + 16 * j + (lane & 15), ch = 2 * (d & 3) + (lane >> 4);
+                    uint32_t f0, f1, f2, f3;
+                    ldsm4_trans(vb + (d >> 2) * C::HALF + row * 128 + ((ch ^ (row & 7)) << 4), f0, f1, f2, f3);
+                    E::mma(o[2 * d], p, f0, f1);
+                    E::mma(o[2 * d + 1], p, f2, f3);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * slot);
+            if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
+            if (!(u.flags & LAST)) continue;
+            // ---- the share is done: join the warps that have its rows, and store it
             l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
             l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
             l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
             l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-            // (another warp with the same keys may have found it)
-            if (least < most) named_sync(1, 32 * WARPS);
-            if (least < most && *reinterpret_cast<volatile int*>(&ctl->not_finite)) {
-                const int kh = s.head0 / (a.H / a.Hk);
-                for (int k = max(least, s.u0 * UNIT); k < min(most, s.u1 * UNIT); ++k) {
-                    const int p = __ldg(list + (k >> a.log_page));
-                    if ((k % UNIT) / KW != wk || p < 0 || p >= a.pages) continue;
-                    const T* vr = static_cast<const T*>(a.v) + p * a.rv.page + (int64_t)(k & ((1 << a.log_page) - 1)) * a.rv.token + (int64_t)kh * a.rv.head + 2 * (lane & 3);
+            if (least < u.n) {
+                if (!together()) break;                       // (another warp with the same keys may have found it)
+                if (*reinterpret_cast<volatile int*>(&ctl->not_finite)) {
+                    const int* list = u.b < 0 ? a.prefix_pages : a.table + (size_t)u.b * a.width;
+                    const int kh = u.head0 / (a.H / a.Hk);
+                    for (int k = max(least, from); k < min(u.n, u.k0 + UNIT); ++k) {
+                        const int p = __ldg(list + (k >> a.log_page));
+                        if ((k % UNIT) / KW != wk || p < 0 || p >= a.pages) continue;
+                        const T* vr = static_cast<const T*>(a.v) + p * a.rv.page + (int64_t)(k & ((1 << a.log_page) - 1)) * a.rv.token + (int64_t)kh * a.rv.head + 2 * (lane & 3);
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
+                        for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float f = to_float(vr[8 * j + e]);
-                            if (fabsf(f) < INFINITY) continue;
-                            if (k < v0) o[j][e] += f;
-                            if (k < v1) o[j][2 + e] += f;
-                        }
+                            for (int e = 0; e < 2; ++e) {
+                                const float f = to_float(vr[8 * j + e]);
+                                if (fabsf(f) < INFINITY) continue;
+                                if (k < v0) o[j][e] += f;
+                                if (k < v1) o[j][2 + e] += f;
+                            }
+                    }
                 }
             }
-            // join the warps that share the rows, halving their number
+            float f0 = 1.f, f1 = 1.f;                         // factors of this warp's own sums (MT = 4: the only ones)
+            float lt0 = l0, lt1 = l1, mt0 = m0, mt1 = m1;
             float* sum = reinterpret_cast<float*>(smem + C::SUM);
+            if constexpr (WK > 1) {
+                if (!together()) break;                       // the share before has been read
+                if ((lane & 3) == 0) {
+                    ctl->ml[warp][lane >> 2] = m0; ctl->ml[warp][8 + (lane >> 2)] = m1;
+                    ctl->ml[warp][16 + (lane >> 2)] = l0; ctl->ml[warp][24 + (lane >> 2)] = l1;
+                }
 #pragma unroll
-            for (int half = WK / 2; half; half >>= 1) {
-                const int pair = mt * half + (wk % half);
-                float* dst = sum + (size_t)pair * 16 * D;
-                if (wk >= half && wk < 2 * half) {
+                for (int j = 0; j < D / 8; ++j)
+                    *reinterpret_cast<float4*>(sum + (warp * 16 * D) + (j * 32 + lane) * 4) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+                if (!together()) break;
+                mt0 = mt1 = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j) {
-                        *reinterpret_cast<float4*>(dst + (j * 32 + lane) * 4) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-                    }
-                    if ((lane & 3) == 0) {
-                        ctl->ml[pair][lane >> 2] = m0; ctl->ml[pair][8 + (lane >> 2)] = m1;
-                        ctl->ml[pair][16 + (lane >> 2)] = l0; ctl->ml[pair][24 + (lane >> 2)] = l1;
+                for (int w = 0; w < WK; ++w) {
+                    mt0 = fmaxf(mt0, ctl->ml[mt * WK + w][lane >> 2]);
+                    mt1 = fmaxf(mt1, ctl->ml[mt * WK + w][8 + (lane >> 2)]);
+                }
+                lt0 = lt1 = 0.f;
+            }
+            constexpr int JN = D / 8 / WK;                    // every warp stores a share of the columns
+            float acc[JN][4];
+            if constexpr (WK > 1) {
+#pragma unroll
+                for (int j = 0; j < JN; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const int src = mt * WK + w;
+                    f0 = mt0 == -INFINITY ? 0.f : ex2_approx(ctl->ml[src][lane >> 2] - mt0);
+                    f1 = mt1 == -INFINITY ? 0.f : ex2_approx(ctl->ml[src][8 + (lane >> 2)] - mt1);
+                    lt0 += ctl->ml[src][16 + (lane >> 2)] * f0;
+                    lt1 += ctl->ml[src][24 + (lane >> 2)] * f1;
+#pragma unroll
+                    for (int j = 0; j < JN; ++j) {
+                        const float4 v = *reinterpret_cast<const float4*>(sum + src * 16 * D + ((wk * JN + j) * 32 + lane) * 4);
+                        acc[j][0] += v.x * f0; acc[j][1] += v.y * f0; acc[j][2] += v.z * f1; acc[j][3] += v.w * f1;
                     }
                 }
-                named_sync(1, 32 * WARPS);
-                if (wk < half) {
-                    const float n0 = ctl->ml[pair][lane >> 2], n1 = ctl->ml[pair][8 + (lane >> 2)], t0 = fmaxf(m0, n0), t1 = fmaxf(m1, n1);
-                    const float f0 = t0 == -INFINITY ? 0.f : ex2_approx(m0 - t0), f1 = t1 == -INFINITY ? 0.f : ex2_approx(m1 - t1);
-                    const float g0 = t0 == -INFINITY ? 0.f : ex2_approx(n0 - t0), g1 = t1 == -INFINITY ? 0.f : ex2_approx(n1 - t1);
-                    l0 = l0 * f0 + ctl->ml[pair][16 + (lane >> 2)] * g0;
-                    l1 = l1 * f1 + ctl->ml[pair][24 + (lane >> 2)] * g1;
-                    m0 = t0; m1 = t1;
+            } else {
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j) {
-                        const float4 w = *reinterpret_cast<const float4*>(dst + (j * 32 + lane) * 4);
-                        o[j][0] = o[j][0] * f0 + w.x * g0; o[j][1] = o[j][1] * f0 + w.y * g0;
-                        o[j][2] = o[j][2] * f1 + w.z * g1; o[j][3] = o[j][3] * f1 + w.w * g1;
-                    }
-                }
-                named_sync(1, 32 * WARPS);
-            }
-            if (wk == 0) {
-                const float i0 = l0 != 0.f ? 1.f / l0 : 0.f, i1 = l1 != 0.f ? 1.f / l1 : 0.f;
-                auto store = [&](int row, float m, float l, float inv, int e) {
-                    if (row >= s.rows) return;
-                    const int64_t at = (int64_t)(s.t0 + row / a.pack) * a.H + s.head0 + row % a.pack;
-                    float* dst = s.starts ? (s.b < 0 ? a.p_o : a.a_o) + at * D : a.b_o + ((int64_t)blockIdx.x * ROWS + row) * D;
-                    float* z = s.starts ? (s.b < 0 ? a.p_lse : a.a_lse) + at : a.b_lse + (int64_t)blockIdx.x * ROWS + row;
-                    const bool lost = *abort_flag != 0;       // a wait gave up: NaN
+                for (int j = 0; j < JN; ++j)
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
-                        *reinterpret_cast<float2*>(dst + 8 * j + 2 * (lane & 3)) =
-                            lost ? make_float2(__uint_as_float(kNaN32), __uint_as_float(kNaN32)) : make_float2(o[j][e] * inv, o[j][e + 1] * inv);
-                    if ((lane & 3) == 0) *z = lost ? __uint_as_float(kNaN32) : l != 0.f ? m + log2f(l) : -INFINITY;
-                };
-                store(r0, m0, l0, i0, 0);
-                store(r1, m1, l1, i1, 2);
+                    for (int e = 0; e < 4; ++e) acc[j][e] = o[j][e];
             }
-            u += s.u1 - s.u0;
+            auto store = [&](int row, float m, float l, int e) {
+                if (row >= u.rows) return;
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+                const int64_t at = (int64_t)(u.t0 + row / a.pack) * a.H + u.head0 + row % a.pack;
+                const bool starts = u.flags & STARTS;
+                float* dst = (starts ? (u.b < 0 ? a.p_o : a.a_o) + at * D : a.b_o + ((int64_t)blockIdx.x * ROWS + row) * D) + 8 * JN * wk + 2 * (lane & 3);
+                float* z = starts ? (u.b < 0 ? a.p_lse : a.a_lse) + at : a.b_lse + (int64_t)blockIdx.x * ROWS + row;
+#pragma unroll
+                for (int j = 0; j < JN; ++j)
+                    *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(acc[j][e] * inv, acc[j][e + 1] * inv);
+                if (wk == 0 && (lane & 3) == 0) *z = l != 0.f ? m + log2f(l) : -INFINITY;
+            };
+            store(r0, mt0, lt0, 0);
+            store(r1, mt1, lt1, 2);
         }
     }
+    // the join waits for this kernel, this kernel for the one of the prefix
+    wait_prerequisites();
     __syncthreads();
 }
 
-// A warp per row: the parts of the prefix, part A of the row's own item, and the part B's of the CTAs that went on with it.
+// A warp per row: the parts of the prefix, part A of the row's own item, and the part B's of the CTAs that went on with it. A lane looks
+// up a part's LSE, so that a row costs two round trips to memory and not two per part.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(T* o, float* lse, const __grid_constant__ PrefixArgs a) {
     constexpr int C = D / 32;
     const int lane = threadIdx.x & 31;
     const int64_t rows = (int64_t)a.B * a.N * a.H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    wait_prerequisites();
     if (row >= rows) return;
     const int h = (int)(row % a.H), t = (int)(row / a.H), b = t / a.N, i = t % a.N, vh = h / a.pack;
-    float acc[C] = {}, sum = 0.f, top = -INFINITY;
-    auto add = [&](const float* src, float z) {
-        if (z == -INFINITY) return;
-        const float next = fmaxf(top, z), f = ex2_approx(top - next), g = z != z ? z : ex2_approx(z - next);
-        top = next;
-        sum = sum * f + g;
-        if constexpr (C == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src + C * lane);
-            acc[0] = acc[0] * f + v.x * g; acc[1] = acc[1] * f + v.y * g; acc[2] = acc[2] * f + v.z * g; acc[3] = acc[3] * f + v.w * g;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(src + C * lane);
-            acc[0] = acc[0] * f + v.x * g; acc[1] = acc[1] * f + v.y * g;
-        }
-    };
     const long long W = a.first ? a.first[a.B] : 0, ctas = min((long long)a.ctas, W);
-    // an item's parts: A, and B of the CTAs after the one with its first unit up to the one with its last
-    auto item = [&](long long u, long long units, const float* po, const float* pl, int r) {
-        if (units <= 0) return;
-        add(po + row * D, pl[row]);
-        const int c0 = (int)(((u + 1) * ctas - 1) / W), c1 = (int)(((u + units) * ctas - 1) / W);
-        for (int c = c0 + 1; c <= c1; ++c) add(a.b_o + ((int64_t)c * ROWS + r) * D, a.b_lse[(int64_t)c * ROWS + r]);
+    // parts of an item: A, and B of the CTAs after the one with its first unit up to the one with its last
+    struct Item { int n, c0; };
+    auto item_at = [&](long long start, int units) {
+        Item it{0, 0};
+        if (units > 0) {
+            it.c0 = (int)(((start + ITEM + 1) * ctas - 1) / W);
+            it.n = 1 + (int)(((start + ITEM + units) * ctas - 1) / W) - it.c0;
+        }
+        return it;
     };
-    if (a.prefix_item) {
-        const long long n = (a.prefix_len + UNIT - 1) / UNIT;
-        item(vh * n, n, a.p_o, a.p_lse, t * a.pack + h % a.pack);
-    } else {
-        for (int p = 0; p < a.p_parts; ++p) add(a.p_o + (p * rows + row) * D, a.p_lse[p * rows + row]);
+    const int pu = a.prefix_item ? units_of(a.prefix_len) : 0, own = a.first ? units_of(own_length(a, b)) : 0, blk = i / a.per_block;
+    const Item pi = a.prefix_item ? item_at((long long)vh * (pu + ITEM), pu) : Item{a.p_parts, 0};
+    const Item oi = own ? item_at(a.first[b] + (long long)(blk * a.vheads + vh) * (own + ITEM), own) : Item{0, 0};
+    const int parts = pi.n + oi.n, pr = t * a.pack + h % a.pack, orow = (i - blk * a.per_block) * a.pack + h % a.pack;
+    // where part p lies: its row of D floats; its LSE
+    auto find = [&](int p, const float*& src, const float*& z) {
+        if (p < pi.n && !a.prefix_item) { src = a.p_o + (p * rows + row) * D; z = a.p_lse + p * rows + row; return; }
+        const bool pre = p < pi.n;
+        const int q = pre ? p : p - pi.n, r = pre ? pr : orow;
+        const int64_t slot = (int64_t)((pre ? pi.c0 : oi.c0) + q) * ROWS + r;
+        src = q ? a.b_o + slot * D : (pre ? a.p_o : a.a_o) + row * D;
+        z = q ? a.b_lse + slot : (pre ? a.p_lse : a.a_lse) + row;
+    };
+    float acc[C] = {}, sum = 0.f, top = -INFINITY;
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+        const float *src = nullptr, *zp = nullptr;
+        float z = -INFINITY;
+        if (p0 + lane < parts) {
+            find(p0 + lane, src, zp);
+            z = *zp;
+        }
+        float next = fmaxf(top, z);
+        for (int d = 16; d; d >>= 1) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
+        if (next > top) {
+            const float f = ex2_approx(top - next);           // (0 at first)
+            sum *= f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] *= f;
+            top = next;
+        }
+        // NaN, or +infinity, makes the row NaN; -infinity is a part without a key: what it holds is not read
+        const float w = z == -INFINITY ? 0.f : z != z ? z : ex2_approx(z - top);
+        const int n = min(32, parts - p0);
+#pragma unroll 4
+        for (int p = 0; p < n; ++p) {
+            const float wp = __shfl_sync(0xffffffffu, w, p);
+            const float* sp = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), p));
+            if (__shfl_sync(0xffffffffu, z, p) == -INFINITY) continue;
+            sum += wp;
+            if constexpr (C == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(sp + C * lane);
+                acc[0] += v.x * wp; acc[1] += v.y * wp; acc[2] += v.z * wp; acc[3] += v.w * wp;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(sp + C * lane);
+                acc[0] += v.x * wp; acc[1] += v.y * wp;
+            }
+        }
     }
-    if (a.first) {
-        const long long n = (own_length(a, b) + UNIT - 1) / UNIT;
-        const int blk = i / a.per_block;
-        item(a.first[b] + (blk * a.vheads + vh) * n, n, a.a_o, a.a_lse, (i - blk * a.per_block) * a.pack + h % a.pack);
-    }
+    // a wait gave up, here or earlier: parts are missing
+    if (*reinterpret_cast<volatile int*>(a.status) != 0) sum = __uint_as_float(kNaN32);
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
     for (int c = 0; c < C / 2; ++c)
@@ -539,15 +610,29 @@ Plan make_plan(int B, int N, int H, int Hk, int D, int prefix_len, int width) {
     return p;
 }
 
-template <typename T, int D> int launch_own(const void* k, CacheRows rk, const void* v, CacheRows rv, const PrefixArgs& a, int row_tiles, cudaStream_t st) {
+template <typename T, int D, int MT>
+int launch_own(const CUtensorMap& tk, const CUtensorMap& tv, const PrefixArgs& a, bool behind_prefix, cudaStream_t st) {
+    auto kern = own_kernel<T, D, MT>;
+    constexpr int bytes = (int)Own<D, MT>::BYTES;
+    if (int rc = opt_in_shared_memory((const void*)kern, bytes)) return rc;
+    // behind the kernel of the prefix it may start as that one's CTAs end: they have nothing to do with one another
+    if (behind_prefix) {
+        const cudaError_t e = launch_dependent(kern, dim3(a.ctas), dim3(OWN_THREADS), bytes, st, tk, tv, a);
+        if (e != cudaSuccess) return set_error(-2, cudaGetErrorString(e));
+    } else {
+        kern<<<a.ctas, OWN_THREADS, bytes, st>>>(tk, tv, a);
+    }
+    ES_CHECK_LAUNCH("own_kernel");
+    return 0;
+}
+
+template <typename T, int D>
+int launch_own(const void* k, CacheRows rk, const void* v, CacheRows rv, const PrefixArgs& a, int row_tiles, bool behind_prefix, cudaStream_t st) {
     CUtensorMap tk, tv;
     if (int rc = make_pages_map<T>(&tk, k, D, a.Hk, 1 << a.log_page, a.pages, rk, UNIT)) return rc;
     if (int rc = make_pages_map<T>(&tv, v, D, a.Hk, 1 << a.log_page, a.pages, rv, UNIT)) return rc;
-    auto kern = row_tiles == 1 ? own_kernel<T, D, 1> : row_tiles == 2 ? own_kernel<T, D, 2> : own_kernel<T, D, 4>;
-    if (int rc = opt_in_shared_memory((const void*)kern, (int)Own<D>::BYTES)) return rc;
-    kern<<<a.ctas, OWN_THREADS, Own<D>::BYTES, st>>>(tk, tv, a);
-    ES_CHECK_LAUNCH("own_kernel");
-    return 0;
+    return row_tiles == 1 ? launch_own<T, D, 1>(tk, tv, a, behind_prefix, st) : row_tiles == 2 ? launch_own<T, D, 2>(tk, tv, a, behind_prefix, st)
+                                                                                              : launch_own<T, D, 4>(tk, tv, a, behind_prefix, st);
 }
 
 }  // namespace
@@ -607,8 +692,9 @@ extern "C" int es_prefix_attn(const void* q, const void* k_cache, const void* v_
     auto go = [&](auto t, auto d) {
         using T = decltype(t);
         if (p.own)
-            if (int rc = launch_own<T, d>(k_cache, rk, v_cache, rv, a, p.row_tiles, st)) return rc;
-        join_kernel<T, d><<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>((T*)o, lse, a);
+            if (int rc = launch_own<T, d>(k_cache, rk, v_cache, rv, a, p.row_tiles, p.prefix_tiles, st)) return rc;
+        const cudaError_t e = launch_dependent(join_kernel<T, d>, dim3((unsigned)((p.rows + 7) / 8)), dim3(256), 0, st, (T*)o, lse, a);
+        if (e != cudaSuccess) return set_error(-2, cudaGetErrorString(e));
         ES_CHECK_LAUNCH("join_kernel");
         return 0;
     };
