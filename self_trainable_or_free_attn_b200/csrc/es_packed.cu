@@ -63,7 +63,8 @@ extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, v
     if (int rc = check_sizes("es_packed_attn_fwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
     if (total_q == 0) return 0;
     if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v))) return set_error(-1, "es_packed_attn_fwd: null pointer");
-    if (!aligned(16, q, k, v, o, o_rest)) return set_error(-1, "es_packed_attn_fwd: q, k, v, o, o_rest must be 16-byte aligned");
+    if (!aligned(16, q, k, v, workspace) || !aligned(32, o, o_rest))
+        return set_error(-1, "es_packed_attn_fwd: q, k, v and the workspace must be 16-byte, o and o_rest 32-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head)) return set_error(-1, "es_packed_attn_fwd: strides must be multiples of 8 elements");
     const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
     return packed_fwd_tc(q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, o, o_rest, lse, b, D, dtype, workspace, (cudaStream_t)stream);

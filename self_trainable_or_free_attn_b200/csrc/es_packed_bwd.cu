@@ -45,27 +45,6 @@ struct BwdArgs {
     int* status;
 };
 
-// Row r of the tile at `tile`, its values that are not finite set to 0; whether there were any.
-template <typename T, int D> __device__ __forceinline__ bool clean_row(uint8_t* tile, int r) {
-    uint8_t* row = tile + r * 128;
-    bool any = false;
-#pragma unroll
-    for (int d = 0; d < D / 64; ++d)
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-            const uint4 v = *reinterpret_cast<const uint4*>(row + d * HALF + 16 * (ch ^ (r & 7)));
-            any |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
-        }
-    if (any) {
-        for (int d = 0; d < D / 64; ++d)
-            for (int ch = 0; ch < 8; ++ch) {
-                uint4* v = reinterpret_cast<uint4*>(row + d * HALF + 16 * ch);
-                *v = make_uint4(finite_only<T>(v->x), finite_only<T>(v->y), finite_only<T>(v->z), finite_only<T>(v->w));
-            }
-    }
-    return any;
-}
-
 template <typename T, int D> __device__ __forceinline__ void store_row(T* dst, uint32_t tcol, int from, int to, bool any, bool valid, float factor) {
 #pragma unroll 1
     for (int h = from; h < to; ++h) {

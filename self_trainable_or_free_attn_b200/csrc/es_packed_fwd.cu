@@ -29,17 +29,30 @@ constexpr float RAISE = 8.f;                                 // log2 of the fact
 template <int D> struct Cfg {
     static constexpr uint32_t TILE = TM * D * 2;             // [d half][128 rows][128 B]
     static constexpr int NSLOT = D == 128 ? 5 : 10;
-    static constexpr uint32_t Q = 0, RING = 2 * TILE, CTL = RING + NSLOT * TILE, BYTES = CTL + 512;
+    static constexpr uint32_t Q = 0, RING = 2 * TILE, CTL = RING + NSLOT * TILE, BYTES = CTL + 768;
+};
+// What a CTA does next.
+struct Work {
+    int q0, n_tok;       // first token, tokens (up to two tiles); n_tok <= 0: nothing more
+    int base, nk;        // token t sees keys 0 .. base + t (causal), 0 .. nk - 1
+    int k0;              // first key row
+    int vh, split;
+    int i0, end0, end1;  // key tiles of the two row tiles: i0 .. end - 1 (none where end = i0)
+    __host__ __device__ __forceinline__ int end(int s) const { return s ? end1 : end0; }
+    __host__ __device__ __forceinline__ int last() const { return end0 > end1 ? end0 : end1; }
 };
 struct Ctl {
-    uint64_t qfull[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain;
+    uint64_t qfull[2], qempty[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain, wfull[2], wempty[2], next;
+    alignas(16) uint32_t answer[4];
     uint32_t tmem_base;
-    int abort, not_finite;
+    int abort, not_finite[2];
+    Work work[2], held;  // held: taken, but not handed on before a wait gave up
 };
-static_assert(sizeof(Ctl) <= 512, "control block");
+static_assert(sizeof(Ctl) <= 768, "control block");
 
 struct FwdArgs {
     Batch b;
+    int64_t slots;                                           // row tile pairs, some of them empty
     int pack, tokens, splits;                                // heads per row group, tokens per 128 rows, CTAs that share a tile's keys
     int vheads;                                              // kv_heads * (G / pack)
     void* o;
@@ -55,16 +68,62 @@ struct FwdArgs {
     int64_t v_page;
 };
 
-// What a CTA does.
-struct Work {
-    int q0, n_tok;       // first token, tokens (up to two tiles)
-    int base, nk;        // token t sees keys 0 .. base + t (causal), 0 .. nk - 1
-    int k0;              // first key row
-    int i0, i1;          // its key tiles
-};
-
 __device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
 }  // namespace
+
+// The grid's tile t: split and heads go fastest, and the last tiles of a causal sequence, which see the most keys, first.
+template <bool PAGED> __device__ __forceinline__ Work work_of(const FwdArgs& a, int64_t t, int lane) {
+    const int wide = a.vheads * a.splits, span = 2 * a.tokens;
+    const int64_t x = t / wide;
+    const int hs = (int)(t - x * wide);
+    Work w{};
+    w.vh = hs % a.vheads;
+    w.split = hs / a.vheads;
+    if (PAGED) {
+        w.q0 = (int)x * span;
+        w.n_tok = min(span, a.b.Tq - w.q0);
+        w.nk = a.nk;
+    } else {
+        const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, (int)(a.slots - 1 - x), span, lane);
+        w.q0 = at.first;
+        w.n_tok = at.n;
+        if (at.n > 0 && at.seq >= 0) {
+            w.k0 = a.b.k_at(at.seq);
+            w.nk = max(a.b.k_at(at.seq + 1) - w.k0, 0);
+            w.base = at.offset + w.nk - at.length;
+        }
+    }
+    auto key_tiles = [&](int s) {
+        const int last = min((s + 1) * a.tokens, w.n_tok) - 1;
+        return last >= s * a.tokens ? (seen_by(a, w, last) + TN - 1) / TN : 0;
+    };
+    const int n0 = key_tiles(0), n1 = key_tiles(1), all = max(n0, n1), i1 = (int)((int64_t)all * (w.split + 1) / a.splits);
+    w.i0 = (int)((int64_t)all * w.split / a.splits);
+    w.end0 = min(max(n0, w.i0), i1);
+    w.end1 = min(max(n1, w.i0), i1);
+    return w;
+}
+
+// A running CTA takes the place of one of its grid that has not started (its index, or -1 where there is none left): CTAs are as many as
+// fit, and what one sets up serves all the tiles it takes. One thread asks; after a refusal it must not ask again.
+__device__ __forceinline__ void ask_next(uint32_t answer, uint32_t bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int next_of(uint32_t answer) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "mov.b32 %0, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n\t"
+        "selp.u32 %1, 1, 0, p;\n\t}"
+        : "=r"(x), "=r"(got)
+        : "r"(answer)
+        : "memory");
+    return got ? (int)x : -1;
+}
 
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -72,38 +131,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                   const __grid_constant__ FwdArgs a) {
     using C = Cfg<D>;
     constexpr uint32_t O_COL = 256;
+    constexpr int USERS = 10;                                // warps that take each tile's work
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wide = a.vheads * a.splits, hs = blockIdx.x % wide, vh = hs % a.vheads, split = hs / a.vheads, span = 2 * a.tokens;
-    const int per_kv = a.b.G / a.pack, kh = vh / per_kv, head0 = vh * a.pack;
     if (PAGED) launch_dependents();                          // the requests' own tokens may go ahead where an SM is free
-    Work w{};
-    if (PAGED) {
-        w.q0 = blockIdx.x / wide * span;
-        w.n_tok = min(span, a.b.Tq - w.q0);
-        w.nk = a.nk;
-    } else {
-        // the last tiles of a causal sequence see the most keys: they go first
-        const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / wide - 1 - blockIdx.x / wide, span, lane);
-        w.q0 = at.first;
-        w.n_tok = at.n;
-        if (at.n <= 0) return;
-        if (at.seq >= 0) {
-            w.k0 = a.b.k_at(at.seq);
-            w.nk = max(a.b.k_at(at.seq + 1) - w.k0, 0);
-            w.base = at.offset + w.nk - at.length;
-        }
-    }
-    // key tiles of the two row tiles
-    int n[2];
-    for (int s = 0; s < 2; ++s) {
-        const int last = min((s + 1) * a.tokens, w.n_tok) - 1;
-        n[s] = last >= s * a.tokens ? (seen_by(a, w, last) + TN - 1) / TN : 0;
-    }
-    const int all = max(n[0], n[1]);
-    w.i0 = (int)((int64_t)all * split / a.splits);
-    w.i1 = (int)((int64_t)all * (split + 1) / a.splits);
-    const int nt = w.i1 - w.i0;
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -111,16 +142,21 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int earlier = *reinterpret_cast<volatile int*>(a.status);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&ctl->qfull[i]), 1);
+            mbar_init(smem_u32(&ctl->qempty[i]), 1);
             mbar_init(smem_u32(&ctl->sfull[i]), 1);
             mbar_init(smem_u32(&ctl->pfull[i]), 128);
             mbar_init(smem_u32(&ctl->ofull[i]), 1);
+            mbar_init(smem_u32(&ctl->wfull[i]), 1);
+            mbar_init(smem_u32(&ctl->wempty[i]), USERS);
+            ctl->work[i].n_tok = 0;
         }
         for (int i = 0; i < C::NSLOT; ++i) {
             mbar_init(smem_u32(&ctl->full[i]), 1);
             mbar_init(smem_u32(&ctl->empty[i]), 1);
         }
         mbar_init(smem_u32(&ctl->drain), 1);
-        ctl->not_finite = 0;
+        mbar_init(smem_u32(&ctl->next), 1);
+        ctl->held.n_tok = 0;
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 910);
         mbar_fence_init();
@@ -135,248 +171,306 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
-    // iterations of tile s: i0 .. end(s) - 1
-    const int end0 = min(max(n[0], w.i0), w.i1), end1 = min(max(n[1], w.i0), w.i1);
-    uint32_t issued = 0;
+    bool ok = *abort_flag == 0;
+    // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
+    auto enter = [&](int n, Work& w) {
+        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        if (ok) w = ctl->work[n & 1];
+        return ok && w.n_tok > 0;
+    };
+    auto leave = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->wempty[n & 1]));
+    };
+    uint32_t issued = 0, q_loads[2] = {0, 0};
 
     if (warp >= 8) {
-    reg_dec<REGS_REST>();
-    if (warp == 9) {
-        // ------------------------------------------------------------ loads: Q, then K(i), V(i) for every i
-        bool ok = *abort_flag == 0;
-        const int box = min(TN, PAGED ? 1 << a.log_page : TN), boxes = TN / box;
-        if (ok && nt > 0 && (PAGED || lane == 0)) {
-            if (lane == 0) {
-                tma_prefetch_desc(&tmK);
-                tma_prefetch_desc(&tmV);
-                const uint32_t qbytes = (uint32_t)(a.tokens * a.pack * D * 2);
-                for (int s = 0; s < 2; ++s) {
-                    if ((s ? end1 : end0) <= w.i0) continue; // nobody would wait for it
-                    mbar_arrive_expect_tx(smem_u32(&ctl->qfull[s]), qbytes);
-                    for (int d = 0; d < D / 64; ++d)
-                        tma_load_3d(base + C::Q + s * C::TILE + d * HALF, &tmQ, smem_u32(&ctl->qfull[s]), 64 * d, head0, w.q0 + s * a.tokens);
+        reg_dec<REGS_REST>();
+        if (warp == 10) {
+            // -------------------------------------------------------- which tiles: one ahead of the others
+            int64_t t = blockIdx.x;
+            uint32_t asked = 0;
+            for (int n = 0;;) {
+                Work w{};
+                if (t >= 0) {
+                    w = work_of<PAGED>(a, t, lane);
+                    if (lane == 0 && w.n_tok > 0) ctl->held = w;
+                }
+                if (!ok) break;
+                if (t >= 0 && lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
+                if (t < 0 || w.n_tok > 0) {
+                    ok = mbar_wait_warp(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, abort_flag, a.status, 611);
+                    if (ok && lane == 0) {
+                        ctl->work[n & 1] = w;
+                        ctl->not_finite[n & 1] = 0;
+                        mbar_arrive(smem_u32(&ctl->wfull[n & 1]));
+                    }
+                    ++n;
+                    __syncwarp();
+                    if (t < 0) break;
+                }
+                // (also where a wait gave up: what the answer takes from the grid nobody else will do)
+                const bool there = mbar_wait_warp(smem_u32(&ctl->next), asked & 1, abort_flag, a.status, 612) ||
+                                   mbar_wait_answer(smem_u32(&ctl->next), asked & 1);
+                ++asked;
+                t = there ? next_of(smem_u32(ctl->answer)) : -1;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (!ok) {
+                    if (t >= 0) {
+                        w = work_of<PAGED>(a, t, lane);
+                        if (lane == 0 && w.n_tok > 0) ctl->held = w;
+                    }
+                    break;
                 }
             }
+        } else if (warp == 9) {
+            // -------------------------------------------------------- loads: Q, then K(i), V(i) for every i
+            const int box = min(TN, PAGED ? 1 << a.log_page : TN), boxes = TN / box;
+            const uint32_t qbytes = (uint32_t)(a.tokens * a.pack * D * 2);
+            const int per_kv = a.b.G / a.pack;
+            if (lane == 0) {
+                tma_prefetch_desc(&tmQ);
+                tma_prefetch_desc(&tmK);
+                tma_prefetch_desc(&tmV);
+            }
             uint32_t slot = 0, par = 1;
-            for (int i = w.i0; i < w.i1 && ok; ++i) {
-                // paged: a lane per box; a page that is not of the cache, or behind the keys, is loaded as zeros
-                int page = a.pages;
-                if (PAGED && lane < boxes && i * TN + lane * box < w.nk) {
-                    const int p = __ldg(a.list + ((i * TN + lane * box) >> a.log_page));
-                    if (p >= 0 && p < a.pages) page = p;
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                const int kh = w.vh / per_kv, head0 = w.vh * a.pack, i1 = w.last();
+                for (int s = 0; s < 2 && ok; ++s) {
+                    if (w.end(s) <= w.i0) continue;          // nobody would wait for it
+                    ok = mbar_wait_warp(smem_u32(&ctl->qempty[s]), (q_loads[s] & 1) ^ 1, abort_flag, a.status, 600);
+                    if (ok && lane == 0) {
+                        mbar_arrive_expect_tx(smem_u32(&ctl->qfull[s]), qbytes);
+                        for (int d = 0; d < D / 64; ++d)
+                            tma_load_3d(base + C::Q + s * C::TILE + d * HALF, &tmQ, smem_u32(&ctl->qfull[s]), 64 * d, head0, w.q0 + s * a.tokens);
+                    }
+                    __syncwarp();
+                    if (ok) ++q_loads[s];
                 }
-                for (int x = 0; x < 2 && ok; ++x) {
-                    ok = PAGED ? mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 601) : mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 601);
-                    if (!ok) break;
-                    const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
-                    if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
-                    if (PAGED) {
+                for (int i = w.i0; i < i1 && ok; ++i) {
+                    // paged: a lane per box; a page that is not of the cache, or behind the keys, is loaded as zeros
+                    int page = a.pages;
+                    if (PAGED && lane < boxes && i * TN + lane * box < w.nk) {
+                        const int p = __ldg(a.list + ((i * TN + lane * box) >> a.log_page));
+                        if (p >= 0 && p < a.pages) page = p;
+                    }
+                    for (int x = 0; x < 2 && ok; ++x) {
+                        ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 601);
+                        if (!ok) break;
+                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(bar, C::TILE);
+                            if (!PAGED)
+                                for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.k0 + i * TN);
+                        }
                         __syncwarp();
-                        if (lane < boxes)
+                        if (PAGED && lane < boxes)
                             for (int d = 0; d < D / 64; ++d)
                                 tma_load_4d(dst + d * HALF + lane * box * 128, x ? &tmV : &tmK, bar, 64 * d, kh, (i * TN) & ((1 << a.log_page) - 1), page);
                         __syncwarp();
-                    } else {
-                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.k0 + i * TN);
+                        ++issued;
+                        if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
-                    ++issued;
-                    if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                 }
             }
-        }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ MMAs
-        constexpr uint32_t ID_QK = umma_idesc<T>(128, TN, 0, 0), ID_PV = umma_idesc<T>(128, D, 0, 1);
-        const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dv0 = umma_desc_sw128(0, HALF, 1024);
-        const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, v_hi = (uint32_t)(dv0 >> 32), v_lo = (uint32_t)dv0;
-        bool ok = *abort_flag == 0;
-        auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
-        auto take = [&](int seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 603); };
-        auto issue_qk = [&](int s, int seq) {
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t qa = k_lo + ((base + C::Q + s * C::TILE) >> 4), kb = k_lo + ((base + C::RING + slot_of(seq) * C::TILE) >> 4);
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
-                    umma_ss_lohi(tmem + s * 128, qa + off, k_hi, kb + off, k_hi, ID_QK, ks > 0);
-                }
-                umma_commit(smem_u32(&ctl->sfull[s]));
-            }
-            __syncwarp();
-        };
-        auto release = [&](int seq) {
-            if (elect_one()) umma_commit(empty0 + 8 * slot_of(seq));
-            __syncwarp();
-        };
-        const int end[2] = {end0, end1};
-        if (nt > 0 && ok) {
-            take(0);
-            for (int s = 0; s < 2; ++s)
-                if (end[s] > w.i0) {
-                    ok = ok && mbar_wait_warp(smem_u32(&ctl->qfull[s]), 0, abort_flag, a.status, 602);
-                    if (ok) issue_qk(s, 0);
-                }
-            if (ok) release(0);
-        }
-        for (int i = 0; i < nt && ok; ++i) {
-            const int vseq = 2 * i + 1, kseq = 2 * i + 2;
-            bool v_in = false, k_in = false;
-#pragma unroll 1
-            for (int s = 0; s < 2; ++s) {
-                if (w.i0 + i >= end[s]) continue;
-                if (!v_in) { take(vseq); v_in = true; }
-                ok = ok && mbar_wait_warp(smem_u32(&ctl->pfull[s]), i & 1, abort_flag, a.status, 604);
-                if (!ok) break;
+        } else if (warp == 8) {
+            // -------------------------------------------------------- MMAs
+            constexpr uint32_t ID_QK = umma_idesc<T>(128, TN, 0, 0), ID_PV = umma_idesc<T>(128, D, 0, 1);
+            const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dv0 = umma_desc_sw128(0, HALF, 1024);
+            const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, v_hi = (uint32_t)(dv0 >> 32), v_lo = (uint32_t)dv0;
+            uint32_t first = 0, products[2] = {0, 0}, tiles[2] = {0, 0};         // K / V tiles, P's and row tiles before this work
+            auto slot_of = [&](uint32_t seq) { return seq % C::NSLOT; };
+            auto take = [&](uint32_t seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), (seq / C::NSLOT) & 1, abort_flag, a.status, 603); };
+            auto issue_qk = [&](int s, uint32_t seq, bool last) {
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t vb = v_lo + ((base + C::RING + slot_of(vseq) * C::TILE) >> 4);
+                    const uint32_t qa = k_lo + ((base + C::Q + s * C::TILE) >> 4), kb = k_lo + ((base + C::RING + slot_of(seq) * C::TILE) >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        umma_ts_lohi(tmem + O_COL + s * D, tmem + s * 128 + ks * 8, vb + ((ks * 2048) >> 4), v_hi, ID_PV, (i > 0 || ks > 0) ? 1u : 0u);
-                    if (w.i0 + i + 1 == end[s]) umma_commit(smem_u32(&ctl->ofull[s]));
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                        umma_ss_lohi(tmem + s * 128, qa + off, k_hi, kb + off, k_hi, ID_QK, ks > 0);
+                    }
+                    umma_commit(smem_u32(&ctl->sfull[s]));
+                    if (last) umma_commit(smem_u32(&ctl->qempty[s]));
                 }
                 __syncwarp();
-                if (w.i0 + i + 1 < end[s]) {
-                    if (!k_in) { take(kseq); k_in = true; }
-                    if (!ok) break;
-                    issue_qk(s, kseq);                       // P of this tile has been read by then: MMAs run in their order
+            };
+            auto release = [&](uint32_t seq) {
+                if (elect_one()) umma_commit(empty0 + 8 * slot_of(seq));
+                __syncwarp();
+            };
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                const int nt = w.last() - w.i0;
+                if (nt <= 0) continue;
+                take(first);
+                for (int s = 0; s < 2; ++s)
+                    if (w.end(s) > w.i0) {
+                        ok = ok && mbar_wait_warp(smem_u32(&ctl->qfull[s]), tiles[s] & 1, abort_flag, a.status, 602);
+                        if (ok) issue_qk(s, first, w.i0 + 1 == w.end(s));
+                        ++tiles[s];
+                    }
+                if (ok) release(first);
+                for (int i = 0; i < nt && ok; ++i) {
+                    // (the tiles of K and V are there long before P as a rule: nothing but P is waited for between the products)
+                    const uint32_t vseq = first + 2 * i + 1, kseq = vseq + 1;
+                    take(vseq);
+                    if (i + 1 < nt) take(kseq);
+#pragma unroll 1
+                    for (int s = 0; s < 2; ++s) {
+                        if (w.i0 + i >= w.end(s)) continue;
+                        ok = ok && mbar_wait_warp(smem_u32(&ctl->pfull[s]), products[s] & 1, abort_flag, a.status, 604);
+                        if (!ok) break;
+                        ++products[s];
+                        tc_fence_after();
+                        const int left = w.end(s) - (w.i0 + i);          // iterations of this row tile, with this one
+                        const bool last = s == 1 || w.i0 + i >= w.end(1);    // no other row tile reads these K and V
+                        if (elect_one()) {
+                            const uint32_t vb = v_lo + ((base + C::RING + slot_of(vseq) * C::TILE) >> 4);
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                umma_ts_lohi(tmem + O_COL + s * D, tmem + s * 128 + ks * 8, vb + ((ks * 2048) >> 4), v_hi, ID_PV, (i > 0 || ks > 0) ? 1u : 0u);
+                            if (left == 1) umma_commit(smem_u32(&ctl->ofull[s]));
+                            if (last) umma_commit(empty0 + 8 * slot_of(vseq));
+                            if (left > 1) {
+                                // over P, which has been read by then: MMAs run in their order
+                                const uint32_t qa = k_lo + ((base + C::Q + s * C::TILE) >> 4), kb = k_lo + ((base + C::RING + slot_of(kseq) * C::TILE) >> 4);
+#pragma unroll
+                                for (int ks = 0; ks < D / 16; ++ks) {
+                                    const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
+                                    umma_ss_lohi(tmem + s * 128, qa + off, k_hi, kb + off, k_hi, ID_QK, ks > 0);
+                                }
+                                umma_commit(smem_u32(&ctl->sfull[s]));
+                                if (left == 2) umma_commit(smem_u32(&ctl->qempty[s]));
+                            }
+                            if (last && i + 1 < nt) umma_commit(empty0 + 8 * slot_of(kseq));
+                        }
+                        __syncwarp();
+                    }
                 }
+                first += 2 * nt;
             }
-            if (!ok) break;
-            release(vseq);
-            if (i + 1 < nt) release(kseq);
+            // every MMA issued above has finished before tensor memory is freed
+            if (elect_one()) umma_commit(smem_u32(&ctl->drain));
+            __syncwarp();
+            mbar_wait(smem_u32(&ctl->drain), 0, abort_flag, a.status, 606);
         }
-        // every MMA issued above has finished before tensor memory is freed
-        if (elect_one()) umma_commit(smem_u32(&ctl->drain));
-        __syncwarp();
-        mbar_wait(smem_u32(&ctl->drain), 0, abort_flag, a.status, 606);
-    }
     } else {
         // ------------------------------------------------------------ softmax and epilogue
         reg_inc<REGS_MATH>();
-        const int s = warp >> 2, r = tid & 127;
-        const int tok = s * a.tokens + r / a.pack, head = head0 + r % a.pack;
-        const bool valid = r / a.pack < a.tokens && tok < w.n_tok;
-        const int vis = valid ? seen_by(a, w, tok) : 0;
-        const int whole = seen_by(a, w, s * a.tokens) / TN;  // tiles before this one are seen by every row (its first sees the fewest keys)
-        const int end = s ? end1 : end0;
-        const uint32_t scol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + s * 128, ocol = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + O_COL + s * D;
+        const int s = warp >> 2, r = tid & 127, row_tok = s * a.tokens + r / a.pack, row_head = r % a.pack;
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16), scol = tl + s * 128, ocol = tl + O_COL + s * D;
         const float c = a.b.scale * kLog2e;
-        float m = -INFINITY, l = 0.f;
-        bool ok = *abort_flag == 0;
         const int box = min(TN, PAGED ? 1 << a.log_page : TN);
-        // paged: a bit per box of tile i whose page is not of the cache; looked up a tile ahead
-        auto bad_pages = [&](int i) -> uint32_t {
-            const int k = i * TN + lane * box;
-            const int p = lane * box < TN && k < w.nk ? __ldg(a.list + (k >> a.log_page)) : 0;
-            return __ballot_sync(0xffffffffu, p < 0 || p >= a.pages);
-        };
-        uint32_t bad = 0, bad_next = PAGED && w.i0 < end ? bad_pages(w.i0) : 0u;
-        for (int i = w.i0; i < end && ok; ++i) {
-            const int it = i - w.i0;
-            if (PAGED) {
-                bad = bad_next;
-                if (i + 1 < end) bad_next = bad_pages(i + 1);
+        uint32_t first = 0, products = 0, tiles = 0;         // K / V tiles, P's and row tiles before this work
+        Work w;
+        for (int n = 0; enter(n, w); ++n) {
+            const int head = w.vh * a.pack + row_head, end = w.end(s);
+            const bool valid = r / a.pack < a.tokens && row_tok < w.n_tok;
+            const int vis = valid ? seen_by(a, w, row_tok) : 0;
+            const int whole = seen_by(a, w, s * a.tokens) / TN;      // tiles before this one are seen by every row (its first sees the fewest keys)
+            float m = -INFINITY, l = 0.f;
+            // paged: a bit per box of tile i whose page is not of the cache; looked up a tile ahead
+            auto bad_pages = [&](int i) -> uint32_t {
+                const int k = i * TN + lane * box;
+                const int p = lane * box < TN && k < w.nk ? __ldg(a.list + (k >> a.log_page)) : 0;
+                return __ballot_sync(0xffffffffu, p < 0 || p >= a.pages);
+            };
+            uint32_t bad = 0, bad_next = PAGED && w.i0 < end ? bad_pages(w.i0) : 0u;
+            for (int i = w.i0; i < end && ok; ++i) {
+                if (PAGED) {
+                    bad = bad_next;
+                    if (i + 1 < end) bad_next = bad_pages(i + 1);
+                }
+                ok = mbar_wait_warp(smem_u32(&ctl->sfull[s]), products & 1, abort_flag, a.status, 607);
+                if (!ok) break;
+                ++products;
+                tc_fence_after();
+                uint32_t x[128];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tmem_ld32(scol + 32 * j, x + 32 * j);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tmem_wait_ld_regs(x + 32 * j);
+                if (i >= whole) {
+                    const int lim = vis - i * TN;
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        if (j >= lim) x[j] = 0xff800000u;
+                }
+                if (PAGED && bad) {
+                    // (their keys and values are zeros: nothing of them can reach the row but the logit 0)
+                    const int shift = min(a.log_page, 7);
+#pragma unroll
+                    for (int j = 0; j < TN; j += 16)
+                        if ((bad >> (j >> shift)) & 1)
+#pragma unroll
+                            for (int jj = 0; jj < 16; ++jj) x[j + jj] = 0xff800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < TN; j += 2) top[(j >> 1) & 3] = fmaxf(fmaxf(top[(j >> 1) & 3], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
+                const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+                const bool raise = m == -INFINITY ? y > -INFINITY : y > m + RAISE;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float next = raise ? y : m, shrink = raise ? (m == -INFINITY ? 0.f : ex2_approx(m - next)) : 1.f;
+                    m = next;
+                    l *= shrink;
+                    if (i > w.i0) {
+                        // (P V of the iteration before was issued before this S: it has written O)
+#pragma unroll 1
+                        for (int h = 0; h < D / 32; ++h) {
+                            uint32_t o[32];
+                            tmem_ld32(ocol + 32 * h, o);
+                            tmem_wait_ld_regs(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                            tmem_st32(ocol + 32 * h, o);
+                        }
+                    }
+                }
+                const float off = m == -INFINITY ? 0.f : -m;
+                const float2 cc = make_float2(c, c), oo = make_float2(off, off);
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), cc, oo);
+                        const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                        sum = __fadd2_rn(sum, e);
+                        p[j] = pack2<T>(e.x, e.y);
+                    }
+                    tmem_st32(scol + 32 * h, p);
+                }
+                l += sum.x + sum.y;
+                if (i >= whole) {
+                    // V rows that some rows of the tile may not see
+                    const uint32_t vseq = first + 2 * (i - w.i0) + 1, slot = vseq % C::NSLOT;
+                    ok = mbar_wait_warp(full0 + 8 * slot, (vseq / C::NSLOT) & 1, abort_flag, a.status, 608);
+                    if (!ok) break;
+                    if (clean_row<T, D>(smem + C::RING + slot * C::TILE, r)) *reinterpret_cast<volatile int*>(&ctl->not_finite[n & 1]) = 1;
+                    fence_proxy_async_smem();
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&ctl->pfull[s]));
             }
-            ok = mbar_wait_warp(smem_u32(&ctl->sfull[s]), it & 1, abort_flag, a.status, 607);
+            const bool any = end > w.i0;
+            if (any) {
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->ofull[s]), tiles & 1, abort_flag, a.status, 609);
+                ++tiles;
+            }
             if (!ok) break;
             tc_fence_after();
-            uint32_t x[128];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_ld32(scol + 32 * j, x + 32 * j);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_wait_ld_regs(x + 32 * j);
-            if (i >= whole) {
-                const int lim = vis - i * TN;
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    if (j >= lim) x[j] = 0xff800000u;
-            }
-            if (PAGED && bad) {
-                // (their keys and values are zeros: nothing of them can reach the row but the logit 0)
-                const int shift = min(a.log_page, 7);
-#pragma unroll
-                for (int j = 0; j < TN; j += 16)
-                    if ((bad >> (j >> shift)) & 1)
-#pragma unroll
-                        for (int jj = 0; jj < 16; ++jj) x[j + jj] = 0xff800000u;
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < TN; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[j]));
-            const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-            const bool raise = m == -INFINITY ? y > -INFINITY : y > m + RAISE;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float next = raise ? y : m, shrink = raise ? (m == -INFINITY ? 0.f : ex2_approx(m - next)) : 1.f;
-                m = next;
-                l *= shrink;
-                if (it > 0) {
-                    // (P V of the iteration before was issued before this S: it has written O)
-#pragma unroll 1
-                    for (int h = 0; h < D / 32; ++h) {
-                        uint32_t o[32];
-                        tmem_ld32(ocol + 32 * h, o);
-                        tmem_wait_ld_regs(o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                        tmem_st32(ocol + 32 * h, o);
-                    }
-                }
-            }
-            const float off = m == -INFINITY ? 0.f : -m;
-            const float2 cc = make_float2(c, c), oo = make_float2(off, off);
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t p[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), cc, oo);
-                    const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
-                    sum = __fadd2_rn(sum, e);
-                    p[j] = pack2<T>(e.x, e.y);
-                }
-                tmem_st32(scol + 32 * h, p);
-            }
-            l += sum.x + sum.y;
-            if (i >= whole) {
-                // V rows that some rows of the tile may not see
-                const int vseq = 2 * it + 1;
-                const uint32_t slot = (uint32_t)vseq % C::NSLOT;
-                ok = mbar_wait_warp(full0 + 8 * slot, ((uint32_t)vseq / C::NSLOT) & 1, abort_flag, a.status, 608);
-                if (!ok) break;
-                uint8_t* row = smem + C::RING + slot * C::TILE + r * 128;
-                bool any = false;
-#pragma unroll
-                for (int d = 0; d < D / 64; ++d)
-#pragma unroll
-                    for (int ch = 0; ch < 8; ++ch) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(row + d * HALF + 16 * (ch ^ (r & 7)));
-                        any |= not_finite<T>(v.x) || not_finite<T>(v.y) || not_finite<T>(v.z) || not_finite<T>(v.w);
-                    }
-                if (any) {
-                    for (int d = 0; d < D / 64; ++d)
-                        for (int ch = 0; ch < 8; ++ch) {
-                            uint4* v = reinterpret_cast<uint4*>(row + d * HALF + 16 * ch);
-                            *v = make_uint4(finite_only<T>(v->x), finite_only<T>(v->y), finite_only<T>(v->z), finite_only<T>(v->w));
-                        }
-                    *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
-                }
-                fence_proxy_async_smem();
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(smem_u32(&ctl->pfull[s]));
-        }
-        if (end > w.i0) ok = ok && mbar_wait_warp(smem_u32(&ctl->ofull[s]), 0, abort_flag, a.status, 609);
-        if (ok) {
-            tc_fence_after();
-            const bool any = end > w.i0;
-            const float inv = l != 0.f ? 1.f / l : 0.f;      // 0: a row without a key; NaN stays NaN
-            const bool fix = any && *reinterpret_cast<volatile int*>(&ctl->not_finite) != 0;
-            const int64_t row = (int64_t)(w.q0 + tok) * a.b.H + head;
-            const int from = max(w.i0, min(seen_by(a, w, 0), seen_by(a, w, min(a.tokens, w.n_tok - 1))) / TN) * TN, to = min(vis, w.i1 * TN);
+            first += 2 * (w.last() - w.i0);
+            const bool fix = any && *reinterpret_cast<volatile int*>(&ctl->not_finite[n & 1]) != 0;
+            const float inv = l != 0.f ? 1.f / l : 0.f;      // l = 0: a row without a key; NaN stays NaN
+            const int64_t row = (int64_t)(w.q0 + row_tok) * a.b.H + head, part = (int64_t)w.split * a.b.Tq * a.b.H + row;
 #pragma unroll 1
             for (int h = 0; h < D / 32; ++h) {
                 uint32_t o[32];
@@ -386,9 +480,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     tmem_ld32(ocol + 32 * h, o);
                     tmem_wait_ld_regs(o);
                 }
+                if (!valid) continue;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(l != 0.f ? __uint_as_float(o[j]) * inv : 0.f);
-                if (fix && valid) {
+                if (fix) {
+                    const int kh = w.vh / (a.b.G / a.pack);
+                    const int from = max(w.i0, seen_by(a, w, 0) / TN) * TN, to = min(vis, w.last() * TN);
                     for (int k = from; k < to; ++k) {
                         const T* vr = static_cast<const T*>(a.v) + (int64_t)kh * a.rv.head + 32 * h;
                         if (PAGED) {
@@ -405,33 +502,29 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         }
                     }
                 }
-                if (!valid) continue;
                 if (PAGED || a.splits > 1) {
-                    float4* dst = reinterpret_cast<float4*>(a.part_o + ((int64_t)split * a.b.Tq * a.b.H + row) * D + 32 * h);
                     if (any)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+                        for (int j = 0; j < 4; ++j) store8(a.part_o + part * D + 32 * h + 8 * j, o + 8 * j);
                 } else {
                     uint32_t p[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) p[j] = pack2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row * D + 32 * h);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) dst[j] = make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+                    store8(static_cast<T*>(a.o) + row * D + 32 * h, p);
+                    store8(static_cast<T*>(a.o) + row * D + 32 * h + 16, p + 8);
                     if (a.o_rest) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) p[j] = rest2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]), p[j]);
-                        dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o_rest) + row * D + 32 * h);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) dst[j] = make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+                        store8(static_cast<T*>(a.o_rest) + row * D + 32 * h, p);
+                        store8(static_cast<T*>(a.o_rest) + row * D + 32 * h + 16, p + 8);
                     }
                 }
             }
+            leave(n);
             if (valid) {
                 const float z = l != 0.f ? m + log2f(l) : -INFINITY;
-                if (PAGED || a.splits > 1) a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = z;
-                else a.lse[(int64_t)head * a.b.Tq + w.q0 + tok] = z * kLn2;
+                if (PAGED || a.splits > 1) a.part_lse[part] = z;
+                else a.lse[(int64_t)head * a.b.Tq + w.q0 + row_tok] = z * kLn2;
             }
         }
     }
@@ -442,7 +535,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         // a wait gave up: give the loads a moment (100 us in all) to land before shared memory goes away
         const uint64_t t_end = global_timer_ns() + 100000ull;
         for (int s = 0; s < 2; ++s)
-            while (issued && (s ? end1 : end0) > w.i0 && !mbar_try_wait(smem_u32(&ctl->qfull[s]), 0) && global_timer_ns() < t_end) {}
+            while (q_loads[s] && !mbar_try_wait(smem_u32(&ctl->qfull[s]), (q_loads[s] - 1) & 1) && global_timer_ns() < t_end) {}
         for (uint32_t back = 1; back <= (uint32_t)C::NSLOT && back <= issued; ++back) {
             const uint32_t sq = issued - back;
             while (!mbar_try_wait(full0 + 8 * (sq % C::NSLOT), (sq / C::NSLOT) & 1) && global_timer_ns() < t_end) {}
@@ -456,15 +549,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tmem_dealloc(tmem, 512);
     }
     if (*abort_flag) {
-        // NaN in all that the CTA owns: the caller's memory is not initialised
-        for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
-            const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head0 + e % a.pack;
-            if (PAGED || a.splits > 1) {
-                a.part_lse[(int64_t)split * a.b.Tq * a.b.H + row] = __uint_as_float(kNaN32);
-                for (int d = 0; d < D; ++d) a.part_o[((int64_t)split * a.b.Tq * a.b.H + row) * D + d] = __uint_as_float(kNaN32);
-            } else {
-                a.lse[(int64_t)(head0 + e % a.pack) * a.b.Tq + w.q0 + e / a.pack] = __uint_as_float(kNaN32);
-                for (int d = 0; d < D / 2; ++d) reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D)[d] = kNaN16x2;
+        // NaN in the tiles that the CTA had taken and may not have finished: the caller's memory is not initialised
+        for (int x = 0; x < 3; ++x) {
+            const Work w = x == 2 ? ctl->held : ctl->work[x];
+            for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
+                const int head = w.vh * a.pack + e % a.pack;
+                const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head;
+                if (PAGED || a.splits > 1) {
+                    a.part_lse[(int64_t)w.split * a.b.Tq * a.b.H + row] = __uint_as_float(kNaN32);
+                    for (int d = 0; d < D; ++d) a.part_o[((int64_t)w.split * a.b.Tq * a.b.H + row) * D + d] = __uint_as_float(kNaN32);
+                } else {
+                    a.lse[(int64_t)head * a.b.Tq + w.q0 + e / a.pack] = __uint_as_float(kNaN32);
+                    for (int d = 0; d < D / 2; ++d) reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + row * D)[d] = kNaN16x2;
+                }
             }
         }
     }
@@ -522,7 +619,8 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     if (int rc = make_rows_map<T>(&tv, v, D, a.b.Hk, tk_rows, rv, 1, TN)) return rc;
     auto kern = packed_fwd_kernel<T, D, false>;
     if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
-    const int64_t grid = (int64_t)a.vheads * a.splits * piece_slots(a.b.Tq, 2 * a.tokens, a.b.B);
+    a.slots = piece_slots(a.b.Tq, 2 * a.tokens, a.b.B);
+    const int64_t grid = (int64_t)a.vheads * a.splits * a.slots;
     if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_fwd: too many tiles");
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
     ES_CHECK_LAUNCH("packed_fwd_kernel");

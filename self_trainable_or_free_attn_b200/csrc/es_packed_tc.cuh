@@ -48,6 +48,36 @@ __device__ __forceinline__ Piece find_piece(const int* cu, int B, int tokens, in
 }
 inline int64_t piece_slots(int tokens, int span, int B) { return tokens / span + B + 2; }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+// The larger of three, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x for x <= 64 on the FMA pipes: 2^n times a polynomial of the rest f in [-1/2, 1/2], the degree-4 one whose largest relative error is
+// smallest (2.6e-6, by the exchange of its extrema). Below -126 the result is 2^-126 instead of less. x must not be NaN.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    constexpr float ROUND = 12582912.f;                      // 1.5 * 2^23: adding it leaves n in the low bits
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 t = __fadd2_rn(x, make_float2(ROUND, ROUND)), n = __fadd2_rn(t, make_float2(-ROUND, -ROUND));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
+    p = __ffma2_rn(p, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+    p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {       // either of two packed values
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
     return (w & E) == E || ((w >> 16) & E) == E;
@@ -57,6 +87,52 @@ template <typename T> __device__ __forceinline__ uint32_t finite_only(uint32_t w
     if ((w & E) == E) w &= 0xFFFF0000u;
     if (((w >> 16) & E) == E) w &= 0xFFFFu;
     return w;
+}
+
+// Row r of the tile at `tile` in shared memory, its values that are not finite set to 0; whether there were any. (0 times a value, summed: NaN
+// if one of them is not finite, in one instruction for two values.)
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> { typedef __nv_bfloat162 type; };
+template <> struct Pair<__half> { typedef __half2 type; };
+template <typename T, int D> __device__ __forceinline__ bool clean_row(uint8_t* tile, int r) {
+    typedef typename Pair<T>::type P;
+    uint8_t* row = tile + r * 128;
+    const uint32_t zero = 0;
+    P acc[4] = {*reinterpret_cast<const P*>(&zero), *reinterpret_cast<const P*>(&zero), *reinterpret_cast<const P*>(&zero), *reinterpret_cast<const P*>(&zero)};
+    const P z = acc[0];
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + d * HALF + 16 * (ch ^ (r & 7)));
+            const uint32_t* w = &v.x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = __hfma2(*reinterpret_cast<const P*>(w + j), z, acc[j]);
+        }
+    acc[0] = __hadd2(__hadd2(acc[0], acc[1]), __hadd2(acc[2], acc[3]));
+    const float2 sum = unpack2<T>(*reinterpret_cast<const uint32_t*>(&acc[0]));
+    if (sum.x == 0.f && sum.y == 0.f) return false;
+    for (int d = 0; d < D / 64; ++d)
+        for (int ch = 0; ch < 8; ++ch) {
+            uint4* v = reinterpret_cast<uint4*>(row + d * HALF + 16 * ch);
+            *v = make_uint4(finite_only<T>(v->x), finite_only<T>(v->y), finite_only<T>(v->z), finite_only<T>(v->w));
+        }
+    return true;
+}
+
+// 32 bytes at once: a row's sectors are written whole. dst is 32-byte aligned.
+__device__ __forceinline__ void store8(void* dst, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// After a wait has given up, whether an answer on its way to shared memory has come (100 us at most).
+__device__ __forceinline__ bool mbar_wait_answer(uint32_t bar, uint32_t parity) {
+    const uint64_t t_end = global_timer_ns() + 100000ull;
+    bool there = mbar_try_wait(bar, parity);
+    while (!there && global_timer_ns() < t_end) there = mbar_try_wait(bar, parity);
+    return __all_sync(0xffffffffu, there) != 0;
 }
 
 // What rounding x and y to the type left of them, itself rounded: together 16 bits of mantissa in bf16.
