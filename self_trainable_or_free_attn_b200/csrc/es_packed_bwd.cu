@@ -112,11 +112,11 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&ctl->sfull[i]), 1);
             mbar_init(smem_u32(&ctl->rfull[i]), 32);
-            mbar_init(smem_u32(&ctl->rempty[i]), 256);
+            mbar_init(smem_u32(&ctl->rempty[i]), 8);
         }
         mbar_init(smem_u32(&ctl->dpfull), 1);
-        mbar_init(smem_u32(&ctl->pfull), 256);
-        mbar_init(smem_u32(&ctl->dsfull), 256);
+        mbar_init(smem_u32(&ctl->pfull), 8);
+        mbar_init(smem_u32(&ctl->dsfull), 8);
         mbar_init(smem_u32(&ctl->gfull), 1);
         mbar_init(smem_u32(&ctl->drain), 1);
         ctl->not_finite = 0;
@@ -144,7 +144,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     tc_fence_after();
     const uint32_t tmem = ctl->tmem_base;
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
-    float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then delta
+    float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then minus delta
     float* row_delta = row_lse + C::NROW * TM;
     uint32_t issued = 0;
     // walked tile i: query heads head0 .., first token
@@ -187,7 +187,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     const int64_t g = (int64_t)(h0 + r % a.pack) * a.b.Tq + q0 + t;
                     const float z = valid ? __ldg(a.lse + g) : -INFINITY;
                     l[x] = z == -INFINITY ? -INFINITY : -z * kLog2e;       // (added to the logit: P of a row without keys, or of none, is 0)
-                    d[x] = valid ? __ldg(a.delta + g) : 0.f;
+                    d[x] = valid ? -__ldg(a.delta + g) : 0.f;
                 }
                 ok = mbar_wait_warp(smem_u32(&ctl->rempty[i % C::NROW]), ((i / C::NROW) & 1) ^ 1, abort_flag, a.status, 622);
                 if (!ok) break;
@@ -274,72 +274,86 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_ld32(scol + 32, x + 32);
             tmem_wait_ld_regs(x);
             tmem_wait_ld_regs(x + 32);
-            const float4* rl = reinterpret_cast<const float4*>(row_lse + (i % C::NROW) * TM + 64 * ch);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float4 z = rl[j];
-                x[4 * j] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j]), c, z.x)));
-                x[4 * j + 1] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 1]), c, z.y)));
-                x[4 * j + 2] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 2]), c, z.z)));
-                x[4 * j + 3] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(x[4 * j + 3]), c, z.w)));
-            }
             const int lim = cut ? max(r - diag - t0, 0) * a.pack - 64 * ch : 0;      // columns before it do not see the key
-            if (masked) {
-                // columns that are not rows of the sequence have an offset of -inf: P is 0 unless their logit is not finite
-                const int end = min(loaded, (nq - t0) * a.pack) - 64 * ch;
-#pragma unroll
-                for (int j = 0; j < 64; ++j)
-                    if (j < lim || j >= end) x[j] = 0;
-            }
-            {
+            const int end = min(loaded, (nq - t0) * a.pack) - 64 * ch;               // columns from here on are not rows of the sequence
+            const float4* rl = reinterpret_cast<const float4*>(row_lse + (i % C::NROW) * TM + 64 * ch);
+            // P; one pair in four on the FMA pipes, as many as take no longer than the others take the 16 exponentials a clock of an SM
+            auto probabilities = [&](auto cut_tile) {
+                const float2 cc = make_float2(c, c);
                 uint32_t p[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) p[j] = pack2<T>(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                for (int j = 0; j < 16; ++j) {
+                    const float4 z = rl[j];
+                    const float2 z0 = __ffma2_rn(make_float2(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])), cc, make_float2(z.x, z.y));
+                    const float2 z1 = __ffma2_rn(make_float2(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])), cc, make_float2(z.z, z.w));
+                    float2 e0 = make_float2(ex2_approx(z0.x), ex2_approx(z0.y));
+                    float2 e1 = !decltype(cut_tile)::value && j % 2 == 1 ? ex2_poly(z1) : make_float2(ex2_approx(z1.x), ex2_approx(z1.y));
+                    if (decltype(cut_tile)::value) {
+                        if (4 * j < lim || 4 * j >= end) e0.x = 0.f;
+                        if (4 * j + 1 < lim || 4 * j + 1 >= end) e0.y = 0.f;
+                        if (4 * j + 2 < lim || 4 * j + 2 >= end) e1.x = 0.f;
+                        if (4 * j + 3 < lim || 4 * j + 3 >= end) e1.y = 0.f;
+                    }
+                    x[4 * j] = __float_as_uint(e0.x); x[4 * j + 1] = __float_as_uint(e0.y);
+                    x[4 * j + 2] = __float_as_uint(e1.x); x[4 * j + 3] = __float_as_uint(e1.y);
+                    p[2 * j] = pack2<T>(e0.x, e0.y);
+                    p[2 * j + 1] = pack2<T>(e1.x, e1.y);
+                }
                 tmem_st32(scol, p);
-            }
+            };
             if (masked) {
+                probabilities(std::true_type{});
                 // dP of this tile is there too: from here on its Q and dO are read by the second products only
                 ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 630);
                 if (!ok) break;
                 const uint32_t slot = (uint32_t)(2 * i + ch) % C::NSLOT;             // half of the threads Q, half dO
                 if (clean_row<T, D>(smem + C::RING + slot * C::TILE, r)) *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
                 fence_proxy_async_smem();
+            } else {
+                probabilities(std::false_type{});
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&ctl->pfull));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->pfull));
             ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 631);
             if (!ok) break;
             tc_fence_after();
+            uint32_t y[64];
+            tmem_ld32(dpcol, y);
+            tmem_ld32(dpcol + 32, y + 32);
+            tmem_wait_ld_regs(y);
+            tmem_wait_ld_regs(y + 32);
             const float4* rd = reinterpret_cast<const float4*>(row_delta + (i % C::NROW) * TM + 64 * ch);
-            uint32_t ds[32];
+            auto differences = [&](auto cut_tile) {
+                uint32_t ds[32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t y[32];
-                tmem_ld32(dpcol + 32 * h, y);
-                tmem_wait_ld_regs(y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float4 z = rd[8 * h + j];
-                    const uint32_t* xp = x + 32 * h + 4 * j;
-                    float g0 = __uint_as_float(xp[0]) * (__uint_as_float(y[4 * j]) - z.x), g1 = __uint_as_float(xp[1]) * (__uint_as_float(y[4 * j + 1]) - z.y);
-                    float g2 = __uint_as_float(xp[2]) * (__uint_as_float(y[4 * j + 2]) - z.z), g3 = __uint_as_float(xp[3]) * (__uint_as_float(y[4 * j + 3]) - z.w);
-                    if (masked) {                            // (0 times what a hidden row holds)
-                        const int k = 32 * h + 4 * j, end = min(loaded, (nq - t0) * a.pack) - 64 * ch;
-                        if (k < lim || k >= end) g0 = 0.f;
-                        if (k + 1 < lim || k + 1 >= end) g1 = 0.f;
-                        if (k + 2 < lim || k + 2 >= end) g2 = 0.f;
-                        if (k + 3 < lim || k + 3 >= end) g3 = 0.f;
+                for (int j = 0; j < 16; ++j) {
+                    const float4 z = rd[j];                  // minus delta
+                    float2 g0 = __fmul2_rn(make_float2(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1])),
+                                           __fadd2_rn(make_float2(__uint_as_float(y[4 * j]), __uint_as_float(y[4 * j + 1])), make_float2(z.x, z.y)));
+                    float2 g1 = __fmul2_rn(make_float2(__uint_as_float(x[4 * j + 2]), __uint_as_float(x[4 * j + 3])),
+                                           __fadd2_rn(make_float2(__uint_as_float(y[4 * j + 2]), __uint_as_float(y[4 * j + 3])), make_float2(z.z, z.w)));
+                    if (decltype(cut_tile)::value) {         // (0 times what a hidden row holds)
+                        if (4 * j < lim || 4 * j >= end) g0.x = 0.f;
+                        if (4 * j + 1 < lim || 4 * j + 1 >= end) g0.y = 0.f;
+                        if (4 * j + 2 < lim || 4 * j + 2 >= end) g1.x = 0.f;
+                        if (4 * j + 3 < lim || 4 * j + 3 >= end) g1.y = 0.f;
                     }
-                    ds[16 * h + 2 * j] = pack2<T>(g0, g1);
-                    ds[16 * h + 2 * j + 1] = pack2<T>(g2, g3);
+                    ds[2 * j] = pack2<T>(g0.x, g0.y);
+                    ds[2 * j + 1] = pack2<T>(g1.x, g1.y);
                 }
-            }
-            mbar_arrive(smem_u32(&ctl->rempty[i % C::NROW]));
-            tmem_st32(dpcol, ds);
+                tmem_st32(dpcol, ds);
+            };
+            if (masked) differences(std::true_type{});
+            else differences(std::false_type{});
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&ctl->dsfull));
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ctl->rempty[i % C::NROW]));
+                mbar_arrive(smem_u32(&ctl->dsfull));
+            }
         }
         if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 632);
         if (ok) {
@@ -416,7 +430,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
         for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctl->sfull[i]), 1);
         mbar_init(smem_u32(&ctl->dpfull), 1);
-        mbar_init(smem_u32(&ctl->dsfull), 256);
+        mbar_init(smem_u32(&ctl->dsfull), 8);
         mbar_init(smem_u32(&ctl->gfull), 1);
         mbar_init(smem_u32(&ctl->drain), 1);
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
@@ -532,45 +546,57 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             tmem_ld32(scol + 32, x + 32);
             tmem_wait_ld_regs(x);
             tmem_wait_ld_regs(x + 32);
-            const float2 cc = make_float2(c, c), oo = make_float2(off, off);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float2 y = __ffma2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), cc, oo);
-                x[2 * j] = __float_as_uint(ex2_approx(y.x));
-                x[2 * j + 1] = __float_as_uint(ex2_approx(y.y));
-            }
             const bool masked = i >= whole;
             const int lim = vis - i * TN - 64 * ch;
+            // P; one pair in four on the FMA pipes (of tiles that no mask cuts)
+            auto probabilities = [&](auto mixed) {
+                const float2 cc = make_float2(c, c), oo = make_float2(off, off);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), cc, oo);
+                    const float2 e = decltype(mixed)::value && j % 4 == 3 ? ex2_poly(z) : make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                    x[2 * j] = __float_as_uint(e.x);
+                    x[2 * j + 1] = __float_as_uint(e.y);
+                }
+            };
             if (masked) {
+                probabilities(std::false_type{});
                 // S has read K by now; what is left is dQ, where hidden keys have dS = 0. A half of d for each half of the threads
                 uint8_t* tile = smem + C::RING + (uint32_t)(2 * i) % C::NSLOT * C::TILE;
                 if (64 * ch < D) clean_row<T, 64>(tile + ch * HALF, r);
                 fence_proxy_async_smem();
+            } else {
+                probabilities(std::true_type{});
             }
             ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 651);
             if (!ok) break;
             tc_fence_after();
-            uint32_t ds[32];
+            uint32_t y[64];
+            tmem_ld32(dpcol, y);
+            tmem_ld32(dpcol + 32, y + 32);
+            tmem_wait_ld_regs(y);
+            tmem_wait_ld_regs(y + 32);
+            auto differences = [&](auto cut_tile) {
+                uint32_t ds[32];
+                const float2 nd = make_float2(-delta, -delta);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t y[32];
-                tmem_ld32(dpcol + 32 * h, y);
-                tmem_wait_ld_regs(y);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int k = 32 * h + 2 * j;
-                    float g0 = __uint_as_float(x[k]) * (__uint_as_float(y[2 * j]) - delta), g1 = __uint_as_float(x[k + 1]) * (__uint_as_float(y[2 * j + 1]) - delta);
-                    if (masked) {
-                        if (k >= lim) g0 = 0.f;
-                        if (k + 1 >= lim) g1 = 0.f;
+                for (int j = 0; j < 32; ++j) {
+                    float2 g = __fmul2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
+                                          __fadd2_rn(make_float2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])), nd));
+                    if (decltype(cut_tile)::value) {
+                        if (2 * j >= lim) g.x = 0.f;
+                        if (2 * j + 1 >= lim) g.y = 0.f;
                     }
-                    ds[16 * h + j] = pack2<T>(g0, g1);
+                    ds[j] = pack2<T>(g.x, g.y);
                 }
-            }
-            tmem_st32(scol, ds);
+                tmem_st32(scol, ds);
+            };
+            if (masked) differences(std::true_type{});
+            else differences(std::false_type{});
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&ctl->dsfull));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->dsfull));
         }
         if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 652);
         if (ok) {

@@ -55,19 +55,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
                  : "memory");
 }
 
-// The larger of three, NaN if one of them is.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 // 2^x for x <= 64 on the FMA pipes: 2^n times a polynomial of the rest f in [-1/2, 1/2], the degree-4 one whose largest relative error is
-// smallest (2.6e-6, by the exchange of its extrema). Below -126 the result is 2^-126 instead of less. x must not be NaN.
+// smallest (2.6e-6, by the exchange of its extrema). Below -126 the result is 2^-126 instead of less; NaN stays NaN.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
     constexpr float ROUND = 12582912.f;                      // 1.5 * 2^23: adding it leaves n in the low bits
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
     const float2 t = __fadd2_rn(x, make_float2(ROUND, ROUND)), n = __fadd2_rn(t, make_float2(-ROUND, -ROUND));
     const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
     float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
@@ -75,7 +68,7 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
     p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
     p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+    return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u)));
 }
 
 template <typename T> __device__ __forceinline__ bool not_finite(uint32_t w) {       // either of two packed values
