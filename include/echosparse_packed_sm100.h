@@ -25,31 +25,24 @@ extern "C" {
 
 /* Attention of every sequence of a packed batch to its own keys. q [total_q, heads, D], k, v [total_k, kv_heads, D] with a token and a
  * head stride each; o [total_q, heads, D] contiguous, lse [heads, total_q]; o_rest (like o, or NULL) receives what rounding o left, for
- * es_packed_delta. Sequence b has queries cu_q[b] .. cu_q[b + 1] and keys cu_k[b] ..
- * cu_k[b + 1]; with causal, query i of nq sees key j of nk where j <= i + nk - nq. workspace: es_packed_workspace_bytes bytes, may be
- * NULL where that is 0. */
-long long es_packed_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D);
+ * the backward. Sequence b has queries cu_q[b] .. cu_q[b + 1] and keys cu_k[b] ..
+ * cu_k[b + 1]; with causal, query i of nq sees key j of nk where j <= i + nk - nq. workspace: es_packed_fwd_workspace_bytes bytes,
+ * may be NULL where that is 0. */
+long long es_packed_fwd_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D);
 int es_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, const int32_t* cu_q,
                        const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D, int64_t q_token,
                        int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, float scale, int32_t causal,
                        int32_t dtype, void* workspace, void* stream);
 
-/* delta [heads, total_q] = the row sums of dO o (o + o_rest), which both backward passes read. dout with strides, o, o_rest contiguous; o_rest
- * may be NULL. */
-int es_packed_delta(const void* o, const void* o_rest, const void* dout, float* delta, int32_t total_q, int32_t heads, int32_t D, int64_t do_token,
-                    int64_t do_head, int32_t dtype, void* stream);
-
-/* The two passes of the backward: dq [total_q, heads, D] contiguous, one owner per query row; dk, dv [total_k, kv_heads, D] contiguous, one
- * owner per key row, summed over the query heads of the key's group. No atomics: the same inputs give the same bits. */
-int es_packed_attn_bwd_q(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq,
-                         const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k, int32_t heads,
-                         int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token,
-                         int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal, int32_t dtype, void* stream);
-int es_packed_attn_bwd_kv(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk,
-                          void* dv, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k,
-                          int32_t heads, int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
-                          int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal,
-                          int32_t dtype, void* stream);
+/* The backward of es_packed_attn_fwd: dq [total_q, heads, D] and dk, dv [total_k, kv_heads, D] contiguous, dk and dv summed over the query heads
+ * of the key's group. o and o_rest (or NULL) are the forward's, dout has a token and a head stride. dq, or dk and dv, may be NULL. One owner per row and no
+ * atomics: the same inputs give the same bits. workspace: es_packed_bwd_workspace_bytes bytes. */
+long long es_packed_bwd_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D);
+int es_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse,
+                       void* dq, void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k,
+                       int32_t heads, int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
+                       int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal, int32_t dtype,
+                       void* workspace, void* stream);
 
 /* Attention of the newest `tokens` queries of each request to a shared prefix and to the request's own tokens, both in pages of a cache
  * k_cache, v_cache [pages, page_size, kv_heads, D] (page, token and head strides). q, o [batch, tokens, heads, D] contiguous, lse

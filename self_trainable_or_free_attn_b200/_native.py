@@ -73,11 +73,10 @@ SIGNATURES = {
                                _I, _I, _I, _P],
     "es_vsa_tier_rep_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
     "es_vsa_tier_unpool": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
-    "es_packed_workspace_bytes": [_I] * 6,
+    "es_packed_fwd_workspace_bytes": [_I] * 6,
     "es_packed_attn_fwd": [_P] * 8 + [_I] * 6 + [_I64] * 6 + [_F, _I, _I, _P, _P],
-    "es_packed_delta": [_P, _P, _P, _P, _I, _I, _I, _I64, _I64, _I, _P],
-    "es_packed_attn_bwd_q": [_P] * 9 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
-    "es_packed_attn_bwd_kv": [_P] * 10 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P],
+    "es_packed_bwd_workspace_bytes": [_I] * 6,
+    "es_packed_attn_bwd": [_P] * 12 + [_I] * 6 + [_I64] * 8 + [_F, _I, _I, _P, _P],
     "es_prefix_workspace_bytes": [_I] * 8,
     "es_prefix_attn": [_P] * 6 + [_I, _I, _P, _I, _P] + [_I] * 7 + [_I64] * 6 + [_F, _I, _P, _P],
     "es_extend_tables": [_P] * 4 + [_I] * 5 + [_P] * 6,
@@ -86,8 +85,8 @@ SIGNATURES = {
 _RESTYPES = {"es_last_error": ctypes.c_char_p, "es_launch_count": ctypes.c_longlong,
              "es_dense_scratch_bytes": ctypes.c_longlong,
              "es_vsa_topk_workspace_bytes": ctypes.c_longlong, "es_vsa_split_plan_workspace_bytes": ctypes.c_longlong,
-             "es_vsa_topk_bits_offset": ctypes.c_longlong, "es_packed_workspace_bytes": ctypes.c_longlong,
-             "es_prefix_workspace_bytes": ctypes.c_longlong}
+             "es_vsa_topk_bits_offset": ctypes.c_longlong, "es_packed_fwd_workspace_bytes": ctypes.c_longlong,
+             "es_packed_bwd_workspace_bytes": ctypes.c_longlong, "es_prefix_workspace_bytes": ctypes.c_longlong}
 
 _lib = None
 

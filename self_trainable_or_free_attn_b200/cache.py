@@ -54,8 +54,7 @@ def extend_tables(lengths, new_tokens, table, free_pages, page_size, *, total):
         raise ValueError(f"page_size must be at least 1, got {page_size}")
     if not 0 <= total < 2 ** 31:
         raise ValueError(f"total must be 0 or more, got {total}")
-    mk = lambda n: torch.empty(n, device=table.device, dtype=torch.int32)
-    plan = CachePlan(mk(total), mk(total), mk(B + 1), mk(B), mk(2))
+    plan = CachePlan(*torch.empty(2 * total + 2 * B + 3, device=table.device, dtype=torch.int32).split_with_sizes((total, total, B + 1, B, 2)))
     _call("es_extend_tables", N.ptr(lengths), N.ptr(new_tokens), N.ptr(table), N.ptr(free_pages), free_pages.numel(), B, width, page_size,
           total, N.ptr(plan.slots), N.ptr(plan.positions), N.ptr(plan.cu_new), N.ptr(plan.lengths), N.ptr(plan.taken), N.stream_ptr())
     return plan

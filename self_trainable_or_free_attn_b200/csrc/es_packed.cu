@@ -12,8 +12,10 @@ namespace packed {
 
 int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, void* o_rest,
                   float* lse, const Batch& b, int D, int dtype, void* ws, cudaStream_t st);
-int packed_bwd_tc(bool kv, const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const float* lse, const float* delta,
-                  void* d0, void* d1, const Batch& b, int D, int dtype, cudaStream_t st);
+long long packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D);
+int packed_bwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const float* lse, const float* delta, void* dq,
+                  void* dk, void* dv, const Batch& b, int D, int dtype, void* ws, cudaStream_t st);
+long long packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D);
 
 namespace {
 
@@ -54,7 +56,10 @@ template <typename F> int with_type(int dtype, int D, F f) {
 using namespace es;
 using namespace es::packed;
 
-extern "C" long long es_packed_workspace_bytes(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+extern "C" long long es_packed_fwd_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D) {
+    if (check_sizes("es_packed_fwd_workspace_bytes", batch, total_q, total_k, heads, kv_heads, D, 0)) return 0;
+    return packed_fwd_workspace(batch, total_q, total_k, heads, kv_heads, D);
+}
 
 extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, const int32_t* cu_q, const int32_t* cu_k,
                                   int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D,
@@ -62,60 +67,54 @@ extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, v
                                   float scale, int32_t causal, int32_t dtype, void* workspace, void* stream) {
     if (int rc = check_sizes("es_packed_attn_fwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
     if (total_q == 0) return 0;
-    if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v))) return set_error(-1, "es_packed_attn_fwd: null pointer");
-    if (!aligned(16, q, k, v, workspace) || !aligned(32, o, o_rest))
-        return set_error(-1, "es_packed_attn_fwd: q, k, v and the workspace must be 16-byte, o and o_rest 32-byte aligned");
+    if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v)) || (!workspace && packed_fwd_workspace(batch, total_q, total_k, heads, kv_heads, D)))
+        return set_error(-1, "es_packed_attn_fwd: null pointer");
+    if (!aligned(16, q, k, v) || !aligned(32, o, o_rest, workspace))
+        return set_error(-1, "es_packed_attn_fwd: q, k, v must be 16-byte, o, o_rest and the workspace 32-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head)) return set_error(-1, "es_packed_attn_fwd: strides must be multiples of 8 elements");
     const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
     return packed_fwd_tc(q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, o, o_rest, lse, b, D, dtype, workspace, (cudaStream_t)stream);
 }
 
-extern "C" int es_packed_delta(const void* o, const void* o_rest, const void* dout, float* delta, int32_t total_q, int32_t heads, int32_t D, int64_t do_token,
-                               int64_t do_head, int32_t dtype, void* stream) {
-    if (int rc = check_sizes("es_packed_delta", 0, total_q, 0, heads, heads, D, dtype)) return rc;
-    if (total_q == 0) return 0;
-    if (!o || !dout || !delta) return set_error(-1, "es_packed_delta: null pointer");
-    if (!aligned(16, o, o_rest, dout)) return set_error(-1, "es_packed_delta: o, o_rest and dout must be 16-byte aligned");
-    if (!whole_chunks(do_token, do_head)) return set_error(-1, "es_packed_delta: strides must be multiples of 8 elements");
-    return with_type(dtype, D, [&](auto t, auto d) {
-        using T = decltype(t);
-        const int64_t grid = ((int64_t)total_q * heads * (d / 8) + 255) / 256;
-        if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_delta: too many rows");
-        delta_kernel<T, d><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>((const uint4*)o, (const uint4*)o_rest, (const T*)dout, {do_token, do_head}, delta, total_q,
-                                                                             heads);
-        ES_CHECK_LAUNCH("delta_kernel");
-        return 0;
-    });
+// The workspace of the backward: delta, then what dK / dV shared out over several CTAs needs.
+static long long delta_bytes(int total_q, int heads) { return ((long long)total_q * heads * 4 + 255) / 256 * 256; }
+
+extern "C" long long es_packed_bwd_workspace_bytes(int32_t batch, int32_t total_q, int32_t total_k, int32_t heads, int32_t kv_heads, int32_t D) {
+    if (check_sizes("es_packed_bwd_workspace_bytes", batch, total_q, total_k, heads, kv_heads, D, 0)) return 0;
+    return delta_bytes(total_q, heads) + packed_bwd_workspace(batch, total_q, total_k, heads, kv_heads, D);
 }
 
-extern "C" int es_packed_attn_bwd_q(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq,
-                                    const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k, int32_t heads,
-                                    int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
-                                    int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal,
-                                    int32_t dtype, void* stream) {
-    if (int rc = check_sizes("es_packed_attn_bwd_q", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
-    if (total_q == 0) return 0;
-    if (!q || !dout || !lse || !delta || !dq || !cu_q || !cu_k || (total_k && (!k || !v))) return set_error(-1, "es_packed_attn_bwd_q: null pointer");
-    if (!aligned(16, q, k, v, dout, dq)) return set_error(-1, "es_packed_attn_bwd_q: q, k, v, dout, dq must be 16-byte aligned");
+extern "C" int es_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dout, const float* lse, void* dq,
+                                  void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k,
+                                  int32_t heads, int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head,
+                                  int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal, int32_t dtype,
+                                  void* workspace, void* stream) {
+    if (int rc = check_sizes("es_packed_attn_bwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
+    if (!total_q) dq = nullptr;
+    if (!total_k) dk = dv = nullptr;
+    if (!dq && !dk && !dv) return 0;
+    if ((dk == nullptr) != (dv == nullptr)) return set_error(-1, "es_packed_attn_bwd: null pointer (dk and dv go together)");
+    if (!cu_q || !cu_k || (total_q && (!q || !o || !dout || !lse || !workspace)) || (total_k && (!k || !v)) ||
+        (!workspace && packed_bwd_workspace(batch, total_q, total_k, heads, kv_heads, D)))
+        return set_error(-1, "es_packed_attn_bwd: null pointer");
+    if (!aligned(16, q, k, v, o, o_rest, dout) || !aligned(32, dq, dk, dv, workspace))
+        return set_error(-1, "es_packed_attn_bwd: q, k, v, o, o_rest, dout must be 16-byte, dq, dk, dv and the workspace 32-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head, do_token, do_head))
-        return set_error(-1, "es_packed_attn_bwd_q: strides must be multiples of 8 elements");
+        return set_error(-1, "es_packed_attn_bwd: strides must be multiples of 8 elements");
+    const cudaStream_t st = (cudaStream_t)stream;
+    float* delta = static_cast<float*>(workspace);
+    if (total_q) {
+        const int rc = with_type(dtype, D, [&](auto t, auto d) {
+            using T = decltype(t);
+            const int64_t grid = ((int64_t)total_q * heads * (d / 8) + 255) / 256;
+            if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many rows");
+            delta_kernel<T, d><<<(unsigned)grid, 256, 0, st>>>((const uint4*)o, (const uint4*)o_rest, (const T*)dout, {do_token, do_head}, delta, total_q, heads);
+            ES_CHECK_LAUNCH("delta_kernel");
+            return 0;
+        });
+        if (rc) return rc;
+    }
     const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
-    return packed_bwd_tc(false, q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, dout, {do_token, do_head}, lse, delta, dq, nullptr, b, D, dtype,
-                         (cudaStream_t)stream);
-}
-
-extern "C" int es_packed_attn_bwd_kv(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dk,
-                                     void* dv, const int32_t* cu_q, const int32_t* cu_k, int32_t batch, int32_t total_q, int32_t total_k,
-                                     int32_t heads, int32_t kv_heads, int32_t D, int64_t q_token, int64_t q_head, int64_t k_token,
-                                     int64_t k_head, int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale,
-                                     int32_t causal, int32_t dtype, void* stream) {
-    if (int rc = check_sizes("es_packed_attn_bwd_kv", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
-    if (total_k == 0) return 0;
-    if (!k || !v || !dk || !dv || !cu_q || !cu_k || (total_q && (!q || !dout || !lse || !delta))) return set_error(-1, "es_packed_attn_bwd_kv: null pointer");
-    if (!aligned(16, q, k, v, dout, dk, dv)) return set_error(-1, "es_packed_attn_bwd_kv: q, k, v, dout, dk, dv must be 16-byte aligned");
-    if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head, do_token, do_head))
-        return set_error(-1, "es_packed_attn_bwd_kv: strides must be multiples of 8 elements");
-    const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
-    return packed_bwd_tc(true, q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, dout, {do_token, do_head}, lse, delta, dk, dv, b, D, dtype,
-                         (cudaStream_t)stream);
+    return packed_bwd_tc(q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, dout, {do_token, do_head}, lse, delta, dq, dk, dv, b, D, dtype,
+                         static_cast<uint8_t*>(workspace) + delta_bytes(total_q, heads), st);
 }

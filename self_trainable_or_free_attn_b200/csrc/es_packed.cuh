@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -62,6 +63,12 @@ inline int check_sizes(const char* name, int B, int Tq, int Tk, int H, int Hk, i
     else if (D != 64 && D != 128) what = ": D must be 64 or 128";
     else if (dtype != 0 && dtype != 1) what = ": dtype must be 0 (bf16) or 1 (fp16)";
     return what ? set_error(-1, (std::string(name) + what).c_str()) : 0;
+}
+
+inline int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+    return n;
 }
 
 template <typename... S> inline bool whole_chunks(S... s) { return (((uint64_t)s | ... | 0ull) & 7) == 0; }

@@ -40,12 +40,16 @@ struct BwdArgs {
     int pack, tokens;                                        // heads per row group, tokens per 128 rows
     const float *lse, *delta;
     void *d0, *d1;                                           // dQ, or dK and dV
+    int splits;                                              // CTAs that share the rows a key tile is walked by
+    float* part;                                             // their sums: [split][dV, dK][key][head][D]
     const void* dout;                                        // for what is not finite
     Rows rdo;
     int* status;
 };
 
-template <typename T, int D> __device__ __forceinline__ void store_row(T* dst, uint32_t tcol, int from, int to, bool any, bool valid, float factor) {
+// A thread's row of an accumulator in tensor memory, columns 32 from .. 32 to - 1, times a factor: to dst, or as it is to part.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T* dst, float* part, uint32_t tcol, int from, int to, bool any, bool valid, float factor) {
 #pragma unroll 1
     for (int h = from; h < to; ++h) {
         uint32_t g[32];
@@ -56,13 +60,17 @@ template <typename T, int D> __device__ __forceinline__ void store_row(T* dst, u
             tmem_wait_ld_regs(g);
         }
         if (!valid) continue;
-        uint4* out = reinterpret_cast<uint4*>(dst + 32 * h);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t p[4];
+        for (int j = 0; j < 32; ++j) g[j] = __float_as_uint(__uint_as_float(g[j]) * factor);
+        if (part) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) p[x] = pack2<T>(__uint_as_float(g[8 * j + 2 * x]) * factor, __uint_as_float(g[8 * j + 2 * x + 1]) * factor);
-            out[j] = make_uint4(p[0], p[1], p[2], p[3]);
+            for (int j = 0; j < 4; ++j) store8(part + 32 * h + 8 * j, g + 8 * j);
+        } else {
+            uint32_t p[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) p[j] = pack2<T>(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
+            store8(dst + 32 * h, p);
+            store8(dst + 32 * h + 16, p + 8);
         }
     }
 }
@@ -87,9 +95,9 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     constexpr uint32_t DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kh = blockIdx.x % a.b.Hk;
+    const int wide = a.b.Hk * a.splits, kh = blockIdx.x % wide % a.b.Hk, split = blockIdx.x % wide / a.b.Hk;
     // (the first keys of a causal sequence are seen by the most queries)
-    const Piece at = find_piece(a.b.cu_k, a.b.B, a.b.Tk, blockIdx.x / a.b.Hk, TN, lane);
+    const Piece at = find_piece(a.b.cu_k, a.b.B, a.b.Tk, blockIdx.x / wide, TN, lane);
     if (at.n <= 0) return;
     int q0 = 0, nq = 0, diag = 0, first = 0;                 // diag: query t sees the owner's keys 0 .. t + diag
     if (at.seq >= 0) {
@@ -98,7 +106,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         diag = a.b.causal ? at.length - nq - at.offset : TN;
         first = min(max(-diag, 0), nq);                      // the first query that sees one of them
     }
-    const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens, nt = subs * per;
+    const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens;
+    const int tile0 = (int)((int64_t)subs * per * split / a.splits), nt = (int)((int64_t)subs * per * (split + 1) / a.splits) - tile0;
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -148,8 +157,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float* row_delta = row_lse + C::NROW * TM;
     uint32_t issued = 0;
     // walked tile i: query heads head0 .., first token
-    auto head_of = [&](int i) { return kh * a.b.G + (i / per) * a.pack; };
-    auto token_of = [&](int i) { return first + (i % per) * a.tokens; };
+    auto head_of = [&](int i) { return kh * a.b.G + (tile0 + i) / per * a.pack; };
+    auto token_of = [&](int i) { return first + (tile0 + i) % per * a.tokens; };
 
     if (warp >= 8) {
         reg_dec<REGS_REST>();
@@ -362,7 +371,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             const bool valid = r < at.n;
             // warps 0-3 write dV, warps 4-7 dK
             T* dst = static_cast<T*>(ch ? a.d0 : a.d1) + row * D;
-            store_row<T, D>(dst, tl + (ch ? DK_COL : DV_COL), 0, D / 32, nt > 0, valid, ch ? a.b.scale : 1.f);
+            float* part = a.splits > 1 ? a.part + ((int64_t)(2 * split + ch) * a.b.Tk * a.b.Hk + row) * D : nullptr;
+            store_row<T, D>(dst, part, tl + (ch ? DK_COL : DV_COL), 0, D / 32, nt > 0, valid, ch ? a.b.scale : 1.f);
             if (ch == 0 && valid && nt > 0 && *reinterpret_cast<volatile int*>(&ctl->not_finite)) {
                 // what is not finite in dO of the rows of cut tiles that see this key
                 for (int i = 0; i < nt; ++i) {
@@ -373,7 +383,9 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                             const T* src = static_cast<const T*>(a.dout) + (int64_t)(q0 + t) * a.rdo.token + (int64_t)h * a.rdo.head;
                             for (int d = 0; d < D; ++d) {
                                 const float e = to_float(src[d]);
-                                if (!(fabsf(e) < INFINITY)) dst[d] = from_float<T>(to_float(dst[d]) + e);
+                                if (fabsf(e) < INFINITY) continue;
+                                if (part) part[d] += e;
+                                else dst[d] = from_float<T>(to_float(dst[d]) + e);
                             }
                         }
                 }
@@ -391,7 +403,12 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (*abort_flag)
+    if (*abort_flag && a.splits > 1) {
+        for (int e = tid; e < at.n * D; e += THREADS) {
+            const int64_t w = ((int64_t)(at.first + e / D) * a.b.Hk + kh) * D + e % D, all = (int64_t)a.b.Tk * a.b.Hk * D;
+            a.part[2 * split * all + w] = a.part[(2 * split + 1) * all + w] = __uint_as_float(kNaN32);
+        }
+    } else if (*abort_flag)
         for (int e = tid; e < at.n * (D / 2); e += THREADS) {
             const int64_t w = ((int64_t)(at.first + e / (D / 2)) * a.b.Hk + kh) * (D / 2) + e % (D / 2);
             static_cast<uint32_t*>(a.d0)[w] = static_cast<uint32_t*>(a.d1)[w] = kNaN16x2;
@@ -602,7 +619,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (ok) {
             tc_fence_after();
             T* dst = static_cast<T*>(a.d0) + ((int64_t)(at.first + tok) * a.b.H + head) * D;
-            store_row<T, D>(dst, tl + DQ_COL, ch * (D / 64), (ch + 1) * (D / 64), nt > 0, valid, a.b.scale);
+            store_row<T, D>(dst, nullptr, tl + DQ_COL, ch * (D / 64), (ch + 1) * (D / 64), nt > 0, valid, a.b.scale);
         }
     }
 
@@ -623,8 +640,37 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
 }
 
+// dK, dV = the sums of their parts in the order of the CTAs; four values a thread.
+template <typename T> __global__ void __launch_bounds__(256) sum_kernel(const float4* part, T* dk, T* dv, int splits, int64_t n4) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= 2 * n4) return;
+    float4 s = part[i];
+    for (int p = 1; p < splits; ++p) {
+        const float4 x = part[2 * p * n4 + i];
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    T* dst = i < n4 ? dv + 4 * i : dk + 4 * (i - n4);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
+
+// CTAs that share the rows that walk a key tile: as many as make the pass shortest, in walked tiles. What is known of the lengths is
+// their mean; START: a CTA's start and end; the longest walk is taken for twice the mean of uneven sequences.
+static int kv_splits(int B, int Tq, int Tk, int H, int Hk, int D) {
+    constexpr double START = 6, LAUNCH = 4, BYTES = 4e6;     // a launch, and the bytes of the parts that move, in the time of a tile
+    const int sms = sm_count(), pack = rows_pack(H / Hk), tokens = TM / pack;
+    const double tiles = Hk * (Tk / (double)TN + 0.5 * B), walk = (double)Tq / std::max(1, B) / tokens * (H / Hk / pack), longest = B > 1 ? 2 * walk : walk;
+    int best = 1;
+    double least = 0;
+    for (int n = 1; n <= 16; ++n) {
+        const double cost = std::max(tiles * n / sms * (0.5 * walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 16.0 * n * Tk * Hk * D / BYTES : 0);
+        if (n == 1 || cost < 0.9 * least) { best = n; least = cost; }
+    }
+    return best;
+}
+
 template <typename T, int D>
-static int launch(bool kv, const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const BwdArgs& a, cudaStream_t st) {
+static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, BwdArgs a, void* dq, void* dk, void* dv,
+                  cudaStream_t st) {
     CUtensorMap tq, tk, tv, tdo;
     // (a batch without queries or without keys loads none, but a map needs an extent)
     long long nq = a.b.Tq, nk = a.b.Tk;
@@ -635,33 +681,49 @@ static int launch(bool kv, const void* q, Rows rq, const void* k, Rows rk, const
     if (int rc = make_rows_map<T>(&tdo, dout, D, qh, nq, rdo, qbox, a.tokens)) return rc;
     if (int rc = make_rows_map<T>(&tk, k, D, kvh, nk, rk, 1, TN)) return rc;
     if (int rc = make_rows_map<T>(&tv, v, D, kvh, nk, rv, 1, TN)) return rc;
-    const int64_t grid = kv ? a.b.Hk * piece_slots(a.b.Tk, TN, a.b.B) : a.b.H / a.pack * piece_slots(a.b.Tq, a.tokens, a.b.B);
-    if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many tiles");
-    auto kern = kv ? packed_bwd_kv_kernel<T, D> : packed_bwd_q_kernel<T, D>;
-    if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
-    kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, tdo, a);
-    ES_CHECK_LAUNCH("packed_bwd_kernel");
+    for (int kv = 0; kv < 2; ++kv) {
+        if (!(kv ? dk : dq)) continue;
+        const int64_t grid = kv ? (int64_t)a.b.Hk * a.splits * piece_slots(a.b.Tk, TN, a.b.B) : a.b.H / a.pack * piece_slots(a.b.Tq, a.tokens, a.b.B);
+        if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many tiles");
+        auto kern = kv ? packed_bwd_kv_kernel<T, D> : packed_bwd_q_kernel<T, D>;
+        if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
+        a.d0 = kv ? dk : dq;
+        a.d1 = dv;
+        kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, tdo, a);
+        ES_CHECK_LAUNCH("packed_bwd_kernel");
+    }
+    if (dk && a.splits > 1) {
+        const int64_t n4 = (int64_t)a.b.Tk * a.b.Hk * D / 4, blocks = (2 * n4 + 255) / 256;
+        if (blocks > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many rows");
+        sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(reinterpret_cast<const float4*>(a.part), static_cast<T*>(dk), static_cast<T*>(dv), a.splits, n4);
+        ES_CHECK_LAUNCH("sum_kernel");
+    }
     return 0;
 }
 
-// The caller has checked sizes and pointers. kv: d0 = dK, d1 = dV; else d0 = dQ.
-int packed_bwd_tc(bool kv, const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const float* lse, const float* delta,
-                  void* d0, void* d1, const Batch& b, int D, int dtype, cudaStream_t st) {
+long long packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
+    const int n = kv_splits(B, Tq, Tk, H, Hk, D);
+    return n > 1 ? 2ll * n * Tk * Hk * D * 4 : 0;
+}
+
+// The caller has checked sizes and pointers; dq, or dk and dv, may be null. ws: packed_bwd_workspace bytes.
+int packed_bwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, const void* dout, Rows rdo, const float* lse, const float* delta, void* dq,
+                  void* dk, void* dv, const Batch& b, int D, int dtype, void* ws, cudaStream_t st) {
     BwdArgs a{};
     a.b = b;
     a.pack = rows_pack(b.G);
     a.tokens = TM / a.pack;
     a.lse = lse;
     a.delta = delta;
-    a.d0 = d0;
-    a.d1 = d1;
+    a.splits = kv_splits(b.B, b.Tq, b.Tk, b.H, b.Hk, D);
+    a.part = static_cast<float*>(ws);
     a.dout = dout;
     a.rdo = rdo;
     a.status = device_status_ptr();
     if (!a.status) return set_error(-2, "es_packed_attn_bwd: the device status word is not available on this device");
     if (D == 64)
-        return dtype == 0 ? launch<__nv_bfloat16, 64>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st) : launch<__half, 64>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st);
-    return dtype == 0 ? launch<__nv_bfloat16, 128>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st) : launch<__half, 128>(kv, q, rq, k, rk, v, rv, dout, rdo, a, st);
+        return dtype == 0 ? launch<__nv_bfloat16, 64>(q, rq, k, rk, v, rv, dout, rdo, a, dq, dk, dv, st) : launch<__half, 64>(q, rq, k, rk, v, rv, dout, rdo, a, dq, dk, dv, st);
+    return dtype == 0 ? launch<__nv_bfloat16, 128>(q, rq, k, rk, v, rv, dout, rdo, a, dq, dk, dv, st) : launch<__half, 128>(q, rq, k, rk, v, rv, dout, rdo, a, dq, dk, dv, st);
 }
 
 }  // namespace packed

@@ -631,16 +631,37 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     return 0;
 }
 
-// The caller has checked sizes and pointers.
+// CTAs that share the keys of a pair of row tiles: as many as make the launch shortest, in iterations of 128 keys. What is known of the
+// lengths is their mean; START: a tile's start and end; the longest walk is taken for twice the mean of uneven sequences.
+static int fwd_splits(int B, int Tq, int Tk, int H, int Hk, int D) {
+    constexpr double START = 4, LAUNCH = 3, BYTES = 8e6;     // a launch, and the bytes of the parts that move, in the time of an iteration
+    const int sms = sm_count(), pack = rows_pack(H / Hk), span = 2 * (TM / pack);
+    const double tiles = H / pack * (Tq / (double)span + 0.5 * B), walk = (double)Tk / std::max(1, B) / TN, longest = B > 1 ? 2 * walk : walk;
+    int best = 1;
+    double least = 0;
+    for (int n = 1; n <= 32; ++n) {
+        const double cost = std::max(tiles * n / sms * (walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 8.0 * n * Tq * H * D / BYTES : 0);
+        if (n == 1 || cost < 0.9 * least) { best = n; least = cost; }
+    }
+    return best;
+}
+
+long long packed_fwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D) {
+    const int n = fwd_splits(B, Tq, Tk, H, Hk, D);
+    return n > 1 ? (long long)n * Tq * H * (D + 1) * 4 : 0;
+}
+
+// The caller has checked sizes and pointers. ws: packed_fwd_workspace bytes.
 int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v, Rows rv, void* o, void* o_rest,
                   float* lse, const Batch& b, int D, int dtype, void* ws, cudaStream_t st) {
-    (void)ws;
     FwdArgs a{};
     a.b = b;
     a.pack = rows_pack(b.G);
     a.tokens = TM / a.pack;
-    a.splits = 1;
+    a.splits = fwd_splits(b.B, b.Tq, b.Tk, b.H, b.Hk, D);
     a.vheads = b.H / a.pack;
+    a.part_o = static_cast<float*>(ws);
+    a.part_lse = a.part_o + (int64_t)a.splits * b.Tq * b.H * D;
     a.o = o;
     a.o_rest = o_rest;
     a.lse = lse;

@@ -552,12 +552,6 @@ __global__ void __launch_bounds__(256) join_kernel(T* o, float* lse, const __gri
     if (lane == 0) lse[((int64_t)b * a.H + h) * a.N + i] = sum != 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-    return n;
-}
-
 // How a call is cut up, from its sizes alone: the workspace and the kernels go by the same plan.
 struct Plan {
     bool prefix_item, prefix_tiles, own;

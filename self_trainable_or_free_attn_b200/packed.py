@@ -30,9 +30,13 @@ def usable(t):
             and all(n == 1 or (s % 8 == 0 and t.shape[-1] <= s < 2 ** 39) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
 
 
+def _plain(t):
+    return t.is_contiguous() and t.data_ptr() % 16 == 0
+
+
 def rows(t):
     """t itself where the kernels can read it, else a copy."""
-    return t if usable(t) else t.clone(memory_format=torch.contiguous_format)
+    return t if _plain(t) or usable(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def strides(t):
@@ -77,14 +81,23 @@ def check_ints(ref, **tensors):
     for name, t in tensors.items():
         if t.device != ref.device:
             raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
-        if t.dtype not in (torch.int32, torch.int64):
-            raise RuntimeError(f"{name} must be int32, got {t.dtype}")
-        out.append(t.to(torch.int32).contiguous())
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            if t.dtype not in (torch.int32, torch.int64):
+                raise RuntimeError(f"{name} must be int32, got {t.dtype}")
+            t = t.to(torch.int32).contiguous()
+        out.append(t)
     return out
 
 
 def _call(name, *args):
-    N.check(getattr(N.load(), name)(*args), name)
+    rc = getattr(N.load(), name)(*args)
+    if rc:
+        N.check(rc, name)
+
+
+def _workspace(name, q, sizes):
+    n = getattr(N.load(), name)(*sizes)
+    return torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
 
 
 def _fwd(q, k, v, cu_q, cu_k, scale, causal, with_rest):
@@ -92,19 +105,17 @@ def _fwd(q, k, v, cu_q, cu_k, scale, causal, with_rest):
     o = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
     rest = torch.empty_like(o) if with_rest else None
     lse = torch.empty(H, T, device=q.device, dtype=torch.float32)
-    B, Hk = cu_q.numel() - 1, k.shape[1]
-    n = int(N.load().es_packed_workspace_bytes(B, T, k.shape[0], H, Hk, D))
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-    _call("es_packed_attn_fwd", N.ptr(q), N.ptr(k), N.ptr(v), N.ptr(o), N.ptr(rest), N.ptr(lse), N.ptr(cu_q), N.ptr(cu_k), B, T, k.shape[0], H,
-          Hk, D, *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
+    sizes = (cu_q.numel() - 1, T, k.shape[0], H, k.shape[1], D)
+    ws = _workspace("es_packed_fwd_workspace_bytes", q, sizes)
+    _call("es_packed_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), N.ptr(rest), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), *sizes,
+          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
     return o, rest, lse
 
 
 class _Function(torch.autograd.Function):
     @staticmethod
-    @N.device_guard
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
-        o, rest, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal, any(ctx.needs_input_grad[:3]))
+        o, rest, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal, True)
         ctx.save_for_backward(q, k, v, o, rest, lse, cu_q, cu_k)
         ctx.scale, ctx.causal = scale, causal
         ctx.mark_non_differentiable(lse)
@@ -119,20 +130,15 @@ class _Function(torch.autograd.Function):
             return (None,) * 7
         q, k, v, o, rest, lse, cu_q, cu_k = ctx.saved_tensors
         dout = rows(dout)
-        (T, H, D), (Tk, Hk, _) = q.shape, k.shape
-        delta = torch.empty_like(lse)
-        dt, st = _DTYPES[q.dtype], N.stream_ptr()
-        _call("es_packed_delta", N.ptr(o), N.ptr(rest), N.ptr(dout), N.ptr(delta), T, H, D, *strides(dout), dt, st)
-        sizes = (cu_q.numel() - 1, T, Tk, H, Hk, D, *strides(q), *strides(k), *strides(v), *strides(dout), ctx.scale, ctx.causal, dt, st)
-        ins = [N.ptr(t) for t in (q, k, v, dout, lse, delta)]
-        cus = (N.ptr(cu_q), N.ptr(cu_k))
-        dq = dk = dv = None
-        if ctx.needs_input_grad[0]:
-            dq = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
-            _call("es_packed_attn_bwd_q", *ins, N.ptr(dq), *cus, *sizes)
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dk, dv = (torch.empty(Tk, Hk, D, device=q.device, dtype=q.dtype) for _ in range(2))
-            _call("es_packed_attn_bwd_kv", *ins, N.ptr(dk), N.ptr(dv), *cus, *sizes)
+        sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        need = ctx.needs_input_grad
+        mk = lambda t: torch.empty(t.shape, device=t.device, dtype=t.dtype)
+        dq = mk(q) if need[0] else None
+        dk, dv = (mk(k), mk(v)) if need[1] or need[2] else (None, None)
+        ws = _workspace("es_packed_bwd_workspace_bytes", q, sizes)
+        _call("es_packed_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), N.ptr(dq), N.ptr(dk),
+              N.ptr(dv), cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides(q), *strides(k), *strides(v), *strides(dout), ctx.scale, ctx.causal, _DTYPES[q.dtype],
+              N.ptr(ws), N.stream_ptr())
         return dq, dk, dv, None, None, None, None
 
 
@@ -163,5 +169,9 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, retur
     if max(q.shape[0], k.shape[0]) >= 2 ** 31 - 256:
         raise RuntimeError("at most 2**31 - 257 tokens")
     scale = softmax_scale(scale, q.shape[2])
-    o, lse = _Function.apply(rows(q), rows(k), rows(v), cu_q, cu_k, scale, int(bool(causal)))
+    args = (rows(q), rows(k), rows(v), cu_q, cu_k, scale, int(bool(causal)))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _Function.apply(*args)
+    else:
+        o, _, lse = _fwd(*args, False)
     return (o, lse) if return_lse else o

@@ -10,23 +10,14 @@ BIG = 0x10000
 
 def _fwd(**over):
     a = dict(q=BIG, k=2 * BIG, v=3 * BIG, o=4 * BIG, rest=8 * BIG, lse=5 * BIG, cu_q=6 * BIG, cu_k=7 * BIG, B=2, Tq=10, Tk=12, H=4, Hk=2, D=64,
-             qt=256, qh=64, kt=128, kh=64, vt=128, vh=64, scale=0.1, causal=1, dtype=0, ws=None, st=None)
+             qt=256, qh=64, kt=128, kh=64, vt=128, vh=64, scale=0.1, causal=1, dtype=0, ws=9 * BIG, st=None)
     a.update(over)
     return a
 
 
-def _bwd(kv, **over):
-    a = dict(q=BIG, k=2 * BIG, v=3 * BIG, do=4 * BIG, lse=5 * BIG, delta=6 * BIG, d0=7 * BIG)
-    if kv:
-        a["d1"] = 8 * BIG
-    a.update(cu_q=9 * BIG, cu_k=10 * BIG, B=2, Tq=10, Tk=12, H=4, Hk=2, D=64, qt=256, qh=64, kt=128, kh=64, vt=128, vh=64, dt=256, dh=64,
-             scale=0.1, causal=1, dtype=0, st=None)
-    a.update(over)
-    return a
-
-
-def _delta(**over):
-    a = dict(o=BIG, rest=None, do=2 * BIG, delta=3 * BIG, T=10, H=4, D=64, dt=256, dh=64, dtype=0, st=None)
+def _bwd(**over):
+    a = dict(q=BIG, k=2 * BIG, v=3 * BIG, o=4 * BIG, rest=None, do=5 * BIG, lse=6 * BIG, dq=7 * BIG, dk=8 * BIG, dv=9 * BIG, cu_q=10 * BIG, cu_k=11 * BIG, B=2,
+             Tq=10, Tk=12, H=4, Hk=2, D=64, qt=256, qh=64, kt=128, kh=64, vt=128, vh=64, dt=256, dh=64, scale=0.1, causal=1, dtype=0, ws=12 * BIG, st=None)
     a.update(over)
     return a
 
@@ -55,12 +46,10 @@ def _store(**over):
 SIZES = [dict(B=-1), dict(Tq=-1), dict(Tk=-1), dict(Tq=0x7FFFFF00), dict(H=0), dict(H=3), dict(Hk=0), dict(D=96), dict(dtype=2)]
 REFUSED = (
     [("es_packed_attn_fwd", _fwd, x) for x in SIZES + [dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(lse=None), dict(cu_q=None), dict(cu_k=None),
-                                                       dict(q=BIG + 8), dict(k=BIG + 8), dict(v=BIG + 2), dict(o=BIG + 8), dict(rest=BIG + 8), dict(qt=257), dict(kh=60), dict(vt=4)]]
-    + [(f"es_packed_attn_bwd_{n}", lambda kv=kv, **o: _bwd(kv, **o), x) for n, kv in (("q", False), ("kv", True))
-       for x in SIZES + [dict(q=None), dict(do=None), dict(lse=None), dict(delta=None), dict(d0=None), dict(cu_q=None), dict(do=BIG + 8), dict(d0=BIG + 8), dict(dt=4),
-                         dict(qh=65)]]
-    + [("es_packed_delta", _delta, x) for x in [dict(T=-1), dict(H=0), dict(D=32), dict(dtype=3), dict(o=None), dict(do=None), dict(delta=None), dict(o=BIG + 8),
-                                                dict(do=BIG + 8), dict(dh=3)]]
+                                                       dict(q=BIG + 8), dict(k=BIG + 8), dict(v=BIG + 2), dict(o=BIG + 16), dict(rest=BIG + 8), dict(ws=BIG + 16), dict(qt=257), dict(kh=60), dict(vt=4)]]
+    + [("es_packed_attn_bwd", _bwd, x) for x in SIZES + [dict(q=None), dict(k=None), dict(o=None), dict(do=None), dict(lse=None), dict(dk=None), dict(dv=None), dict(cu_q=None),
+                                                         dict(cu_k=None), dict(ws=None), dict(do=BIG + 8), dict(rest=BIG + 8), dict(dq=BIG + 16), dict(dk=BIG + 16), dict(ws=BIG + 16),
+                                                         dict(dt=4), dict(qh=65)]]
     + [("es_prefix_attn", _prefix, x) for x in [dict(B=-1), dict(N=-1), dict(H=3), dict(D=32), dict(dtype=9), dict(page=48), dict(page=512), dict(plen=49), dict(plen=-1),
                                                 dict(width=-1), dict(P=-1), dict(np=-1), dict(P=2 ** 30), dict(width=2 ** 28), dict(q=None), dict(k=None), dict(o=None),
                                                 dict(lse=None), dict(pages=None), dict(table=None), dict(lengths=None), dict(q=BIG + 8), dict(v=BIG + 8), dict(o=BIG + 4),
@@ -69,8 +58,7 @@ REFUSED = (
                                                   dict(free=None), dict(slots=None), dict(pos=None), dict(cu=None), dict(out=None), dict(taken=None)]]
     + [("es_store_kv", _store, x) for x in [dict(T=-1), dict(Hk=0), dict(D=80), dict(P=-1), dict(page=0), dict(P=2 ** 30), dict(k=None), dict(vc=None), dict(slots=None),
                                             dict(k=BIG + 8), dict(kc=BIG + 8), dict(kt=4), dict(vcp=2050)]])
-GOOD = {"es_packed_attn_fwd": _fwd, "es_packed_attn_bwd_q": lambda **o: _bwd(False, **o), "es_packed_attn_bwd_kv": lambda **o: _bwd(True, **o),
-        "es_packed_delta": _delta, "es_prefix_attn": _prefix, "es_extend_tables": _extend, "es_store_kv": _store}
+GOOD = {"es_packed_attn_fwd": _fwd, "es_packed_attn_bwd": _bwd, "es_prefix_attn": _prefix, "es_extend_tables": _extend, "es_store_kv": _store}
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are made up: without a GPU no call can reach a kernel with them")
@@ -89,9 +77,9 @@ def test_empty_calls_return_at_once():
     from self_trainable_or_free_attn_b200 import _native
     lib = _native.load()
     assert lib.es_packed_attn_fwd(*_fwd(Tq=0).values()) == 0
-    assert lib.es_packed_delta(*_delta(T=0).values()) == 0
-    assert lib.es_packed_attn_bwd_q(*_bwd(False, Tq=0).values()) == 0
-    assert lib.es_packed_attn_bwd_kv(*_bwd(True, Tk=0).values()) == 0
+    assert lib.es_packed_attn_bwd(*_bwd(Tq=0, Tk=0).values()) == 0
+    assert lib.es_packed_attn_bwd(*_bwd(dq=None, dk=None, dv=None).values()) == 0
+    assert lib.es_packed_attn_bwd(*_bwd(Tk=0, dq=None).values()) == 0
     assert lib.es_prefix_attn(*_prefix(B=0).values()) == 0
     assert lib.es_store_kv(*_store(T=0).values()) == 0
 
