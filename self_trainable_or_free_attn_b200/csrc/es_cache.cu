@@ -7,7 +7,7 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------- pages and slots
 constexpr int PLAN_THREADS = 256, PLAN_CHUNK = 1024;          // requests that a CTA scans at a time
-constexpr int PLAN_TOKENS = 1024;                             // tokens of a CTA
+constexpr int PLAN_TOKENS = 256;                              // tokens of a CTA: one to a thread
 
 struct PlanArgs {
     const int *lengths, *new_tokens, *free_pages;
@@ -15,30 +15,35 @@ struct PlanArgs {
     int n_free, B, width, page, total;
 };
 
+// Pages of x tokens (x below 2^32, which the sum of two lengths is).
+__device__ __forceinline__ unsigned pages_of(unsigned x, unsigned page) { return x ? (x - 1) / page + 1 : 0; }
+
 // With len = lengths[b], n = new_tokens[b]: the request has have = ceil(len / page) pages and wants ceil((len + n) / page), at most the row's
 // width; its missing pages are free_pages[first ...], first the exclusive sum of need = wanted - held over the requests before it. Every CTA
 // makes both running sums itself (a few KB of L2 per thousand requests; a second kernel would cost a launch) and then places its own
-// share of the requests and of the tokens.
+// share of the requests and of the tokens. Bound by latency: lengths, the free list or the table, stores.
 __global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a) {
-    __shared__ int s_cu[PLAN_CHUNK + 1], s_first[PLAN_CHUNK + 1];
+    __shared__ int s_cu[PLAN_CHUNK + 1], s_first[PLAN_CHUNK], s_len[PLAN_CHUNK];
     __shared__ long long s_warp[2][PLAN_THREADS / 32];
     constexpr int PER = PLAN_CHUNK / PLAN_THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long cap = 0x7FFFFFFF;
+    const unsigned page = (unsigned)a.page, width = (unsigned)a.width;
     long long tokens = 0, pages = 0, missing = 0;             // of the chunks before (the sums may pass 32 bits; what is stored saturates)
     const long long t0 = (long long)blockIdx.x * PLAN_TOKENS, t1 = min(t0 + PLAN_TOKENS, (long long)a.total);
     for (int b0 = 0; b0 < a.B; b0 += PLAN_CHUNK) {
         const int nb = min(PLAN_CHUNK, a.B - b0);
-        long long n[PER], need[PER], sn = 0, sp = 0;
+        unsigned len[PER], n[PER];
+#pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int b = b0 + tid * PER + i;
-            n[i] = need[i] = 0;
-            if (b < b0 + nb) {
-                const long long len = max(a.lengths[b], 0);
-                n[i] = max(a.new_tokens[b], 0);
-                const long long have = min((len + a.page - 1) / a.page, (long long)a.width), want = min((len + n[i] + a.page - 1) / a.page, (long long)a.width);
-                need[i] = want - have;
-            }
+            const int r = tid * PER + i;
+            len[i] = r < nb ? max(a.lengths[b0 + r], 0) : 0;
+            n[i] = r < nb ? max(a.new_tokens[b0 + r], 0) : 0;
+        }
+        long long need[PER], sn = 0, sp = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            need[i] = (long long)min(pages_of(len[i] + n[i], page), width) - (long long)min(pages_of(len[i], page), width);
             sn += n[i]; sp += need[i];
         }
         long long xn = sn, xp = sp;
@@ -49,26 +54,29 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a)
         if (lane == 31) { s_warp[0][warp] = xn; s_warp[1][warp] = xp; }
         __syncthreads();
         long long bn = tokens, bp = pages, an = tokens, ap = pages;
+#pragma unroll
         for (int w = 0; w < PLAN_THREADS / 32; ++w) {
             if (w < warp) { bn += s_warp[0][w]; bp += s_warp[1][w]; }
             an += s_warp[0][w]; ap += s_warp[1][w];
         }
         bn += xn - sn; bp += xp - sp;
+#pragma unroll
         for (int i = 0; i < PER; ++i) {
             s_cu[tid * PER + i] = (int)min(bn, cap);
             s_first[tid * PER + i] = (int)min(bp, cap);
+            s_len[tid * PER + i] = (int)len[i];
             bn += n[i]; bp += need[i];
         }
-        if (tid == 0) { s_cu[PLAN_CHUNK] = (int)min(an, cap); s_first[PLAN_CHUNK] = (int)min(ap, cap); }
+        if (tid == 0) s_cu[PLAN_CHUNK] = (int)min(an, cap);
         __syncthreads();
         // requests: their lengths, table entries and shares of the outputs, spread over the CTAs
         for (int r = blockIdx.x * PLAN_THREADS + tid; r < nb; r += gridDim.x * PLAN_THREADS) {
-            const int b = b0 + r, len = max(a.lengths[b], 0);
-            const long long after = (long long)len + max(a.new_tokens[b], 0);
-            const int have = (int)min(((long long)len + a.page - 1) / a.page, (long long)a.width), want = (int)min((after + a.page - 1) / a.page, (long long)a.width);
+            const int b = b0 + r;
+            const unsigned l = (unsigned)s_len[r], after = l + max(a.new_tokens[b], 0);
+            const int have = (int)min(pages_of(l, page), width), want = (int)min(pages_of(after, page), width);
             const int first = s_first[r], got = min(max(a.n_free - first, 0), want - have);
             for (int j = have; j < want; ++j) a.table[(size_t)b * a.width + j] = j - have < got ? a.free_pages[first + j - have] : -1;
-            a.lengths_out[b] = max(len, (int)min(after, min((long long)(have + got) * a.page, cap)));
+            a.lengths_out[b] = max((int)l, (int)min(min((long long)after, cap), (long long)(have + got) * a.page));
             a.cu_new[b] = s_cu[r];
         }
         // tokens of this CTA that belong to the chunk
@@ -79,20 +87,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a)
                 const int m = (x + y) >> 1;
                 if (s_cu[m] <= t) x = m; else y = m;
             }
-            const int b = b0 + x, len = max(a.lengths[b], 0);
-            const long long pos = (long long)len + (t - s_cu[x]), col = pos / a.page;
-            const int have = (int)min(((long long)len + a.page - 1) / a.page, (long long)a.width);
+            const unsigned l = (unsigned)s_len[x], pos = l + (unsigned)(t - s_cu[x]), col = pos / page, have = min(pages_of(l, page), width);
             int p = -1;
-            if (col < have) p = a.table[(size_t)b * a.width + col];       // (held before the call: nobody writes it)
-            else if (col < a.width && s_first[x] + (col - have) < a.n_free) p = a.free_pages[s_first[x] + (col - have)];
-            const long long slot = (long long)p * a.page + pos % a.page;
+            if (col < have) p = a.table[(size_t)(b0 + x) * a.width + col];        // (held before the call: nobody writes it)
+            else if (col < width && s_first[x] + (long long)(col - have) < a.n_free) p = a.free_pages[s_first[x] + (col - have)];
+            const long long slot = (long long)p * a.page + (pos - col * page);
             a.slots[t] = p >= 0 && slot <= cap ? (int)slot : -1;
-            a.positions[t] = (int)min(pos, cap);
+            a.positions[t] = (int)min((long long)pos, cap);
         }
         if (blockIdx.x == 0)
             for (int r = tid; r < nb; r += PLAN_THREADS) {    // pages needed and not there
-                const int b = b0 + r, len = max(a.lengths[b], 0);
-                const long long held = ((long long)len + a.page - 1) / a.page, wanted = ((long long)len + max(a.new_tokens[b], 0) + a.page - 1) / a.page;
+                const unsigned l = (unsigned)s_len[r];
+                const long long held = pages_of(l, page), wanted = pages_of(l + max(a.new_tokens[b0 + r], 0), page);
                 const long long have = min(held, (long long)a.width), want = min(wanted, (long long)a.width);
                 missing += (wanted - held) - min(max((long long)a.n_free - s_first[r], 0ll), want - have);
             }
@@ -115,6 +121,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a)
 }
 
 // ---------------------------------------------------------------------------------------------- storing
+constexpr int STORE_TOKENS = 4;                               // of a CTA: as many copies of a thread on their way
+
 struct StoreArgs {
     const uint4 *k, *v;
     uint4 *kc, *vc;
@@ -124,21 +132,35 @@ struct StoreArgs {
     int total, Hk, pages, page;
 };
 
-// A thread per 16 bytes: consecutive threads take the chunks of a row of K, then of V.
+// A token's chunks of 16 bytes, K's rows and then V's, to consecutive threads; a thread has the same chunk of all tokens of its CTA.
 template <int D> __global__ void __launch_bounds__(256) store_kv_kernel(StoreArgs a) {
     constexpr int CH = D / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int c = (int)(i % CH);
-    const int64_t row = i / CH;
-    const int64_t th = row >> 1;
-    const int h = (int)(th % a.Hk);
-    const int64_t t = th / a.Hk;
-    if (t >= a.total) return;
-    const int slot = a.slots[t];
-    if (slot < 0 || slot / a.page >= a.pages) return;
-    const int page = slot / a.page, at = slot % a.page;
-    if (row & 1) a.vc[page * a.rvc.page + at * a.rvc.token + h * a.rvc.head + c] = a.v[t * a.rv.token + h * a.rv.head + c];
-    else a.kc[page * a.rkc.page + at * a.rkc.token + h * a.rkc.head + c] = a.k[t * a.rk.token + h * a.rk.head + c];
+    const int64_t t0 = (int64_t)blockIdx.x * STORE_TOKENS;
+    int slot[STORE_TOKENS];
+#pragma unroll
+    for (int j = 0; j < STORE_TOKENS; ++j) slot[j] = t0 + j < a.total ? __ldg(a.slots + t0 + j) : -1;
+    int64_t to_k[STORE_TOKENS], to_v[STORE_TOKENS];
+#pragma unroll
+    for (int j = 0; j < STORE_TOKENS; ++j) {
+        const int page = slot[j] / a.page, at = slot[j] - page * a.page;
+        if (slot[j] < 0 || page >= a.pages) slot[j] = -1;
+        to_k[j] = page * a.rkc.page + at * a.rkc.token;
+        to_v[j] = page * a.rvc.page + at * a.rvc.token;
+    }
+    for (int i = threadIdx.x; i < 2 * a.Hk * CH; i += 256) {
+        const bool is_v = i >= a.Hk * CH;
+        const int x = is_v ? i - a.Hk * CH : i, h = x / CH, c = x % CH;
+        const uint4* src = (is_v ? a.v + h * a.rv.head : a.k + h * a.rk.head) + c;
+        uint4* dst = (is_v ? a.vc + h * a.rvc.head : a.kc + h * a.rkc.head) + c;
+        const int64_t step = is_v ? a.rv.token : a.rk.token;
+        uint4 w[STORE_TOKENS];
+#pragma unroll
+        for (int j = 0; j < STORE_TOKENS; ++j)
+            if (slot[j] >= 0) w[j] = __ldcs(src + (t0 + j) * step);
+#pragma unroll
+        for (int j = 0; j < STORE_TOKENS; ++j)
+            if (slot[j] >= 0) dst[is_v ? to_v[j] : to_k[j]] = w[j];
+    }
 }
 
 }  // namespace
@@ -174,8 +196,7 @@ extern "C" int es_store_kv(const void* k, const void* v, void* k_cache, void* v_
         return set_error(-1, "es_store_kv: strides must be multiples of 8 elements");
     const StoreArgs a{(const uint4*)k, (const uint4*)v, (uint4*)k_cache, (uint4*)v_cache, slots, {k_token / 8, k_head / 8}, {v_token / 8, v_head / 8},
                       {kc_page / 8, kc_token / 8, kc_head / 8}, {vc_page / 8, vc_token / 8, vc_head / 8}, total, kv_heads, pages, page_size};
-    const int64_t n = (int64_t)total * kv_heads * 2 * (D / 8);
-    const unsigned grid = (unsigned)((n + 255) / 256);
+    const unsigned grid = (unsigned)(((int64_t)total + STORE_TOKENS - 1) / STORE_TOKENS);
     if (D == 64) store_kv_kernel<64><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
     else store_kv_kernel<128><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
     ES_CHECK_LAUNCH("store_kv_kernel");

@@ -71,6 +71,9 @@ inline int sm_count() {
     return n;
 }
 
+// Rounds of CTAs, from tiles per SM: whole ones where they are few, later ones fill up as the lengths differ.
+inline double rounds(double x) { return x < 4 ? std::ceil(x) : x; }
+
 template <typename... S> inline bool whole_chunks(S... s) { return (((uint64_t)s | ... | 0ull) & 7) == 0; }
 
 }  // namespace packed

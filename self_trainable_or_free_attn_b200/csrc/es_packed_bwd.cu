@@ -656,13 +656,13 @@ template <typename T> __global__ void __launch_bounds__(256) sum_kernel(const fl
 // CTAs that share the rows that walk a key tile: as many as make the pass shortest, in walked tiles. What is known of the lengths is
 // their mean; START: a CTA's start and end; the longest walk is taken for twice the mean of uneven sequences.
 static int kv_splits(int B, int Tq, int Tk, int H, int Hk, int D) {
-    constexpr double START = 6, LAUNCH = 4, BYTES = 4e6;     // a launch, and the bytes of the parts that move, in the time of a tile
+    constexpr double START = 6, LAUNCH = 4, BYTES = 8e6;     // a launch, and the bytes of the parts that move, in the time of a tile
     const int sms = sm_count(), pack = rows_pack(H / Hk), tokens = TM / pack;
     const double tiles = Hk * (Tk / (double)TN + 0.5 * B), walk = (double)Tq / std::max(1, B) / tokens * (H / Hk / pack), longest = B > 1 ? 2 * walk : walk;
     int best = 1;
     double least = 0;
     for (int n = 1; n <= 16; ++n) {
-        const double cost = std::max(tiles * n / sms * (0.5 * walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 16.0 * n * Tk * Hk * D / BYTES : 0);
+        const double cost = std::max(rounds(tiles * n / sms) * (0.5 * walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 16.0 * n * Tk * Hk * D / BYTES : 0);
         if (n == 1 || cost < 0.9 * least) { best = n; least = cost; }
     }
     return best;

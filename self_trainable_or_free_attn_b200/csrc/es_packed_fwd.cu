@@ -134,7 +134,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     constexpr int USERS = 10;                                // warps that take each tile's work
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (PAGED) launch_dependents();                          // the requests' own tokens may go ahead where an SM is free
+    launch_dependents();                                     // what follows waits for all of this, or (paged) has nothing to do with it
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -567,35 +567,29 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
 }
 
-// o = sum_p 2^(z_p - M) o_p / sum_p 2^(z_p - M), a warp per row; parts without a key (z = -inf) were not written and are not read.
+// o = sum_p 2^(z_p - M) o_p / sum_p 2^(z_p - M), a warp per row, a lane per part's LSE (at most 32 parts). What a part without a key (z =
+// -inf) holds was not written and does not count.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) merge_kernel(const float* part_o, const float* part_lse, T* o, T* o_rest, float* lse, int parts, int Tq, int H) {
+    constexpr int C = D / 32;
     const int lane = threadIdx.x & 31;
     const int64_t rows = (int64_t)Tq * H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    wait_prerequisites();
     if (row >= rows) return;
-    float top = -INFINITY;
-    bool nan = false;
-    for (int p = lane; p < parts; p += 32) {
-        const float z = part_lse[p * rows + row];
-        nan |= z != z;
-        top = fmaxf(top, z);
-    }
-    for (int i = 16; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-    constexpr int C = D / 32;
-    float acc[C] = {}, sum = 0.f;
+    const float z = lane < parts ? part_lse[lane * rows + row] : -INFINITY;
+    float top = z;
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float w = z == -INFINITY ? 0.f : z != z ? z : exp2f(z - top);
+    float acc[C] = {}, sum = w;
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float* src = part_o + row * D + C * lane;
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
-        const float z = part_lse[p * rows + row];
-        if (z == -INFINITY) continue;
-        const float w = exp2f(z - top);
-        sum += w;
-        const float* src = part_o + (p * rows + row) * D + C * lane;
-        if constexpr (C == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src);
-            acc[0] += w * v.x; acc[1] += w * v.y; acc[2] += w * v.z; acc[3] += w * v.w;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(src);
-            acc[0] += w * v.x; acc[1] += w * v.y;
-        }
+        const float wp = __shfl_sync(0xffffffffu, w, p);
+        float v[C];
+        load_floats<C>(src + p * rows * D, v);
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] += wp == 0.f ? 0.f : v[c] * wp;
     }
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
@@ -625,7 +619,9 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
     ES_CHECK_LAUNCH("packed_fwd_kernel");
     if (a.splits > 1) {
-        merge_kernel<T, D><<<(unsigned)(((int64_t)a.b.Tq * a.b.H + 7) / 8), 256, 0, st>>>(a.part_o, a.part_lse, static_cast<T*>(a.o), static_cast<T*>(a.o_rest), a.lse, a.splits, a.b.Tq, a.b.H);
+        const cudaError_t e = launch_dependent(merge_kernel<T, D>, dim3((unsigned)(((int64_t)a.b.Tq * a.b.H + 7) / 8)), dim3(256), 0, st, (const float*)a.part_o,
+                                               (const float*)a.part_lse, static_cast<T*>(a.o), static_cast<T*>(a.o_rest), a.lse, a.splits, a.b.Tq, a.b.H);
+        if (e != cudaSuccess) return set_error(-2, cudaGetErrorString(e));
         ES_CHECK_LAUNCH("merge_kernel");
     }
     return 0;
@@ -640,7 +636,7 @@ static int fwd_splits(int B, int Tq, int Tk, int H, int Hk, int D) {
     int best = 1;
     double least = 0;
     for (int n = 1; n <= 32; ++n) {
-        const double cost = std::max(tiles * n / sms * (walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 8.0 * n * Tq * H * D / BYTES : 0);
+        const double cost = std::max(rounds(tiles * n / sms) * (walk / n + START), longest / n + START) + (n > 1 ? LAUNCH + 8.0 * n * Tq * H * D / BYTES : 0);
         if (n == 1 || cost < 0.9 * least) { best = n; least = cost; }
     }
     return best;

@@ -120,6 +120,16 @@ __device__ __forceinline__ void store8(void* dst, const uint32_t* v) {
                  : "memory");
 }
 
+template <int N> __device__ __forceinline__ void load_floats(const float* src, float* v) {
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[0] = x.x; v[1] = x.y;
+    }
+}
+
 // After a wait has given up, whether an answer on its way to shared memory has come (100 us at most).
 __device__ __forceinline__ bool mbar_wait_answer(uint32_t bar, uint32_t parity) {
     const uint64_t t_end = global_timer_ns() + 100000ull;

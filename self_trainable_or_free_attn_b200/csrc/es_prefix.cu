@@ -527,20 +527,18 @@ __global__ void __launch_bounds__(256) join_kernel(T* o, float* lse, const __gri
         }
         // NaN, or +infinity, makes the row NaN; -infinity is a part without a key: what it holds is not read
         const float w = z == -INFINITY ? 0.f : z != z ? z : ex2_approx(z - top);
+        float all = w;
+        for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+        sum += all;
         const int n = min(32, parts - p0);
 #pragma unroll 4
         for (int p = 0; p < n; ++p) {
             const float wp = __shfl_sync(0xffffffffu, w, p);
             const float* sp = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), p));
-            if (__shfl_sync(0xffffffffu, z, p) == -INFINITY) continue;
-            sum += wp;
-            if constexpr (C == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(sp + C * lane);
-                acc[0] += v.x * wp; acc[1] += v.y * wp; acc[2] += v.z * wp; acc[3] += v.w * wp;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(sp + C * lane);
-                acc[0] += v.x * wp; acc[1] += v.y * wp;
-            }
+            float v[C];
+            load_floats<C>(sp + C * lane, v);
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] += wp == 0.f ? 0.f : v[c] * wp;
         }
     }
     // a wait gave up, here or earlier: parts are missing
