@@ -18,7 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as N
-from .packed import _DTYPES, _call, check_heads, check_ints, check_tokens, rows, softmax_scale, strides, usable
+from .packed import _DTYPES, _call, _workspace, check_heads, check_ints, check_tokens, rows, softmax_scale, strides, usable
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -60,17 +60,15 @@ def extend_tables(lengths, new_tokens, table, free_pages, page_size, *, total):
     return plan
 
 
-def _check_cache(ref, k_cache, v_cache):
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dim() != 4:
-            raise RuntimeError(f"{name} must be [pages, page_size, kv_heads, D], got {tuple(t.shape)}")
-        if not usable(t):
-            raise RuntimeError(f"{name}: the rows of a cache must be contiguous and start on 16 bytes")
-    if k_cache.shape != v_cache.shape:
-        raise RuntimeError("k_cache and v_cache must have one shape")
-    if k_cache.shape[0] * k_cache.shape[1] >= 2 ** 31:
+def _check_cache(k_cache, v_cache):
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise RuntimeError(f"k_cache and v_cache must be [pages, page_size, kv_heads, D], got {tuple(shape)}, {tuple(v_cache.shape)}")
+    if not (usable(k_cache) and usable(v_cache)):
+        raise RuntimeError("the rows of a cache must be contiguous and start on 16 bytes")
+    if shape[0] * shape[1] >= 2 ** 31:
         raise RuntimeError("a cache holds fewer than 2**31 tokens")
-    return k_cache.shape
+    return shape
 
 
 @N.device_guard
@@ -78,7 +76,7 @@ def store_kv(k, v, k_cache, v_cache, slots):
     """Writes k, v [tokens, kv_heads, D] into the cache: token t at slots[t] (page * page_size + offset). Tokens whose slot is
     -1, or lies outside the cache, are skipped. The slots of a call are distinct: of two tokens with one slot either may be stored."""
     check_tokens(k, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
-    P, S, Hk, D = _check_cache(k, k_cache, v_cache)
+    P, S, Hk, D = _check_cache(k_cache, v_cache)
     if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (Hk, D):
         raise RuntimeError("k and v must be [tokens, kv_heads, D] with the heads of the cache")
     check_heads(Hk, Hk, D)
@@ -104,7 +102,7 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
     if q.requires_grad or k_cache.requires_grad or v_cache.requires_grad:
         if torch.is_grad_enabled():
             raise RuntimeError("prefix_attention has no backward: call it under torch.no_grad()")
-    P, S, Hk, D = _check_cache(q, k_cache, v_cache)
+    P, S, Hk, D = _check_cache(k_cache, v_cache)
     if q.dim() != 4 or q.shape[3] != D:
         raise RuntimeError("q must be [batch, tokens, heads, D] with the head dim of the cache")
     if S not in PAGE_SIZES:
@@ -122,8 +120,7 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
     q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
     o = torch.empty(B, T, H, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, H, T, device=q.device, dtype=torch.float32)
-    n = int(N.load().es_prefix_workspace_bytes(B, T, H, Hk, D, prefix_len, table.shape[1], S))
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    ws = _workspace("es_prefix_workspace_bytes", q, (B, T, H, Hk, D, prefix_len, table.shape[1], S))
     _call("es_prefix_attn", N.ptr(q), N.ptr(k_cache), N.ptr(v_cache), N.ptr(o), N.ptr(lse), N.ptr(prefix_pages), prefix_pages.numel(), prefix_len,
           N.ptr(table), table.shape[1], N.ptr(lengths), B, T, H, Hk, D, P, S, *strides(k_cache), *strides(v_cache), softmax_scale(scale, D),
           _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())

@@ -13,6 +13,7 @@ per gradient row: reproducible bit for bit).
 Tokens of no sequence (behind the last, say) get output 0, LSE -inf and gradient 0, and what they hold reaches no other row; the same
 is true of keys that the causal mask hides.
 """
+import functools
 import math
 
 import torch
@@ -26,21 +27,25 @@ DIMS = (64, 128)
 
 def usable(t):
     """Whether the kernels' 16-byte loads can take t [..., D] as it lies: its rows in one piece, no two rows the same memory."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or (s % 8 == 0 and t.shape[-1] <= s < 2 ** 39) for n, s in zip(t.shape[:-1], t.stride()[:-1])))
-
-
-def _plain(t):
-    return t.is_contiguous() and t.data_ptr() % 16 == 0
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous() and t.shape[-1] % 8 == 0:
+        return True
+    return t.stride(-1) == 1 and all(n == 1 or (s % 8 == 0 and t.shape[-1] <= s < 2 ** 39) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
 
 
 def rows(t):
     """t itself where the kernels can read it, else a copy."""
-    return t if _plain(t) or usable(t) else t.clone(memory_format=torch.contiguous_format)
+    return t if usable(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def strides(t):
     """Element strides of all but the last dimension; those of dimensions of one entry, which nothing uses, as if contiguous."""
+    if t.is_contiguous():
+        shape = t.shape
+        if len(shape) == 3:
+            return shape[1] * shape[2], shape[2]
+        return shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]
     whole, out = t.shape[-1], []
     for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         out.append(s if n > 1 else whole)
@@ -66,20 +71,21 @@ def check_heads(q_heads, kv_heads, D):
 
 def check_tokens(ref, **tensors):
     """Every tensor on the CUDA device of `ref` and in its dtype, bf16 or fp16."""
+    dev, dtype = ref.get_device(), ref.dtype
     for name, t in tensors.items():
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor: this operator has no CPU path")
-        if t.device != ref.device:
+        if t.get_device() != dev:
             raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
-        if t.dtype not in _DTYPES or t.dtype != ref.dtype:
+        if t.dtype is not dtype or dtype not in _DTYPES:
             raise RuntimeError("all of them must share the dtype bfloat16 or float16: " + ", ".join(tensors))
 
 
 def check_ints(ref, **tensors):
     """Device tensors of whole numbers as int32, contiguous."""
-    out = []
+    out, dev = [], ref.get_device()
     for name, t in tensors.items():
-        if t.device != ref.device:
+        if t.get_device() != dev:
             raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
         if t.dtype is not torch.int32 or not t.is_contiguous():
             if t.dtype not in (torch.int32, torch.int64):
@@ -95,20 +101,28 @@ def _call(name, *args):
         N.check(rc, name)
 
 
+@functools.lru_cache(maxsize=4096)
+def _bytes(name, device, sizes):
+    """Bytes of scratch, which follow from the sizes (and from the device's number of SMs)."""
+    return int(getattr(N.load(), name)(*sizes))
+
+
 def _workspace(name, q, sizes):
-    n = getattr(N.load(), name)(*sizes)
+    n = _bytes(name, q.get_device(), sizes)
     return torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
 
 
 def _fwd(q, k, v, cu_q, cu_k, scale, causal, with_rest):
     T, H, D = q.shape
-    o = torch.empty(T, H, D, device=q.device, dtype=q.dtype)
-    rest = torch.empty_like(o) if with_rest else None
-    lse = torch.empty(H, T, device=q.device, dtype=torch.float32)
-    sizes = (cu_q.numel() - 1, T, k.shape[0], H, k.shape[1], D)
+    Tk, Hk, _ = k.shape
+    device, dtype = q.device, q.dtype
+    o = torch.empty(T, H, D, device=device, dtype=dtype)
+    rest = torch.empty(T, H, D, device=device, dtype=dtype) if with_rest else None
+    lse = torch.empty(H, T, device=device, dtype=torch.float32)
+    sizes = (cu_q.shape[0] - 1, T, Tk, H, Hk, D)
     ws = _workspace("es_packed_fwd_workspace_bytes", q, sizes)
     _call("es_packed_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), N.ptr(rest), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), *sizes,
-          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
+          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[dtype], N.ptr(ws), N.stream_ptr())
     return o, rest, lse
 
 
@@ -130,7 +144,7 @@ class _Function(torch.autograd.Function):
             return (None,) * 7
         q, k, v, o, rest, lse, cu_q, cu_k = ctx.saved_tensors
         dout = rows(dout)
-        sizes = (cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        sizes = (cu_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
         need = ctx.needs_input_grad
         mk = lambda t: torch.empty(t.shape, device=t.device, dtype=t.dtype)
         dq = mk(q) if need[0] else None
@@ -150,28 +164,28 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, retur
     `causal`: query i of nq sees the keys j <= i + nk - nq of its sequence's nk (the last query sees all); a row that sees none is 0 with
     LSE -inf. `scale`: factor of q k^T, 1 / sqrt(D) by default. cu_q, cu_k are read on the GPU only: nothing synchronises, and a
     captured call follows them when they change."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise RuntimeError(f"{name} must be [tokens, heads, D], got {tuple(t.shape)}")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise RuntimeError(f"q, k, v must be [tokens, heads, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     check_tokens(q, q=q, k=k, v=v)
-    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+    T, H, D = q.shape
+    Tk, Hk, Dk = k.shape
+    if k.shape != v.shape or Dk != D:
         raise RuntimeError("k and v must have one shape, and the head dim of q")
-    check_heads(q.shape[1], k.shape[1], q.shape[2])
+    check_heads(H, Hk, D)
     if cu_k is None:
-        if k.shape[0] != q.shape[0]:
-            raise RuntimeError(f"without cu_k there are as many keys as queries, got {k.shape[0]} and {q.shape[0]}")
+        if Tk != T:
+            raise RuntimeError(f"without cu_k there are as many keys as queries, got {Tk} and {T}")
         cu_q, = check_ints(q, cu_q=cu_q)
         cu_k = cu_q
     else:
         cu_q, cu_k = check_ints(q, cu_q=cu_q, cu_k=cu_k)
-    if cu_q.dim() != 1 or cu_q.numel() < 1 or cu_k.shape != cu_q.shape:
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1 or cu_k.shape != cu_q.shape:
         raise RuntimeError("cu_q and cu_k must be [batch + 1]")
-    if max(q.shape[0], k.shape[0]) >= 2 ** 31 - 256:
+    if max(T, Tk) >= 2 ** 31 - 256:
         raise RuntimeError("at most 2**31 - 257 tokens")
-    scale = softmax_scale(scale, q.shape[2])
-    args = (rows(q), rows(k), rows(v), cu_q, cu_k, scale, int(bool(causal)))
+    scale, causal = softmax_scale(scale, D), 1 if causal else 0
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _Function.apply(*args)
+        o, lse = _Function.apply(rows(q), rows(k), rows(v), cu_q, cu_k, scale, causal)
     else:
-        o, _, lse = _fwd(*args, False)
+        o, _, lse = _fwd(rows(q), rows(k), rows(v), cu_q, cu_k, scale, causal, False)
     return (o, lse) if return_lse else o
