@@ -97,7 +97,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wide = a.b.Hk * a.splits, kh = blockIdx.x % wide % a.b.Hk, split = blockIdx.x % wide / a.b.Hk;
     // (the first keys of a causal sequence are seen by the most queries)
-    const Piece at = find_piece(a.b.cu_k, a.b.B, a.b.Tk, blockIdx.x / wide, TN, lane);
+    const Piece at = find_piece<false>(a.b.cu_k, a.b.B, a.b.Tk, gridDim.x / wide, blockIdx.x / wide, TN, lane);
     if (at.n <= 0) return;
     int q0 = 0, nq = 0, diag = 0, first = 0;                 // diag: query t sees the owner's keys 0 .. t + diag
     if (at.seq >= 0) {
@@ -425,7 +425,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int vheads = a.b.H / a.pack, vh = blockIdx.x % vheads, head0 = vh * a.pack, kh = head0 / a.b.G;
-    const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / vheads - 1 - blockIdx.x / vheads, a.tokens, lane);
+    const Piece at = find_piece<true>(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / vheads, blockIdx.x / vheads, a.tokens, lane);
     if (at.n <= 0) return;
     int k0 = 0, nk = 0, diag = 0;                            // token t of the span sees keys 0 .. t + diag
     if (at.seq >= 0) {

@@ -84,7 +84,7 @@ template <bool PAGED> __device__ __forceinline__ Work work_of(const FwdArgs& a, 
         w.n_tok = min(span, a.b.Tq - w.q0);
         w.nk = a.nk;
     } else {
-        const Piece at = find_piece(a.b.cu_q, a.b.B, a.b.Tq, (int)(a.slots - 1 - x), span, lane);
+        const Piece at = find_piece<true>(a.b.cu_q, a.b.B, a.b.Tq, a.slots, x, span, lane);
         w.q0 = at.first;
         w.n_tok = at.n;
         if (at.n > 0 && at.seq >= 0) {

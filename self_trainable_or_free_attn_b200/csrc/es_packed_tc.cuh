@@ -24,24 +24,46 @@ struct Piece {
     int first, n;        // first token of the batch, tokens (none where n <= 0)
 };
 
-// The span of grid slot x: pieces of the batch are what lies before the first sequence, the sequences, and what lies behind the last; piece
-// i starts at slot floor(start / span) + i, which leaves each piece at least ceil(length / span) slots without a sum over the lengths.
-// The slots are 0 .. floor(tokens / span) + B + 1. A warp searches 32 pieces at a time.
-__device__ __forceinline__ Piece find_piece(const int* cu, int B, int tokens, int x, int span, int lane) {
-    auto start = [&](int i) { return i == 0 ? 0 : min(max(__ldg(cu + i - 1), 0), tokens); };
+// The span of grid slot x. The pieces of a batch are what lies before the first sequence, the sequences, and what lies behind the last. Up to 32 of
+// them, a lane each, are taken longest first, so that the last slots are short ones, each from its last span to its first (LAST_FIRST) or from its
+// first. (24 ragged prompts x 40 heads: the slowest SM 14 % over the mean in the order of the batch.) More of them stay in their order: piece i
+// starts at slot floor(start / span) + i, which leaves each piece at least ceil(length / span) slots without a sum over the lengths, and a
+// warp searches 32 pieces at a time. The slots are 0 .. floor(tokens / span) + B + 1.
+template <bool LAST_FIRST> __device__ __forceinline__ Piece find_piece(const int* cu, int B, int tokens, int64_t slots, int64_t x, int span, int lane) {
+    auto start = [&](int i) { return i == 0 ? 0 : i > B + 1 ? tokens : min(max(__ldg(cu + i - 1), 0), tokens); };
+    Piece p;
+    if (B + 2 <= 32) {
+        const int s = lane < B + 2 ? start(lane) : tokens, e = lane < B + 2 ? start(lane + 1) : tokens;
+        const int length = max(e - s, 0), mine = (length + span - 1) / span;
+        int before = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int l = __shfl_sync(0xffffffffu, length, i), n = __shfl_sync(0xffffffffu, mine, i);
+            if (l > length || (l == length && i < lane)) before += n;
+        }
+        const uint32_t found = __ballot_sync(0xffffffffu, x >= before && x < before + mine);
+        if (found == 0) return Piece{-1, 0, 0, 0, 0};
+        const int i = __ffs(found) - 1, at = (int)x - __shfl_sync(0xffffffffu, before, i), n = __shfl_sync(0xffffffffu, mine, i);
+        p.seq = i >= 1 && i <= B ? i - 1 : -1;
+        p.length = __shfl_sync(0xffffffffu, length, i);
+        p.offset = (LAST_FIRST ? n - 1 - at : at) * span;
+        p.first = __shfl_sync(0xffffffffu, s, i) + p.offset;
+        p.n = min(span, p.length - p.offset);
+        return p;
+    }
+    const int y = (int)(LAST_FIRST ? slots - 1 - x : x);
     int lo = 0, n = B + 2;
     while (n > 1) {
         const int step = (n + 31) >> 5, i = lo + lane * step;
-        const bool before = lane * step < n && start(i) / span + i <= x;
+        const bool before = lane * step < n && start(i) / span + i <= y;
         const int c = max(__popc(__ballot_sync(0xffffffffu, before)), 1) - 1;
         n = min(step, n - c * step);
         lo += c * step;
     }
-    const int s = start(lo), e = lo + 1 < B + 2 ? start(lo + 1) : tokens;
-    Piece p;
+    const int s = start(lo), e = start(lo + 1);
     p.seq = lo >= 1 && lo <= B ? lo - 1 : -1;
     p.length = e - s;
-    p.offset = (x - (s / span + lo)) * span;
+    p.offset = (y - (s / span + lo)) * span;
     p.first = s + p.offset;
     p.n = min(span, e - s - p.offset);
     return p;
