@@ -107,7 +107,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         first = min(max(-diag, 0), nq);                      // the first query that sees one of them
     }
     const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens;
-    const int tile0 = (int)((int64_t)subs * per * split / a.splits), nt = (int)((int64_t)subs * per * (split + 1) / a.splits) - tile0;
+    const int tile0 = (int)((int64_t)subs * per * split / a.splits), nt = uniform((int)((int64_t)subs * per * (split + 1) / a.splits) - tile0);
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -151,7 +151,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then minus delta
     float* row_delta = row_lse + C::NROW * TM;
@@ -434,7 +434,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         diag = nk - at.length + at.offset;
     }
     auto seen_by = [&](int t) { return a.b.causal ? min(max(t + diag + 1, 0), nk) : nk; };
-    const int nt = (seen_by(at.n - 1) + TN - 1) / TN, whole = seen_by(0) / TN;
+    const int nt = uniform((seen_by(at.n - 1) + TN - 1) / TN), whole = seen_by(0) / TN;
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -462,7 +462,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     uint32_t issued = 0;
 

@@ -169,7 +169,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     bool ok = *abort_flag == 0;
     // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
@@ -305,6 +305,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             Work w;
             for (int n = 0; enter(n, w); ++n) {
                 leave(n);
+                w.i0 = uniform(w.i0);
+                w.end0 = uniform(w.end0);
+                w.end1 = uniform(w.end1);
                 const int nt = w.last() - w.i0;
                 if (nt <= 0) continue;
                 take(first);

@@ -17,6 +17,10 @@ constexpr int TM = 128, TN = 128, THREADS = 384;
 constexpr int REGS_MATH = 224, REGS_REST = 56;
 constexpr uint32_t HALF = TM * 128;                          // 128 rows x 64 d, one swizzled box
 
+// A value that all lanes have, said so: what is computed from it stays in the registers of the whole warp, where the MMA instructions want their
+// operands. (From values of the lanes' registers an MMA takes 55 to 70 clocks to issue, as long as it runs.)
+template <typename V> __device__ __forceinline__ V uniform(V x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // A span of consecutive tokens of one sequence (or of the tokens before the first or behind the last: seq = -1).
 struct Piece {
     int seq, length;     // the sequence and its tokens
