@@ -108,6 +108,9 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens;
     const int tile0 = (int)((int64_t)subs * per * split / a.splits), nt = uniform((int)((int64_t)subs * per * (split + 1) / a.splits) - tile0);
+    // Rows that see one key: their P is 1 whatever the logit, and dS is 0 and not what rounding leaves of a difference (where it is a number). They
+    // are the first columns of the first walked tile in causal attention, all rows (more than TM) where the sequence has one key.
+    const int ones = at.length == 1 ? TM + 1 : a.b.causal && at.offset == 0 && nq >= at.length ? a.pack : 0;
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
@@ -325,6 +328,11 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&ctl->pfull));
+            if (ones && (ones > TM || t0 == first)) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                    if (j < ones - 64 * ch && fabsf(__uint_as_float(x[j])) < INFINITY) x[j] = 0;
+            }
             ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 631);
             if (!ok) break;
             tc_fence_after();
@@ -601,7 +609,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     float2 g = __fmul2_rn(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
                                           __fadd2_rn(make_float2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])), nd));
                     if (decltype(cut_tile)::value) {
-                        if (2 * j >= lim) g.x = 0.f;
+                        // (a row that sees one key: P is 1 whatever the logit, and dS is 0 and not what rounding leaves; NaN stays)
+                        if (2 * j >= lim || (vis == 1 && g.x == g.x)) g.x = 0.f;
                         if (2 * j + 1 >= lim) g.y = 0.f;
                     }
                     ds[j] = pack2<T>(g.x, g.y);

@@ -209,6 +209,22 @@ def test_gradients_against_differences():
         assert abs((got["d" + n].double().cpu() * d).sum() - slope) <= bound + 1e-7 * (1 + abs(slope))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D,H,Hk", [(128, 24, 4), (64, 5, 1), (64, 2, 2)])
+def test_rows_that_see_one_key(D, H, Hk, causal):
+    """Their P is 1 whatever the logit: dQ, and what they add to dK, is 0 exactly, and not what rounding leaves of a difference."""
+    q, k, v, do, cu, _ = make([1] * 40, [1] * 40, H, Hk, D, BF)
+    got = _run(q, k, v, do, cu, None, causal)
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+    q, k, v, do, cu_q, cu_k = make([5, 1, 3, 200], [1, 1, 3, 150], H, Hk, D, BF)
+    got = _run(q, k, v, do, cu_q, cu_k, causal)
+    first = [4, 5, 6, 9 + 50] if causal else [0, 1, 2, 3, 4, 5]
+    assert (got["dq"][first] == 0).all() and (got["dk"][:2] == 0).all() and (got["dq"][-1] != 0).any()
+    want = reference(q, k, v, cu_q, cu_k, causal, D ** -0.5, do)
+    for n in want:
+        close(n, got[n], want[n])
+
+
 def test_same_bits_twice_and_partial_gradients():
     from self_trainable_or_free_attn_b200 import packed
     q, k, v, do, cu, _ = make([300, 77, 140], [300, 77, 140], 6, 2, 128, BF)
