@@ -52,7 +52,7 @@ static_assert(sizeof(Ctl) <= 768, "control block");
 
 struct FwdArgs {
     Batch b;
-    int64_t slots;                                           // row tile pairs, some of them empty
+    int64_t slots;                                           // row tile pairs, some of them empty (paged: tiles, with heads and splits)
     int pack, tokens, splits;                                // heads per row group, tokens per 128 rows, CTAs that share a tile's keys
     int vheads;                                              // kv_heads * (G / pack)
     void* o;
@@ -197,7 +197,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     if (lane == 0 && w.n_tok > 0) ctl->held = w;
                 }
                 if (!ok) break;
-                if (t >= 0 && lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
+                if (!PAGED && t >= 0 && lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
                 if (t < 0 || w.n_tok > 0) {
                     ok = mbar_wait_warp(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, abort_flag, a.status, 611);
                     if (ok && lane == 0) {
@@ -208,6 +208,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     ++n;
                     __syncwarp();
                     if (t < 0) break;
+                }
+                if (PAGED) {
+                    // all tiles are alike: every SM has as many, one more at most (taken as CTAs came, some runs had one that did another, 585 us
+                    // instead of 500). After a wait that gave up the join writes NaN whatever the parts hold
+                    t = t + gridDim.x < a.slots ? t + gridDim.x : -1;
+                    if (!ok) break;
+                    continue;
                 }
                 // (also where a wait gave up: what the answer takes from the grid nobody else will do)
                 const bool there = mbar_wait_warp(smem_u32(&ctl->next), asked & 1, abort_flag, a.status, 612) ||
@@ -439,16 +446,16 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 const float2 cc = make_float2(c, c), oo = make_float2(off, off);
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), cc, oo);
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[32 * h + 2 * j]), __uint_as_float(x[32 * h + 2 * j + 1])), cc, oo);
                         const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
                         sum = __fadd2_rn(sum, e);
                         p[j] = pack2<T>(e.x, e.y);
                     }
-                    tmem_st32(scol + 32 * h, p);
+                    tmem_st16(scol + 16 * h, p);
                 }
                 l += sum.x + sum.y;
                 if (i >= whole) {
@@ -676,13 +683,13 @@ int packed_fwd_tc(const void* q, Rows rq, const void* k, Rows rk, const void* v,
 // The part of a batch's new tokens that sees a prefix in pages: `parts` fp32 partial results and log2-domain LSEs, [part][token][head]. The caller has
 // checked sizes and pointers.
 template <typename T, int D>
-static int launch_prefix(const void* q, const void* k, CacheRows rk, const void* v, CacheRows rv, const FwdArgs& a, cudaStream_t st) {
+static int launch_prefix(const void* q, const void* k, CacheRows rk, const void* v, CacheRows rv, FwdArgs a, cudaStream_t st) {
     CUtensorMap tq, tk, tv;
     if (int rc = make_rows_map<T>(&tq, q, D, a.b.H, a.b.Tq, {(int64_t)a.b.H * D, D}, a.pack, a.tokens)) return rc;
     if (int rc = make_pages_map<T>(&tk, k, D, a.b.Hk, 1 << a.log_page, a.pages, rk, TN)) return rc;
     if (int rc = make_pages_map<T>(&tv, v, D, a.b.Hk, 1 << a.log_page, a.pages, rv, TN)) return rc;
-    const int64_t grid = (int64_t)a.vheads * a.splits * ((a.b.Tq + 2 * a.tokens - 1) / (2 * a.tokens));
-    if (grid > 0x7FFFFFFF) return set_error(-1, "es_prefix_attn: too many tiles");
+    a.slots = (int64_t)a.vheads * a.splits * ((a.b.Tq + 2 * a.tokens - 1) / (2 * a.tokens));
+    const int64_t grid = std::min<int64_t>(a.slots, sm_count());
     auto kern = packed_fwd_kernel<T, D, true>;
     if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
