@@ -18,6 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as N
+from ._native import check_status  # noqa: F401
 from .packed import _DTYPES, _call, _workspace, check_heads, check_ints, check_tokens, rows, softmax_scale, strides, usable
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -115,8 +116,8 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
     prefix_len = int(prefix_len)
     if not 0 <= prefix_len <= prefix_pages.numel() * S:
         raise ValueError(f"prefix_len = {prefix_len}: the {prefix_pages.numel()} prefix pages hold 0 to {prefix_pages.numel() * S} tokens")
-    if table.shape[1] * S >= 2 ** 31 or B * T * H >= 2 ** 31:
-        raise RuntimeError("fewer than 2**31 tokens to a row of table, and query rows")
+    if table.shape[1] * S > 2 ** 31 - 256 or B * T * H >= 2 ** 31:
+        raise RuntimeError("at most 2**31 - 256 tokens to a row of table, and fewer than 2**31 query rows")
     q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
     o = torch.empty(B, T, H, D, device=q.device, dtype=q.dtype)
     lse = torch.empty(B, H, T, device=q.device, dtype=torch.float32)

@@ -287,7 +287,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_wait_ld_regs(x);
             tmem_wait_ld_regs(x + 32);
             const int lim = cut ? max(r - diag - t0, 0) * a.pack - 64 * ch : 0;      // columns before it do not see the key
-            const int end = min(loaded, (nq - t0) * a.pack) - 64 * ch;               // columns from here on are not rows of the sequence
+            const int end = min(nq - t0, a.tokens) * a.pack - 64 * ch;               // columns from here on are not rows of the sequence
             const float4* rl = reinterpret_cast<const float4*>(row_lse + (i % C::NROW) * TM + 64 * ch);
             // P; one pair in four on the FMA pipes, as many as take no longer than the others take the 16 exponentials a clock of an SM
             auto probabilities = [&](auto cut_tile) {

@@ -46,7 +46,7 @@ struct Ctl {
     alignas(16) uint32_t answer[4];
     uint32_t tmem_base;
     int abort, not_finite[2];
-    Work work[2], held;  // held: taken, but not handed on before a wait gave up
+    Work work[2], held[2];       // held: taken, but not handed on before a wait gave up; the answer that came after it
 };
 static_assert(sizeof(Ctl) <= 768, "control block");
 
@@ -156,7 +156,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         mbar_init(smem_u32(&ctl->drain), 1);
         mbar_init(smem_u32(&ctl->next), 1);
-        ctl->held.n_tok = 0;
+        ctl->held[0].n_tok = ctl->held[1].n_tok = 0;
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 910);
         mbar_fence_init();
@@ -194,7 +194,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 Work w{};
                 if (t >= 0) {
                     w = work_of<PAGED>(a, t, lane);
-                    if (lane == 0 && w.n_tok > 0) ctl->held = w;
+                    if (lane == 0) ctl->held[0] = w;
                 }
                 if (!ok) break;
                 if (!PAGED && t >= 0 && lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
@@ -226,7 +226,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (!ok) {
                     if (t >= 0) {
                         w = work_of<PAGED>(a, t, lane);
-                        if (lane == 0 && w.n_tok > 0) ctl->held = w;
+                        if (lane == 0) ctl->held[1] = w;
                     }
                     break;
                 }
@@ -560,8 +560,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (*abort_flag) {
         // NaN in the tiles that the CTA had taken and may not have finished: the caller's memory is not initialised
-        for (int x = 0; x < 3; ++x) {
-            const Work w = x == 2 ? ctl->held : ctl->work[x];
+        for (int x = 0; x < 4; ++x) {
+            const Work w = x < 2 ? ctl->work[x] : ctl->held[x - 2];
             for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
                 const int head = w.vh * a.pack + e % a.pack;
                 const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head;

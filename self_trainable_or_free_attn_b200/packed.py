@@ -20,6 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
+from ._native import check_status  # noqa: F401
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 DIMS = (64, 128)

@@ -283,6 +283,45 @@ def test_same_bits_twice_on_another_stream_and_captured():
         assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
 
 
+def test_cache_past_32_bits():
+    """Caches of more than 2^31 elements, the pages in use at their end: stored, and attended to by both kernels of the prefix."""
+    from self_trainable_or_free_attn_b200 import cache
+    P, S, Hk, D = 2 ** 31 // (64 * 4 * 128) + 60, 64, 4, 128
+    kc, vc = (torch.zeros(P, S, Hk, D, dtype=BF, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(1)
+    n = 300
+    k, v = (torch.randn(n, Hk, D, generator=g).to(BF).cuda() for _ in range(2))
+    pages = [P - 1, P - 9, P - 3, P - 30, P - 5]
+    slots = ints([pages[j // S] * S + j % S for j in range(n)])
+    cache.store_kv(k, v, kc, vc, slots)
+    assert torch.equal(kc[pages[1], 7], k[S + 7]) and torch.equal(vc[pages[4], 2], v[4 * S + 2])
+    small = [torch.zeros(5, S, Hk, D, dtype=BF, device="cuda") for _ in range(2)]
+    cache.store_kv(k, v, *small, ints(range(n)))
+    for B in (2, 40):
+        q = torch.randn(B, 1, 8, D, generator=g).to(BF).cuda()
+        own = ints([40 + b for b in range(B)])
+        far = cache.prefix_attention(q, kc, vc, ints(pages[:4]), 250, ints([[pages[4], pages[0]]] * B), own)
+        near = cache.prefix_attention(q, *small, ints([0, 1, 2, 3]), 250, ints([[4, 0]] * B), own)
+        assert torch.equal(far, near) and far.any()
+
+
+def test_outputs_are_nan_until_the_status_word_is_read():
+    """As tests/test_gpu_packed.py: with the prefix in own_kernel and on the tcgen05 kernel."""
+    from self_trainable_or_free_attn_b200 import _native as N, cache
+    cache.check_status()
+    for B in (2, 70):
+        own = [40] * B
+        q, kc, vc, pages, table = _prefix_case(B, 1, 4, 2, 64, 16, 300, own, BF)
+        run = lambda: cache.prefix_attention(q, kc, vc, ints(pages), 300, ints(table), ints(own), return_lse=True)
+        good = run()
+        N.check(N.load().es_selftest_wait_timeout(2000, N.stream_ptr()), "selftest")
+        assert all(torch.isnan(t).all() for t in run())
+        with pytest.raises(N.NativeError, match="status 777"):
+            cache.check_status()
+        assert all(torch.equal(a, b) for a, b in zip(good, run()))
+    cache.check_status()
+
+
 # ---------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("N", [1, 3])
 def test_prompts_then_tokens(N):

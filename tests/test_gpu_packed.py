@@ -133,6 +133,85 @@ def test_what_is_not_finite_stays_where_it_is_seen(which, value, D, causal):
             assert torch.equal(got[n_][:, h].cpu()[~hit], clean[n_][:, h].cpu()[~hit])
 
 
+@pytest.mark.parametrize("which", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_what_is_not_finite_where_the_keys_are_shared_out(which, causal):
+    """The same with so few tiles that several CTAs share a tile's keys, and several the rows that walk a key tile: parts that are added up."""
+    for n_q, n_k, at_q, at_k in (([40, 30], [5000, 3000], 20, 4970), ([1500], [1500], 700, 700)):
+        q, k, v, do, cu_q, cu_k = make(n_q, n_k, 8, 1, 128, BF, seed=4)
+        clean = _run(q, k, v, do, cu_q, cu_k, causal)
+        x = dict(q=q, k=k, v=v, do=do)
+        x[which][at_q if which in ("q", "do") else at_k, 0, 3] = float("nan")
+        got = _run(q, k, v, do, cu_q, cu_k, causal)
+        off = n_k[0] - n_q[0]
+        rows, keys = torch.zeros(cu_q[-1], dtype=torch.bool), torch.zeros(cu_k[-1], dtype=torch.bool)
+        if which in ("q", "do"):
+            rows[at_q] = True
+            keys[:at_q + off + 1 if causal else n_k[0]] = True
+        else:
+            rows[max(0, at_k - off) if causal else 0:n_q[0]] = True
+            keys[:n_k[0]] = True
+        heads = range(1) if which in ("q", "do") else range(8)
+        for h in range(8):
+            hit = rows if h in heads else rows & False
+            for name in ("o", "dq")[which == "do":]:
+                assert torch.equal(_bad(got[name][:, h]).any(1), hit), name
+                assert torch.equal(got[name][:, h].cpu()[~hit], clean[name][:, h].cpu()[~hit])
+        for name in ("dk", "dv")[:1 if which == "v" else 2]:
+            assert torch.equal(_bad(got[name][:, 0]).any(1), keys), name
+            assert torch.equal(got[name][:, 0].cpu()[~keys], clean[name][:, 0].cpu()[~keys])
+
+
+@pytest.mark.parametrize("B", [29, 30, 31, 70, 1100])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(B, causal):
+    """Up to 30 sequences are taken longest first, more in their order; empty ones among them."""
+    g = torch.Generator().manual_seed(B)
+    n = torch.randint(0, 40, (B,), generator=g).tolist()
+    n[3], n[B // 2], n[-1] = 300, 0, 0
+    _check(n, n, 4, 2, 64, BF, causal, seed=B, first=5, behind=9)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last sequences against the definition."""
+    T, H, D = 2 ** 31 // (64 * 64) + 300, 64, 64
+    g = torch.Generator().manual_seed(0)
+    tail = [torch.randn(190, H, D, generator=g).to(BF).cuda() for _ in range(4)]
+    big = [torch.zeros(T, H, D, dtype=BF, device="cuda") for _ in range(4)]
+    for t, x in zip(big, tail):
+        t[-190:] = x
+    from self_trainable_or_free_attn_b200 import packed
+    do = big.pop()
+    leaves = [t.requires_grad_(True) for t in big]
+    o, lse = packed.packed_attention(*leaves, ints([T - 190, T - 100, T]), return_lse=True)
+    grads = torch.autograd.grad(o, leaves, do)
+    want = reference(*tail[:3], [0, 90, 190], [0, 90, 190], True, 0.125, tail[3])
+    close("o", o[-190:], want["o"])
+    close("lse", lse[:, -190:], want["lse"])
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        close(name, got[-190:], want[name])
+        assert not got[:-190].any()
+    assert not o[:-190].any()
+
+
+def test_outputs_are_nan_until_the_status_word_is_read():
+    """A kernel that starts while the status word is set (a wait of an earlier one gave up; here the library's self test, a barrier nobody
+    arrives on, for 2 ms) leaves NaN in all it owns; check_status raises and clears the word."""
+    from self_trainable_or_free_attn_b200 import _native as N, packed
+    packed.check_status()
+    for n_q, n_k, Hk in (([300, 0, 77], [300, 0, 77], 4), ([20], [3000], 1), ([1500], [1500], 1)):
+        q, k, v, do, cu_q, cu_k = make(n_q, n_k, 4, Hk, 128, BF, behind=3)
+        good = _run(q, k, v, do, cu_q, cu_k, True)
+        N.check(N.load().es_selftest_wait_timeout(2000, N.stream_ptr()), "selftest")
+        bad = _run(q, k, v, do, cu_q, cu_k, True)
+        assert all(torch.isnan(bad[n]).all() for n in bad)
+        with pytest.raises(N.NativeError, match="status 777"):
+            packed.check_status()
+        again = _run(q, k, v, do, cu_q, cu_k, True)
+        assert all(torch.equal(good[n], again[n]) for n in good)
+    packed.check_status()
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_strides(D):
     """Thirds of a fused projection, head-major tensors, broadcast heads, rows off 16 bytes, and an output gradient of one value."""
