@@ -196,20 +196,43 @@ def test_prefix_layouts(layout):
     _prefix_check(3, 2, 6, 2, 128, 32, 100, [5, 40, 70], BF, layout=layout)
 
 
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_what_is_not_finite_among_the_newest_tokens(which):
+    """Three queries each: the second's key or value is NaN; the first must not see it."""
+    from self_trainable_or_free_attn_b200 import cache
+    own = [40, 66, 3]
+    q, kc, vc, pages, table = _prefix_case(3, 3, 4, 2, 64, 16, 50, own, BF)
+    args = (ints(pages), 50, ints(table), ints(own))
+    clean = cache.prefix_attention(q, kc, vc, *args)
+    bad = torch.zeros(3, 3, 4, dtype=torch.bool)             # [request, query, head]
+    for b in range(3):
+        if which == "q":
+            q[b, 1, 2] = float("nan")
+            bad[b, 1, 2] = True
+        else:
+            j = own[b] - 2
+            (kc if which == "k" else vc)[table[b][j // 16], j % 16, 1] = float("nan")
+            bad[b, 1:, 2:] = True
+    got = cache.prefix_attention(q, kc, vc, *args)
+    assert torch.equal(~torch.isfinite(got.float()).all(-1).cpu(), bad)
+    assert torch.equal(got.cpu()[~bad], clean.cpu()[~bad])
+
+
 def test_fewer_own_tokens_than_queries():
     """Rows of a padded batch: lengths below the number of queries leave the first queries the prefix alone."""
     _prefix_check(4, 4, 4, 2, 64, 16, 40, [0, 1, 3, 4], BF)
     _prefix_check(4, 4, 4, 2, 64, 16, 0, [0, 1, 3, 4], BF)
 
 
-def test_bad_pages_and_what_lies_behind():
+@pytest.mark.parametrize("B", [3, 70])
+def test_bad_pages_and_what_lies_behind(B):
     """Pages of -1 or beyond the cache are not attended to; lengths beyond the table's row count as the row; NaN in pages of others, and behind the last token
     in a request's own last page, reaches nothing."""
     from self_trainable_or_free_attn_b200 import cache
-    own = [40, 70, 33]
-    q, kc, vc, pages, table = _prefix_case(3, 1, 4, 2, 64, 16, 100, own, BF)
+    own = ([40, 70, 33] * B)[:B]
+    q, kc, vc, pages, table = _prefix_case(B, 1, 4, 2, 64, 16, 100, own, BF)
     used = {(p, j) for i, p in enumerate(pages) for j in range(16) if 16 * i + j < 100}
-    used |= {(table[b][j // 16], j % 16) for b in range(3) for j in range(own[b])}
+    used |= {(table[b][j // 16], j % 16) for b in range(B) for j in range(own[b])}
     for p in range(kc.shape[0]):
         for j in range(16):
             if (p, j) not in used:
@@ -220,30 +243,33 @@ def test_bad_pages_and_what_lies_behind():
     close("o", o, want_o)
     close("lse", lse, want_lse)
     # every page bad, no prefix
-    o, lse = cache.prefix_attention(q, kc, vc, ints([]), 0, ints([[-1] * 6] * 3), ints(own), return_lse=True)
+    o, lse = cache.prefix_attention(q, kc, vc, ints([]), 0, ints([[-1] * 6] * B), ints(own), return_lse=True)
+    assert (o == 0).all() and torch.isinf(lse).all()
+    o, lse = cache.prefix_attention(q, kc, vc, ints([-1] * 9), 140, ints([[-1] * 6] * B), ints(own), return_lse=True)
     assert (o == 0).all() and torch.isinf(lse).all()
     # lengths beyond the row
-    full = cache.prefix_attention(q, kc, vc, ints(pages), 100, ints(table)[:, :2].contiguous(), ints([32, 32, 32]))
-    assert torch.equal(cache.prefix_attention(q, kc, vc, ints(pages), 100, ints(table)[:, :2].contiguous(), ints([99, 2 ** 31 - 1, 32])), full)
+    full = cache.prefix_attention(q, kc, vc, ints(pages), 100, ints(table)[:, :2].contiguous(), ints([32] * B))
+    assert torch.equal(cache.prefix_attention(q, kc, vc, ints(pages), 100, ints(table)[:, :2].contiguous(), ints(([99, 2 ** 31 - 1, 32] * B)[:B])), full)
 
 
-@pytest.mark.parametrize("which", ["q", "k_prefix", "v_prefix", "k_own", "v_own"])
-def test_what_is_not_finite_stays_with_its_request(which):
+@pytest.mark.parametrize("B", [4, 70])
+@pytest.mark.parametrize("which", ["q", "k_prefix", "v_prefix", "v_last", "k_own", "v_own"])
+def test_what_is_not_finite_stays_with_its_request(which, B):
     from self_trainable_or_free_attn_b200 import cache
-    own = [40, 70, 33, 150]
-    q, kc, vc, pages, table = _prefix_case(4, 1, 4, 2, 128, 16, 200, own, BF)
+    own = ([40, 70, 33, 150] * B)[:B]
+    q, kc, vc, pages, table = _prefix_case(B, 1, 4, 2, 128, 16, 200, own, BF)
     args = (ints(pages), 200, ints(table), ints(own))
     clean = cache.prefix_attention(q, kc, vc, *args)
-    bad = torch.zeros(4, 4, dtype=torch.bool)                # [request, head]
+    bad = torch.zeros(B, 4, dtype=torch.bool)                # [request, head]
     if which == "q":
         q[1, 0, 2] = float("nan")
         bad[1, 2] = True
     else:
-        page, at = (pages[5], 3) if which.endswith("prefix") else (table[1][2], 9)
+        page, at = (table[1][2], 9) if which.endswith("own") else (pages[5], 3) if which.endswith("prefix") else (pages[12], 6)
         (kc if which[0] == "k" else vc)[page, at, 1] = float("inf")
         bad[:, 2:] = True
         if which.endswith("own"):
-            bad[[0, 2, 3]] = False
+            bad[torch.arange(B) != 1] = False
     got = cache.prefix_attention(q, kc, vc, *args)
     assert torch.equal(~torch.isfinite(got[:, 0].float()).all(-1).cpu(), bad)
     assert torch.equal(got[:, 0].cpu()[~bad], clean[:, 0].cpu()[~bad])
