@@ -25,15 +25,27 @@ template <int D> struct Cfg {
     static constexpr int NSLOT = D == 128 ? 5 : 10;
     static constexpr uint32_t Y1 = 0, Y2 = TILE, RING = 2 * TILE, ROWS = RING + NSLOT * TILE;
     static constexpr int NROW = 2;                           // stages of LSE and delta
-    static constexpr uint32_t CTL = ROWS + NROW * 2 * TM * 4, BYTES = CTL + 512;
+    static constexpr uint32_t CTL = ROWS + NROW * 2 * TM * 4, BYTES = CTL + 768;
 };
 static_assert(Cfg<128>::BYTES <= 232448, "shared memory");
-struct Ctl {
-    uint64_t yfull, full[10], empty[10], sfull[2], dpfull, pfull, dsfull, rfull[2], rempty[2], gfull, drain;
-    uint32_t tmem_base;
-    int abort, not_finite;
+// What a CTA does next.
+struct Work {
+    int first, n_tok;    // the owner's first token, its tokens; n_tok <= 0: nothing more
+    int w0, nw;          // first token and tokens of the other side of its sequence, which is walked
+    int diag;            // dK / dV: query t sees the owner's keys 0 .. t + diag; dQ: token t of the owner sees keys 0 .. t + diag
+    int nt;              // walked tiles
+    int head, split;     // key head; dQ: first query head
+    int from, per, tile0;        // dK / dV: first query that sees one of the keys, tiles from it to the end, the first of them in this split
+    int ones;            // dK / dV: see below
 };
-static_assert(sizeof(Ctl) <= 512, "control block");
+struct Ctl {
+    uint64_t yfull, yempty, full[10], empty[10], sfull[2], dpfull, pfull, dsfull, rfull[2], rempty[2], gfull, drain, wfull[2], wempty[2], want, next;
+    alignas(16) uint32_t answer[4];
+    uint32_t tmem_base;
+    int abort, not_finite[2];
+    Work work[2], held;          // held: the last one taken, which a wait that gave up may have kept from being handed on
+};
+static_assert(sizeof(Ctl) <= 768, "control block");
 
 struct BwdArgs {
     Batch b;
@@ -43,6 +55,7 @@ struct BwdArgs {
     int splits;                                              // CTAs that share the rows a key tile is walked by
     float* part;                                             // their sums: [split][dV, dK][key][head][D]
     const void* dout;                                        // for what is not finite
+    int64_t slots;                                           // owner tiles, some of them empty
     Rows rdo;
     int* status;
 };
@@ -76,9 +89,9 @@ __device__ __forceinline__ void store_row(T* dst, float* part, uint32_t tcol, in
 }
 
 // The wait of a CTA that gives up for the loads in flight (100 us in all), before shared memory goes away.
-template <int NSLOT> __device__ __forceinline__ void land(Ctl* ctl, uint32_t issued) {
+template <int NSLOT> __device__ __forceinline__ void land(Ctl* ctl, uint32_t owners, uint32_t issued) {
     const uint64_t t_end = global_timer_ns() + 100000ull;
-    while (issued && !mbar_try_wait(smem_u32(&ctl->yfull), 0) && global_timer_ns() < t_end) {}
+    while (owners && !mbar_try_wait(smem_u32(&ctl->yfull), (owners - 1) & 1) && global_timer_ns() < t_end) {}
     for (uint32_t back = 1; back <= (uint32_t)NSLOT && back <= issued; ++back) {
         const uint32_t sq = issued - back;
         while (!mbar_try_wait(smem_u32(&ctl->full[sq % NSLOT]), (sq / NSLOT) & 1) && global_timer_ns() < t_end) {}
@@ -87,6 +100,32 @@ template <int NSLOT> __device__ __forceinline__ void land(Ctl* ctl, uint32_t iss
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------- dK, dV
+// Tile t of the grid: splits and heads go fastest; the first keys of a causal sequence, which the most queries see, first.
+__device__ __forceinline__ Work kv_work(const BwdArgs& a, int64_t t, int lane) {
+    const int wide = a.b.Hk * a.splits;
+    const int64_t x = t / wide;
+    const int hs = (int)(t - x * wide);
+    const Piece at = find_piece<false>(a.b.cu_k, a.b.B, a.b.Tk, a.slots, x, TN, lane);
+    Work w{};
+    w.head = hs % a.b.Hk;
+    w.split = hs / a.b.Hk;
+    w.first = at.first;
+    w.n_tok = at.n;
+    if (at.n <= 0 || at.seq < 0) return w;
+    w.w0 = a.b.q_at(at.seq);
+    w.nw = max(a.b.q_at(at.seq + 1) - w.w0, 0);
+    w.diag = a.b.causal ? at.length - w.nw - at.offset : TN;
+    w.from = min(max(-w.diag, 0), w.nw);
+    w.per = (w.nw - w.from + a.tokens - 1) / a.tokens;
+    const int64_t all = (int64_t)(a.b.G / a.pack) * w.per;
+    w.tile0 = (int)(all * w.split / a.splits);
+    w.nt = (int)(all * (w.split + 1) / a.splits) - w.tile0;
+    // Rows that see one key: their P is 1 whatever the logit, and dS is 0 and not what rounding leaves of a difference (where it is a number). They
+    // are the first columns of the first walked tile in causal attention, all rows (more than TM) where the sequence has one key.
+    w.ones = at.length == 1 ? TM + 1 : a.b.causal && at.offset == 0 && w.nw >= at.length ? a.pack : 0;
+    return w;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -95,28 +134,14 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     constexpr uint32_t DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wide = a.b.Hk * a.splits, kh = blockIdx.x % wide % a.b.Hk, split = blockIdx.x % wide / a.b.Hk;
-    // (the first keys of a causal sequence are seen by the most queries)
-    const Piece at = find_piece<false>(a.b.cu_k, a.b.B, a.b.Tk, gridDim.x / wide, blockIdx.x / wide, TN, lane);
-    if (at.n <= 0) return;
-    int q0 = 0, nq = 0, diag = 0, first = 0;                 // diag: query t sees the owner's keys 0 .. t + diag
-    if (at.seq >= 0) {
-        q0 = a.b.q_at(at.seq);
-        nq = max(a.b.q_at(at.seq + 1) - q0, 0);
-        diag = a.b.causal ? at.length - nq - at.offset : TN;
-        first = min(max(-diag, 0), nq);                      // the first query that sees one of them
-    }
-    const int subs = a.b.G / a.pack, per = (nq - first + a.tokens - 1) / a.tokens;
-    const int tile0 = (int)((int64_t)subs * per * split / a.splits), nt = uniform((int)((int64_t)subs * per * (split + 1) / a.splits) - tile0);
-    // Rows that see one key: their P is 1 whatever the logit, and dS is 0 and not what rounding leaves of a difference (where it is a number). They
-    // are the first columns of the first walked tile in causal attention, all rows (more than TM) where the sequence has one key.
-    const int ones = at.length == 1 ? TM + 1 : a.b.causal && at.offset == 0 && nq >= at.length ? a.pack : 0;
+    constexpr int USERS = 11;                                // warps that take each tile's work
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
     if (tid == 0) {
         const int earlier = *reinterpret_cast<volatile int*>(a.status);
         mbar_init(smem_u32(&ctl->yfull), 1);
+        mbar_init(smem_u32(&ctl->yempty), 1);
         for (int i = 0; i < C::NSLOT; ++i) {
             mbar_init(smem_u32(&ctl->full[i]), 1);
             mbar_init(smem_u32(&ctl->empty[i]), 1);
@@ -125,13 +150,18 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mbar_init(smem_u32(&ctl->sfull[i]), 1);
             mbar_init(smem_u32(&ctl->rfull[i]), 32);
             mbar_init(smem_u32(&ctl->rempty[i]), 8);
+            mbar_init(smem_u32(&ctl->wfull[i]), 1);
+            mbar_init(smem_u32(&ctl->wempty[i]), USERS);
+            ctl->work[i].n_tok = 0;
         }
+        ctl->held.n_tok = 0;
+        mbar_init(smem_u32(&ctl->want), 1);
         mbar_init(smem_u32(&ctl->dpfull), 1);
         mbar_init(smem_u32(&ctl->pfull), 8);
         mbar_init(smem_u32(&ctl->dsfull), 8);
         mbar_init(smem_u32(&ctl->gfull), 1);
         mbar_init(smem_u32(&ctl->drain), 1);
-        ctl->not_finite = 0;
+        mbar_init(smem_u32(&ctl->next), 1);
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 911);
         mbar_fence_init();
@@ -158,66 +188,104 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then minus delta
     float* row_delta = row_lse + C::NROW * TM;
-    uint32_t issued = 0;
+    bool ok = *abort_flag == 0;
+    // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
+    auto enter = [&](int n, Work& w) {
+        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        if (ok) w = ctl->work[n & 1];
+        return ok && w.n_tok > 0;
+    };
+    auto leave = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->wempty[n & 1]));
+    };
+    uint32_t issued = 0, owners = 0;
     // walked tile i: query heads head0 .., first token
-    auto head_of = [&](int i) { return kh * a.b.G + (tile0 + i) / per * a.pack; };
-    auto token_of = [&](int i) { return first + (tile0 + i) % per * a.tokens; };
+    auto head_of = [&](const Work& w, int i) { return w.head * a.b.G + (w.tile0 + i) / w.per * a.pack; };
+    auto token_of = [&](const Work& w, int i) { return w.from + (w.tile0 + i) % w.per * a.tokens; };
 
     if (warp >= 8) {
         reg_dec<REGS_REST>();
-        bool ok = *abort_flag == 0;
-        if (warp == 9) {
+        if (warp == 11) {
+            // -------------------------------------------------------- which tiles
+            hand_out<false>(ctl, [&](int64_t t) { return t >= 0 ? kv_work(a, t, lane) : Work{}; }, 0, ok, lane, abort_flag, a.status, 611);
+        } else if (warp == 9) {
             // -------------------------------------------------------- loads: K, V, then Q(i), dO(i)
-            if (lane == 0 && ok && nt > 0) {
-                mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * C::TILE);
-                for (int d = 0; d < D / 64; ++d) {
-                    tma_load_3d(base + C::Y1 + d * HALF, &tmK, smem_u32(&ctl->yfull), 64 * d, kh, at.first);
-                    tma_load_3d(base + C::Y2 + d * HALF, &tmV, smem_u32(&ctl->yfull), 64 * d, kh, at.first);
+            const uint32_t bytes = (uint32_t)(loaded * D * 2);
+            uint32_t slot = 0, par = 1;
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                if (w.nt <= 0) {
+                    if (lane == 0) mbar_arrive(smem_u32(&ctl->want));
+                    continue;
                 }
-                const uint32_t bytes = (uint32_t)(loaded * D * 2);
-                uint32_t slot = 0, par = 1;
-                for (int i = 0; i < nt && ok; ++i)
+                ok = mbar_wait_warp(smem_u32(&ctl->yempty), (owners & 1) ^ 1, abort_flag, a.status, 620);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * C::TILE);
+                    for (int d = 0; d < D / 64; ++d) {
+                        tma_load_3d(base + C::Y1 + d * HALF, &tmK, smem_u32(&ctl->yfull), 64 * d, w.head, w.first);
+                        tma_load_3d(base + C::Y2 + d * HALF, &tmV, smem_u32(&ctl->yfull), 64 * d, w.head, w.first);
+                    }
+                }
+                __syncwarp();
+                ++owners;
+                for (int i = 0; i < w.nt && ok; ++i) {
+                    const int h0 = head_of(w, i), t0 = w.w0 + token_of(w, i);
                     for (int x = 0; x < 2 && ok; ++x) {
-                        ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 621);
+                        ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 621);
                         if (!ok) break;
-                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
-                        mbar_arrive_expect_tx(bar, bytes);
-                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmDO : &tmQ, bar, 64 * d, head_of(i), q0 + token_of(i));
+                        if (lane == 0) {
+                            const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                            mbar_arrive_expect_tx(bar, bytes);
+                            for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmDO : &tmQ, bar, 64 * d, h0, t0);
+                        }
+                        __syncwarp();
                         ++issued;
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
+                }
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->want));
             }
         } else if (warp == 10) {
-            // -------------------------------------------------------- LSE and delta of tile i, once tile i - 2's have been read
-            for (int i = 0; i < nt && ok; ++i) {
-                float l[4], d[4];
-                const int h0 = head_of(i), t0 = token_of(i);
+            // -------------------------------------------------------- LSE and delta of each walked tile, once those of two tiles before have been read
+            uint32_t seq = 0;
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                for (int i = 0; i < w.nt && ok; ++i, ++seq) {
+                    float l[4], d[4];
+                    const int h0 = head_of(w, i), t0 = token_of(w, i);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int r = lane + 32 * x, t = t0 + r / a.pack;
-                    const bool valid = r < loaded && t < nq;
-                    const int64_t g = (int64_t)(h0 + r % a.pack) * a.b.Tq + q0 + t;
-                    const float z = valid ? __ldg(a.lse + g) : -INFINITY;
-                    l[x] = z == -INFINITY ? -INFINITY : -z * kLog2e;       // (added to the logit: P of a row without keys, or of none, is 0)
-                    d[x] = valid ? -__ldg(a.delta + g) : 0.f;
-                }
-                ok = mbar_wait_warp(smem_u32(&ctl->rempty[i % C::NROW]), ((i / C::NROW) & 1) ^ 1, abort_flag, a.status, 622);
-                if (!ok) break;
+                    for (int x = 0; x < 4; ++x) {
+                        const int r = lane + 32 * x, t = t0 + r / a.pack;
+                        const bool valid = r < loaded && t < w.nw;
+                        const int64_t g = (int64_t)(h0 + r % a.pack) * a.b.Tq + w.w0 + t;
+                        const float z = valid ? __ldg(a.lse + g) : -INFINITY;
+                        l[x] = z == -INFINITY ? -INFINITY : -z * kLog2e;   // (added to the logit: P of a row without keys, or of none, is 0)
+                        d[x] = valid ? -__ldg(a.delta + g) : 0.f;
+                    }
+                    const uint32_t stage = seq % C::NROW;
+                    ok = mbar_wait_warp(smem_u32(&ctl->rempty[stage]), ((seq / C::NROW) & 1) ^ 1, abort_flag, a.status, 622);
+                    if (!ok) break;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    row_lse[(i % C::NROW) * TM + lane + 32 * x] = l[x];
-                    row_delta[(i % C::NROW) * TM + lane + 32 * x] = d[x];
+                    for (int x = 0; x < 4; ++x) {
+                        row_lse[stage * TM + lane + 32 * x] = l[x];
+                        row_delta[stage * TM + lane + 32 * x] = d[x];
+                    }
+                    mbar_arrive(smem_u32(&ctl->rfull[stage]));
                 }
-                mbar_arrive(smem_u32(&ctl->rfull[i % C::NROW]));
             }
         } else if (warp == 8) {
             // -------------------------------------------------------- MMAs
             constexpr uint32_t ID_S = umma_idesc<T>(128, TM, 0, 0), ID_G = umma_idesc<T>(128, D, 0, 1);
             const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dx0 = umma_desc_sw128(0, HALF, 1024);
             const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, x_hi = (uint32_t)(dx0 >> 32), x_lo = (uint32_t)dx0;
-            auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
-            auto take = [&](int seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 623); };
-            auto first_product = [&](int x, int i) {         // x = 0: S(i) = K Q^T, x = 1: dP(i) = V dO^T
+            uint32_t done = 0, tiles = 0;                        // walked tiles and owners before this work
+            auto slot_of = [&](uint32_t seq) { return seq % C::NSLOT; };
+            auto take = [&](uint32_t seq) { ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), (seq / C::NSLOT) & 1, abort_flag, a.status, 623); };
+            auto first_product = [&](int x, uint32_t i, bool last) {         // x = 0: S(i) = K Q^T, x = 1: dP(i) = V dO^T; i counts over all works
                 take(2 * i + x);
                 if (!ok) return;
                 tc_fence_after();
@@ -229,38 +297,44 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         umma_ss_lohi(tmem + x * DP_COL, ya + off, k_hi, xb + off, k_hi, ID_S, ks > 0);
                     }
                     umma_commit(x ? smem_u32(&ctl->dpfull) : smem_u32(&ctl->sfull[0]));
+                    if (x && last) umma_commit(smem_u32(&ctl->yempty));
                 }
                 __syncwarp();
             };
-            auto second_product = [&](int x, int i) {        // x = 0: dK += dS^T Q, x = 1: dV += P^T dO
+            auto second_product = [&](int x, uint32_t i, uint32_t more) {        // x = 0: dK += dS^T Q, x = 1: dV += P^T dO
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * i + x) * C::TILE) >> 4), p = tmem + (x ? 0u : DP_COL);
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks)
                         umma_ts_lohi(tmem + (x ? DV_COL : DK_COL), p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G,
-                                     (i > 0 || ks > 0) ? 1u : 0u);
+                                     ks > 0 ? 1u : more);
                     umma_commit(empty0 + 8 * slot_of(2 * i + x));
                 }
                 __syncwarp();
             };
-            if (nt > 0) {
-                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), 0, abort_flag, a.status, 624);
-                if (ok) first_product(0, 0);
-                if (ok) first_product(1, 0);
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                const int nt = uniform(w.nt);
+                if (nt <= 0) continue;
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), tiles & 1, abort_flag, a.status, 624);
+                ++tiles;
+                if (ok) first_product(0, done, false);
+                if (ok) first_product(1, done, nt == 1);
+                for (int i = 0; i < nt && ok; ++i, ++done) {
+                    ok = mbar_wait_warp(smem_u32(&ctl->pfull), done & 1, abort_flag, a.status, 625);
+                    if (!ok) break;
+                    second_product(1, done, i > 0);
+                    if (i + 1 < nt) first_product(0, done + 1, false);           // (over P, which dV has read: MMAs run in their order)
+                    ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), done & 1, abort_flag, a.status, 626);
+                    if (!ok) break;
+                    second_product(0, done, i > 0);
+                    if (i + 1 < nt) first_product(1, done + 1, i + 2 == nt);
+                }
+                if (ok && elect_one()) umma_commit(smem_u32(&ctl->gfull));
+                __syncwarp();
             }
-            for (int i = 0; i < nt && ok; ++i) {
-                ok = mbar_wait_warp(smem_u32(&ctl->pfull), i & 1, abort_flag, a.status, 625);
-                if (!ok) break;
-                second_product(1, i);
-                if (i + 1 < nt) first_product(0, i + 1);     // (over P, which dV has read: MMAs run in their order)
-                ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), i & 1, abort_flag, a.status, 626);
-                if (!ok) break;
-                second_product(0, i);
-                if (i + 1 < nt) first_product(1, i + 1);
-            }
-            if (ok && nt > 0 && elect_one()) umma_commit(smem_u32(&ctl->gfull));
-            __syncwarp();
             // every MMA issued above has finished before tensor memory is freed
             if (elect_one()) umma_commit(smem_u32(&ctl->drain));
             __syncwarp();
@@ -272,13 +346,17 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const int r = tid & 127, ch = warp >> 2;             // key row, half of the columns
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16), scol = tl + 64 * ch, dpcol = tl + DP_COL + 64 * ch;
         const float c = a.b.scale * kLog2e;
-        bool ok = *abort_flag == 0;
-        for (int i = 0; i < nt && ok; ++i) {
-            const int t0 = token_of(i);
+        uint32_t done = 0, tiles = 0;                        // walked tiles and owners before this work
+        Work w;
+        for (int n = 0; enter(n, w); ++n) {
+        const int nt = w.nt, nw = w.nw, diag = w.diag, first = w.from, stop = first + w.per * a.tokens, last = w.n_tok - 1, ones = w.ones;
+        int t0 = nt > 0 ? token_of(w, 0) : 0;
+        for (int i = 0; i < nt && ok; ++i, ++done) {
+            const uint32_t stage = done % C::NROW;
             // the first of the tile's tokens sees the fewest keys; the rows behind the last token are of other sequences
-            const bool cut = t0 + diag < at.n - 1, masked = cut || t0 + a.tokens > nq;
-            ok = mbar_wait_warp(smem_u32(&ctl->rfull[i % C::NROW]), (i / C::NROW) & 1, abort_flag, a.status, 628) &&
-                 mbar_wait_warp(smem_u32(&ctl->sfull[0]), i & 1, abort_flag, a.status, 629);
+            const bool cut = t0 + diag < last, masked = cut || t0 + a.tokens > nw;
+            ok = mbar_wait_warp(smem_u32(&ctl->rfull[stage]), (done / C::NROW) & 1, abort_flag, a.status, 628) &&
+                 mbar_wait_warp(smem_u32(&ctl->sfull[0]), done & 1, abort_flag, a.status, 629);
             if (!ok) break;
             tc_fence_after();
             uint32_t x[64];
@@ -287,8 +365,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_wait_ld_regs(x);
             tmem_wait_ld_regs(x + 32);
             const int lim = cut ? max(r - diag - t0, 0) * a.pack - 64 * ch : 0;      // columns before it do not see the key
-            const int end = min(nq - t0, a.tokens) * a.pack - 64 * ch;               // columns from here on are not rows of the sequence
-            const float4* rl = reinterpret_cast<const float4*>(row_lse + (i % C::NROW) * TM + 64 * ch);
+            const int end = min(nw - t0, a.tokens) * a.pack - 64 * ch;               // columns from here on are not rows of the sequence
+            const float4* rl = reinterpret_cast<const float4*>(row_lse + stage * TM + 64 * ch);
             // P; one pair in four on the FMA pipes, as many as take no longer than the others take the 16 exponentials a clock of an SM
             auto probabilities = [&](auto cut_tile) {
                 const float2 cc = make_float2(c, c);
@@ -316,10 +394,10 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (masked) {
                 probabilities(std::true_type{});
                 // dP of this tile is there too: from here on its Q and dO are read by the second products only
-                ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 630);
+                ok = mbar_wait_warp(smem_u32(&ctl->dpfull), done & 1, abort_flag, a.status, 630);
                 if (!ok) break;
-                const uint32_t slot = (uint32_t)(2 * i + ch) % C::NSLOT;             // half of the threads Q, half dO
-                if (clean_row<T, D>(smem + C::RING + slot * C::TILE, r)) *reinterpret_cast<volatile int*>(&ctl->not_finite) = 1;
+                const uint32_t slot = (2 * done + ch) % C::NSLOT;             // half of the threads Q, half dO
+                if (clean_row<T, D>(smem + C::RING + slot * C::TILE, r)) *reinterpret_cast<volatile int*>(&ctl->not_finite[n & 1]) = 1;
                 fence_proxy_async_smem();
             } else {
                 probabilities(std::false_type{});
@@ -333,7 +411,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 for (int j = 0; j < 64; ++j)
                     if (j < ones - 64 * ch && fabsf(__uint_as_float(x[j])) < INFINITY) x[j] = 0;
             }
-            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 631);
+            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), done & 1, abort_flag, a.status, 631);
             if (!ok) break;
             tc_fence_after();
             uint32_t y[64];
@@ -341,7 +419,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_ld32(dpcol + 32, y + 32);
             tmem_wait_ld_regs(y);
             tmem_wait_ld_regs(y + 32);
-            const float4* rd = reinterpret_cast<const float4*>(row_delta + (i % C::NROW) * TM + 64 * ch);
+            const float4* rd = reinterpret_cast<const float4*>(row_delta + stage * TM + 64 * ch);
             auto differences = [&](auto cut_tile) {
                 uint32_t ds[32];
 #pragma unroll
@@ -368,42 +446,46 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(smem_u32(&ctl->rempty[i % C::NROW]));
+                mbar_arrive(smem_u32(&ctl->rempty[stage]));
                 mbar_arrive(smem_u32(&ctl->dsfull));
             }
+            t0 += a.tokens;
+            if (t0 >= stop) t0 = first;
         }
-        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 632);
-        if (ok) {
-            tc_fence_after();
-            const int64_t row = (int64_t)(at.first + r) * a.b.Hk + kh;
-            const bool valid = r < at.n;
-            // warps 0-3 write dV, warps 4-7 dK
-            T* dst = static_cast<T*>(ch ? a.d0 : a.d1) + row * D;
-            float* part = a.splits > 1 ? a.part + ((int64_t)(2 * split + ch) * a.b.Tk * a.b.Hk + row) * D : nullptr;
-            store_row<T, D>(dst, part, tl + (ch ? DK_COL : DV_COL), 0, D / 32, nt > 0, valid, ch ? a.b.scale : 1.f);
-            if (ch == 0 && valid && nt > 0 && *reinterpret_cast<volatile int*>(&ctl->not_finite)) {
-                // what is not finite in dO of the rows of cut tiles that see this key
-                for (int i = 0; i < nt; ++i) {
-                    const int t0 = token_of(i);
-                    if (!(t0 + diag < at.n - 1 || t0 + a.tokens > nq)) continue;
-                    for (int t = max(t0, r - diag); t < min(t0 + a.tokens, nq); ++t)
-                        for (int h = head_of(i); h < head_of(i) + a.pack; ++h) {
-                            const T* src = static_cast<const T*>(a.dout) + (int64_t)(q0 + t) * a.rdo.token + (int64_t)h * a.rdo.head;
-                            for (int d = 0; d < D; ++d) {
-                                const float e = to_float(src[d]);
-                                if (fabsf(e) < INFINITY) continue;
-                                if (part) part[d] += e;
-                                else dst[d] = from_float<T>(to_float(dst[d]) + e);
-                            }
+        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), tiles++ & 1, abort_flag, a.status, 632);
+        if (!ok) break;
+        tc_fence_after();
+        w = ctl->work[n & 1];                                // (read again: the loop's registers are few)
+        const int64_t row = (int64_t)(w.first + r) * a.b.Hk + w.head;
+        const bool valid = r < w.n_tok;
+        // warps 0-3 write dV, warps 4-7 dK
+        T* dst = static_cast<T*>(ch ? a.d0 : a.d1) + row * D;
+        float* part = a.splits > 1 ? a.part + ((int64_t)(2 * w.split + ch) * a.b.Tk * a.b.Hk + row) * D : nullptr;
+        store_row<T, D>(dst, part, tl + (ch ? DK_COL : DV_COL), 0, D / 32, w.nt > 0, valid, ch ? a.b.scale : 1.f);
+        if (ch == 0 && valid && w.nt > 0 && *reinterpret_cast<volatile int*>(&ctl->not_finite[n & 1])) {
+            // what is not finite in dO of the rows of cut tiles that see this key
+            for (int i = 0; i < w.nt; ++i) {
+                const int t0 = token_of(w, i);
+                if (!(t0 + w.diag < w.n_tok - 1 || t0 + a.tokens > w.nw)) continue;
+                for (int t = max(t0, r - w.diag); t < min(t0 + a.tokens, w.nw); ++t)
+                    for (int h = head_of(w, i); h < head_of(w, i) + a.pack; ++h) {
+                        const T* src = static_cast<const T*>(a.dout) + (int64_t)(w.w0 + t) * a.rdo.token + (int64_t)h * a.rdo.head;
+                        for (int d = 0; d < D; ++d) {
+                            const float e = to_float(src[d]);
+                            if (fabsf(e) < INFINITY) continue;
+                            if (part) part[d] += e;
+                            else dst[d] = from_float<T>(to_float(dst[d]) + e);
                         }
-                }
+                    }
             }
+        }
+        leave(n);
         }
     }
 
     // ---------------------------------------------------------------- teardown
     __syncwarp();
-    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, issued);
+    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, owners, issued);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -411,19 +493,39 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (*abort_flag && a.splits > 1) {
-        for (int e = tid; e < at.n * D; e += THREADS) {
-            const int64_t w = ((int64_t)(at.first + e / D) * a.b.Hk + kh) * D + e % D, all = (int64_t)a.b.Tk * a.b.Hk * D;
-            a.part[2 * split * all + w] = a.part[(2 * split + 1) * all + w] = __uint_as_float(kNaN32);
+    if (*abort_flag) {
+        // NaN in the tiles that the CTA had taken and may not have finished: the caller's memory is not initialised
+        for (int x = 0; x < 3; ++x) {
+            const Work w = x < 2 ? ctl->work[x] : ctl->held;
+            const int64_t all = (int64_t)a.b.Tk * a.b.Hk * D;
+            for (int e = tid; e < w.n_tok * D; e += THREADS) {
+                const int64_t at = ((int64_t)(w.first + e / D) * a.b.Hk + w.head) * D + e % D;
+                if (a.splits > 1) a.part[2 * w.split * all + at] = a.part[(2 * w.split + 1) * all + at] = __uint_as_float(kNaN32);
+                else static_cast<uint16_t*>(a.d0)[at] = static_cast<uint16_t*>(a.d1)[at] = (uint16_t)kNaN16x2;
+            }
         }
-    } else if (*abort_flag)
-        for (int e = tid; e < at.n * (D / 2); e += THREADS) {
-            const int64_t w = ((int64_t)(at.first + e / (D / 2)) * a.b.Hk + kh) * (D / 2) + e % (D / 2);
-            static_cast<uint32_t*>(a.d0)[w] = static_cast<uint32_t*>(a.d1)[w] = kNaN16x2;
-        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------- dQ
+// Tile t of the grid: heads go fastest; the last rows of a causal sequence, which see the most keys, first.
+__device__ __forceinline__ Work q_work(const BwdArgs& a, int64_t t, int lane) {
+    const int vheads = a.b.H / a.pack;
+    const int64_t x = t / vheads;
+    const Piece at = find_piece<true>(a.b.cu_q, a.b.B, a.b.Tq, a.slots, x, a.tokens, lane);
+    Work w{};
+    w.head = (int)(t - x * vheads) * a.pack;
+    w.first = at.first;
+    w.n_tok = at.n;
+    if (at.n <= 0 || at.seq < 0) return w;
+    w.w0 = a.b.k_at(at.seq);
+    w.nw = max(a.b.k_at(at.seq + 1) - w.w0, 0);
+    w.diag = w.nw - at.length + at.offset;
+    const int last = at.n - 1;
+    w.nt = ((a.b.causal ? min(max(last + w.diag + 1, 0), w.nw) : w.nw) + TN - 1) / TN;
+    return w;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -432,32 +534,34 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     constexpr uint32_t DP_COL = 256, DQ_COL = 384;           // S of even and of odd tiles: columns 0 and 128
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int vheads = a.b.H / a.pack, vh = blockIdx.x % vheads, head0 = vh * a.pack, kh = head0 / a.b.G;
-    const Piece at = find_piece<true>(a.b.cu_q, a.b.B, a.b.Tq, gridDim.x / vheads, blockIdx.x / vheads, a.tokens, lane);
-    if (at.n <= 0) return;
-    int k0 = 0, nk = 0, diag = 0;                            // token t of the span sees keys 0 .. t + diag
-    if (at.seq >= 0) {
-        k0 = a.b.k_at(at.seq);
-        nk = max(a.b.k_at(at.seq + 1) - k0, 0);
-        diag = nk - at.length + at.offset;
-    }
-    auto seen_by = [&](int t) { return a.b.causal ? min(max(t + diag + 1, 0), nk) : nk; };
-    const int nt = uniform((seen_by(at.n - 1) + TN - 1) / TN), whole = seen_by(0) / TN;
+    constexpr int USERS = 10;                                // warps that take each tile's work
     const uint32_t base = smem_u32(smem);
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + C::CTL);
     volatile int* abort_flag = &ctl->abort;
     if (tid == 0) {
         const int earlier = *reinterpret_cast<volatile int*>(a.status);
         mbar_init(smem_u32(&ctl->yfull), 1);
+        mbar_init(smem_u32(&ctl->yempty), 1);
         for (int i = 0; i < C::NSLOT; ++i) {
             mbar_init(smem_u32(&ctl->full[i]), 1);
             mbar_init(smem_u32(&ctl->empty[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctl->sfull[i]), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ctl->sfull[i]), 1);
+            mbar_init(smem_u32(&ctl->rfull[i]), 32);
+            mbar_init(smem_u32(&ctl->rempty[i]), 8);
+            mbar_init(smem_u32(&ctl->wfull[i]), 1);
+            mbar_init(smem_u32(&ctl->wempty[i]), USERS);
+            ctl->work[i].n_tok = 0;
+        }
+        ctl->held.n_tok = 0;
+        mbar_init(smem_u32(&ctl->want), 1);
         mbar_init(smem_u32(&ctl->dpfull), 1);
+        mbar_init(smem_u32(&ctl->pfull), 8);
         mbar_init(smem_u32(&ctl->dsfull), 8);
         mbar_init(smem_u32(&ctl->gfull), 1);
         mbar_init(smem_u32(&ctl->drain), 1);
+        mbar_init(smem_u32(&ctl->next), 1);
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 912);
         mbar_fence_init();
@@ -472,46 +576,77 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tc_fence_after();
     const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
-    uint32_t issued = 0;
+    bool ok = *abort_flag == 0;
+    // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
+    auto enter = [&](int n, Work& w) {
+        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        if (ok) w = ctl->work[n & 1];
+        return ok && w.n_tok > 0;
+    };
+    auto leave = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->wempty[n & 1]));
+    };
+    uint32_t issued = 0, owners = 0;
 
     if (warp >= 8) {
         reg_dec<REGS_REST>();
-        bool ok = *abort_flag == 0;
-        if (warp == 9) {
+        if (warp == 10) {
+            // -------------------------------------------------------- which tiles
+            hand_out<false>(ctl, [&](int64_t t) { return t >= 0 ? q_work(a, t, lane) : Work{}; }, 0, ok, lane, abort_flag, a.status, 611);
+        } else if (warp == 9) {
             // -------------------------------------------------------- loads: Q, dO, then K(i), V(i)
-            if (lane == 0 && ok && nt > 0) {
-                const uint32_t bytes = (uint32_t)(a.tokens * a.pack * D * 2);
-                mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * bytes);
-                for (int d = 0; d < D / 64; ++d) {
-                    tma_load_3d(base + C::Y1 + d * HALF, &tmQ, smem_u32(&ctl->yfull), 64 * d, head0, at.first);
-                    tma_load_3d(base + C::Y2 + d * HALF, &tmDO, smem_u32(&ctl->yfull), 64 * d, head0, at.first);
+            const uint32_t bytes = (uint32_t)(a.tokens * a.pack * D * 2);
+            uint32_t slot = 0, par = 1;
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                if (w.nt <= 0) {
+                    if (lane == 0) mbar_arrive(smem_u32(&ctl->want));
+                    continue;
                 }
-                uint32_t slot = 0, par = 1;
-                for (int i = 0; i < nt && ok; ++i)
+                ok = mbar_wait_warp(smem_u32(&ctl->yempty), (owners & 1) ^ 1, abort_flag, a.status, 640);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(smem_u32(&ctl->yfull), 2 * bytes);
+                    for (int d = 0; d < D / 64; ++d) {
+                        tma_load_3d(base + C::Y1 + d * HALF, &tmQ, smem_u32(&ctl->yfull), 64 * d, w.head, w.first);
+                        tma_load_3d(base + C::Y2 + d * HALF, &tmDO, smem_u32(&ctl->yfull), 64 * d, w.head, w.first);
+                    }
+                }
+                __syncwarp();
+                ++owners;
+                const int kh = w.head / a.b.G;
+                for (int i = 0; i < w.nt && ok; ++i)
                     for (int x = 0; x < 2 && ok; ++x) {
-                        ok = mbar_wait(empty0 + 8 * slot, par, abort_flag, a.status, 641);
+                        ok = mbar_wait_warp(empty0 + 8 * slot, par, abort_flag, a.status, 641);
                         if (!ok) break;
-                        const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
-                        mbar_arrive_expect_tx(bar, C::TILE);
-                        for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, k0 + i * TN);
+                        if (lane == 0) {
+                            const uint32_t bar = full0 + 8 * slot, dst = base + C::RING + slot * C::TILE;
+                            mbar_arrive_expect_tx(bar, C::TILE);
+                            for (int d = 0; d < D / 64; ++d) tma_load_3d(dst + d * HALF, x ? &tmV : &tmK, bar, 64 * d, kh, w.w0 + i * TN);
+                        }
+                        __syncwarp();
                         ++issued;
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->want));
             }
         } else if (warp == 8) {
             // -------------------------------------------------------- MMAs
             constexpr uint32_t ID_S = umma_idesc<T>(128, TN, 0, 0), ID_G = umma_idesc<T>(128, D, 0, 1);
             const uint64_t dk0 = umma_desc_sw128(0, 16, 1024), dx0 = umma_desc_sw128(0, HALF, 1024);
             const uint32_t k_hi = (uint32_t)(dk0 >> 32), k_lo = (uint32_t)dk0, x_hi = (uint32_t)(dx0 >> 32), x_lo = (uint32_t)dx0;
-            auto slot_of = [&](int seq) { return (uint32_t)seq % C::NSLOT; };
-            auto first_product = [&](int x, int i) {         // x = 0: S(i) = Q K^T, x = 1: dP(i) = dO V^T
-                const int seq = 2 * i + x;
-                ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), ((uint32_t)seq / C::NSLOT) & 1, abort_flag, a.status, 643);
+            uint32_t done = 0, tiles = 0;                        // walked tiles and owners before this work
+            auto slot_of = [&](uint32_t seq) { return seq % C::NSLOT; };
+            auto first_product = [&](int x, uint32_t i, bool last) {         // x = 0: S(i) = Q K^T, x = 1: dP(i) = dO V^T; i counts over all works
+                const uint32_t seq = 2 * i + x;
+                ok = ok && mbar_wait_warp(full0 + 8 * slot_of(seq), (seq / C::NSLOT) & 1, abort_flag, a.status, 643);
                 if (!ok) return;
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t ya = k_lo + ((base + (x ? C::Y2 : C::Y1)) >> 4), xb = k_lo + ((base + C::RING + slot_of(seq) * C::TILE) >> 4);
-                    const uint32_t d = tmem + (x ? DP_COL : (uint32_t)(i & 1) * 128);
+                    const uint32_t d = tmem + (x ? DP_COL : (i & 1) * 128);
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks) {
                         const uint32_t off = ((ks >> 2) * HALF + (ks & 3) * 32) >> 4;
@@ -519,30 +654,36 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     }
                     umma_commit(x ? smem_u32(&ctl->dpfull) : smem_u32(&ctl->sfull[i & 1]));
                     if (x) umma_commit(empty0 + 8 * slot_of(seq));       // V is needed no more
+                    if (x && last) umma_commit(smem_u32(&ctl->yempty));
                 }
                 __syncwarp();
             };
-            if (nt > 0) {
-                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), 0, abort_flag, a.status, 644);
-                if (ok) first_product(0, 0);
-                if (ok) first_product(1, 0);
-            }
-            for (int i = 0; i < nt && ok; ++i) {
-                if (i + 1 < nt) first_product(0, i + 1);     // (over dS of tile i - 1, which dQ has read: MMAs run in their order)
-                ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), i & 1, abort_flag, a.status, 646);
-                if (!ok) break;
-                if (i + 1 < nt) first_product(1, i + 1);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * i) * C::TILE) >> 4), p = tmem + (uint32_t)(i & 1) * 128;
+            Work w;
+            for (int n = 0; enter(n, w); ++n) {
+                leave(n);
+                const int nt = uniform(w.nt);
+                if (nt <= 0) continue;
+                ok = ok && mbar_wait_warp(smem_u32(&ctl->yfull), tiles & 1, abort_flag, a.status, 644);
+                ++tiles;
+                if (ok) first_product(0, done, false);
+                if (ok) first_product(1, done, nt == 1);
+                for (int i = 0; i < nt && ok; ++i, ++done) {
+                    if (i + 1 < nt) first_product(0, done + 1, false);           // (over dS of tile i - 1, which dQ has read: MMAs run in their order)
+                    ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), done & 1, abort_flag, a.status, 646);
+                    if (!ok) break;
+                    if (i + 1 < nt) first_product(1, done + 1, i + 2 == nt);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * done) * C::TILE) >> 4), p = tmem + (done & 1) * 128;
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        umma_ts_lohi(tmem + DQ_COL, p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, (i > 0 || ks > 0) ? 1u : 0u);
-                    umma_commit(empty0 + 8 * slot_of(2 * i));
-                    if (i + 1 == nt) umma_commit(smem_u32(&ctl->gfull));
+                        for (int ks = 0; ks < 8; ++ks)
+                            umma_ts_lohi(tmem + DQ_COL, p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, (i > 0 || ks > 0) ? 1u : 0u);
+                        umma_commit(empty0 + 8 * slot_of(2 * done));
+                        if (i + 1 == nt) umma_commit(smem_u32(&ctl->gfull));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             // every MMA issued above has finished before tensor memory is freed
             if (elect_one()) umma_commit(smem_u32(&ctl->drain));
@@ -553,17 +694,21 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         // ------------------------------------------------------------ P, dS and epilogue
         reg_inc<REGS_MATH>();
         const int r = tid & 127, ch = warp >> 2;
-        const int tok = r / a.pack, head = head0 + r % a.pack;
-        const bool valid = tok < a.tokens && tok < at.n;
-        const int vis = valid ? seen_by(tok) : 0;
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16), dpcol = tl + DP_COL + 64 * ch;
         const float c = a.b.scale * kLog2e;
-        const int64_t g = (int64_t)head * a.b.Tq + at.first + tok;
+        const int tok = r / a.pack, lane_head = r % a.pack;
+        uint32_t done = 0, tiles = 0;                        // walked tiles and owners before this work
+        Work w;
+        for (int n = 0; enter(n, w); ++n) {
+        const bool valid = tok < a.tokens && tok < w.n_tok;
+        auto seen_by = [&](int t) { return a.b.causal ? min(max(t + w.diag + 1, 0), w.nw) : w.nw; };
+        const int vis = valid ? seen_by(tok) : 0, whole = seen_by(0) / TN;
+        const int64_t g = (int64_t)(w.head + lane_head) * a.b.Tq + w.first + tok;
         const float z = valid ? a.lse[g] : -INFINITY, off = z == -INFINITY ? -INFINITY : -z * kLog2e, delta = valid ? a.delta[g] : 0.f;
-        bool ok = *abort_flag == 0;
-        for (int i = 0; i < nt && ok; ++i) {
-            const uint32_t scol = tl + (uint32_t)(i & 1) * 128 + 64 * ch;
-            ok = mbar_wait_warp(smem_u32(&ctl->sfull[i & 1]), (i >> 1) & 1, abort_flag, a.status, 649);
+        const int nt = w.nt;
+        for (int i = 0; i < nt && ok; ++i, ++done) {
+            const uint32_t scol = tl + (done & 1) * 128 + 64 * ch;
+            ok = mbar_wait_warp(smem_u32(&ctl->sfull[done & 1]), (done >> 1) & 1, abort_flag, a.status, 649);
             if (!ok) break;
             tc_fence_after();
             uint32_t x[64];
@@ -587,13 +732,13 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             if (masked) {
                 probabilities(std::false_type{});
                 // S has read K by now; what is left is dQ, where hidden keys have dS = 0. A half of d for each half of the threads
-                uint8_t* tile = smem + C::RING + (uint32_t)(2 * i) % C::NSLOT * C::TILE;
+                uint8_t* tile = smem + C::RING + (2 * done) % C::NSLOT * C::TILE;
                 if (64 * ch < D) clean_row<T, 64>(tile + ch * HALF, r);
                 fence_proxy_async_smem();
             } else {
                 probabilities(std::true_type{});
             }
-            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), i & 1, abort_flag, a.status, 651);
+            ok = mbar_wait_warp(smem_u32(&ctl->dpfull), done & 1, abort_flag, a.status, 651);
             if (!ok) break;
             tc_fence_after();
             uint32_t y[64];
@@ -624,17 +769,19 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&ctl->dsfull));
         }
-        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), 0, abort_flag, a.status, 652);
-        if (ok) {
-            tc_fence_after();
-            T* dst = static_cast<T*>(a.d0) + ((int64_t)(at.first + tok) * a.b.H + head) * D;
-            store_row<T, D>(dst, nullptr, tl + DQ_COL, ch * (D / 64), (ch + 1) * (D / 64), nt > 0, valid, a.b.scale);
+        if (nt > 0) ok = ok && mbar_wait_warp(smem_u32(&ctl->gfull), tiles++ & 1, abort_flag, a.status, 652);
+        if (!ok) break;
+        tc_fence_after();
+        w = ctl->work[n & 1];                                // (read again: the loop's registers are few)
+        T* dst = static_cast<T*>(a.d0) + ((int64_t)(w.first + tok) * a.b.H + w.head + lane_head) * D;
+        store_row<T, D>(dst, nullptr, tl + DQ_COL, ch * (D / 64), (ch + 1) * (D / 64), nt > 0, valid, a.b.scale);
+        leave(n);
         }
     }
 
     // ---------------------------------------------------------------- teardown
     __syncwarp();
-    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, issued);
+    if (warp == 9 && lane == 0 && *abort_flag) land<C::NSLOT>(ctl, owners, issued);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -642,11 +789,16 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (*abort_flag)
-        for (int e = tid; e < at.n * a.pack * (D / 2); e += THREADS) {
-            const int row = e / (D / 2);
-            static_cast<uint32_t*>(a.d0)[((int64_t)(at.first + row / a.pack) * a.b.H + head0 + row % a.pack) * (D / 2) + e % (D / 2)] = kNaN16x2;
+    if (*abort_flag) {
+        // NaN in the tiles that the CTA had taken and may not have finished: the caller's memory is not initialised
+        for (int x = 0; x < 3; ++x) {
+            const Work w = x < 2 ? ctl->work[x] : ctl->held;
+            for (int e = tid; e < w.n_tok * a.pack * (D / 2); e += THREADS) {
+                const int row = e / (D / 2);
+                static_cast<uint32_t*>(a.d0)[((int64_t)(w.first + row / a.pack) * a.b.H + w.head + row % a.pack) * (D / 2) + e % (D / 2)] = kNaN16x2;
+            }
         }
+    }
 }
 
 // dK, dV = the sums of their parts in the order of the CTAs; four values a thread.
@@ -692,7 +844,8 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     if (int rc = make_rows_map<T>(&tv, v, D, kvh, nk, rv, 1, TN)) return rc;
     for (int kv = 0; kv < 2; ++kv) {
         if (!(kv ? dk : dq)) continue;
-        const int64_t grid = kv ? (int64_t)a.b.Hk * a.splits * piece_slots(a.b.Tk, TN, a.b.B) : a.b.H / a.pack * piece_slots(a.b.Tq, a.tokens, a.b.B);
+        a.slots = kv ? piece_slots(a.b.Tk, TN, a.b.B) : piece_slots(a.b.Tq, a.tokens, a.b.B);
+        const int64_t grid = a.slots * (kv ? a.b.Hk * a.splits : a.b.H / a.pack);
         if (grid > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many tiles");
         auto kern = kv ? packed_bwd_kv_kernel<T, D> : packed_bwd_q_kernel<T, D>;
         if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;

@@ -42,11 +42,11 @@ struct Work {
     __host__ __device__ __forceinline__ int last() const { return end0 > end1 ? end0 : end1; }
 };
 struct Ctl {
-    uint64_t qfull[2], qempty[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain, wfull[2], wempty[2], next;
+    uint64_t qfull[2], qempty[2], full[10], empty[10], sfull[2], pfull[2], ofull[2], drain, wfull[2], wempty[2], want, next;
     alignas(16) uint32_t answer[4];
     uint32_t tmem_base;
     int abort, not_finite[2];
-    Work work[2], held[2];       // held: taken, but not handed on before a wait gave up; the answer that came after it
+    Work work[2], held;          // held: the last one taken, which a wait that gave up may have kept from being handed on
 };
 static_assert(sizeof(Ctl) <= 768, "control block");
 
@@ -104,27 +104,6 @@ template <bool PAGED> __device__ __forceinline__ Work work_of(const FwdArgs& a, 
     return w;
 }
 
-// A running CTA takes the place of one of its grid that has not started (its index, or -1 where there is none left): CTAs are as many as
-// fit, and what one sets up serves all the tiles it takes. One thread asks; after a refusal it must not ask again.
-__device__ __forceinline__ void ask_next(uint32_t answer, uint32_t bar) {
-    mbar_arrive_expect_tx(bar, 16);
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
-}
-__device__ __forceinline__ int next_of(uint32_t answer) {
-    uint32_t x, got;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
-        "ld.shared.b128 h, [%2];\n\t"
-        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
-        "mov.b32 %0, 0;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n\t"
-        "selp.u32 %1, 1, 0, p;\n\t}"
-        : "=r"(x), "=r"(got)
-        : "r"(answer)
-        : "memory");
-    return got ? (int)x : -1;
-}
-
 template <typename T, int D, bool PAGED>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -156,7 +135,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         mbar_init(smem_u32(&ctl->drain), 1);
         mbar_init(smem_u32(&ctl->next), 1);
-        ctl->held[0].n_tok = ctl->held[1].n_tok = 0;
+        mbar_init(smem_u32(&ctl->want), 1);
+        ctl->held.n_tok = 0;
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 910);
         mbar_fence_init();
@@ -187,50 +167,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (warp >= 8) {
         reg_dec<REGS_REST>();
         if (warp == 10) {
-            // -------------------------------------------------------- which tiles: one ahead of the others
-            int64_t t = blockIdx.x;
-            uint32_t asked = 0;
-            for (int n = 0;;) {
-                Work w{};
-                if (t >= 0) {
-                    w = work_of<PAGED>(a, t, lane);
-                    if (lane == 0) ctl->held[0] = w;
-                }
-                if (!ok) break;
-                if (!PAGED && t >= 0 && lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
-                if (t < 0 || w.n_tok > 0) {
-                    ok = mbar_wait_warp(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, abort_flag, a.status, 611);
-                    if (ok && lane == 0) {
-                        ctl->work[n & 1] = w;
-                        ctl->not_finite[n & 1] = 0;
-                        mbar_arrive(smem_u32(&ctl->wfull[n & 1]));
-                    }
-                    ++n;
-                    __syncwarp();
-                    if (t < 0) break;
-                }
-                if (PAGED) {
-                    // all tiles are alike: every SM has as many, one more at most (taken as CTAs came, some runs had one that did another, 585 us
-                    // instead of 500). After a wait that gave up the join writes NaN whatever the parts hold
-                    t = t + gridDim.x < a.slots ? t + gridDim.x : -1;
-                    if (!ok) break;
-                    continue;
-                }
-                // (also where a wait gave up: what the answer takes from the grid nobody else will do)
-                const bool there = mbar_wait_warp(smem_u32(&ctl->next), asked & 1, abort_flag, a.status, 612) ||
-                                   mbar_wait_answer(smem_u32(&ctl->next), asked & 1);
-                ++asked;
-                t = there ? next_of(smem_u32(ctl->answer)) : -1;
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (!ok) {
-                    if (t >= 0) {
-                        w = work_of<PAGED>(a, t, lane);
-                        if (lane == 0) ctl->held[1] = w;
-                    }
-                    break;
-                }
-            }
+            // -------------------------------------------------------- which tiles
+            // Paged tiles are all alike: every SM has as many, one more at most. (Taken as CTAs came, some runs had one that did another: 585 us instead of
+            // 500 for 256 requests. After a wait that gave up the join writes NaN whatever the parts hold.)
+            hand_out<PAGED>(ctl, [&](int64_t t) { return t >= 0 ? work_of<PAGED>(a, t, lane) : Work{}; }, a.slots, ok, lane, abort_flag, a.status, 611);
         } else if (warp == 9) {
             // -------------------------------------------------------- loads: Q, then K(i), V(i) for every i
             const int box = min(TN, PAGED ? 1 << a.log_page : TN), boxes = TN / box;
@@ -282,6 +222,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
                 }
+                if (!PAGED && lane == 0) mbar_arrive(smem_u32(&ctl->want));
             }
         } else if (warp == 8) {
             // -------------------------------------------------------- MMAs
@@ -560,8 +501,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (*abort_flag) {
         // NaN in the tiles that the CTA had taken and may not have finished: the caller's memory is not initialised
-        for (int x = 0; x < 4; ++x) {
-            const Work w = x < 2 ? ctl->work[x] : ctl->held[x - 2];
+        for (int x = 0; x < 3; ++x) {
+            const Work w = x < 2 ? ctl->work[x] : ctl->held;
             for (int e = tid; e < w.n_tok * a.pack; e += THREADS) {
                 const int head = w.vh * a.pack + e % a.pack;
                 const int64_t row = (int64_t)(w.q0 + e / a.pack) * a.b.H + head;

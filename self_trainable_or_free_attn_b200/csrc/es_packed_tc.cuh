@@ -197,5 +197,63 @@ template <typename T> int make_pages_map(CUtensorMap* m, const void* ptr, int D,
                              const_cast<void*>(ptr), dims, str, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// A running CTA takes the place of one of its grid that has not started (its index, or -1 where there is none left): CTAs are as many as
+// fit, and what one sets up serves all the tiles it takes. One thread asks; after a refusal it must not ask again.
+__device__ __forceinline__ void ask_next(uint32_t answer, uint32_t bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int next_of(uint32_t answer) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "mov.b32 %0, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n\t"
+        "selp.u32 %1, 1, 0, p;\n\t}"
+        : "=r"(x), "=r"(got)
+        : "r"(answer)
+        : "memory");
+    return got ? (int)x : -1;
+}
+
+// The loop of the warp that hands out tiles. What it hands out are `Work`s of a control block C, found by work_of(tile): n_tok <= 0 is nothing to do,
+// or nothing more. DEALT: tiles blockIdx.x, + gridDim.x, ... of `tiles`. Else as ask_next gives them, each asked for when the last loads of the
+// one before have been issued (`want`): its own follow before the ring of the loads is empty, and no CTA holds a tile that another could begin.
+template <bool DEALT, typename C, typename F>
+__device__ __forceinline__ void hand_out(C* ctl, F&& work_of, int64_t tiles, bool ok, int lane, volatile int* abort_flag, int* status, int code) {
+    int64_t t = blockIdx.x;
+    uint32_t asked = 0;
+    for (int n = 0;;) {
+        auto w = work_of(t);                                 // (t < 0: none)
+        if (lane == 0) ctl->held = w;
+        if (t < 0 || w.n_tok > 0) {
+            ok = ok && mbar_wait_warp(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, abort_flag, status, code);
+            if (ok && lane == 0) {
+                ctl->work[n & 1] = w;
+                ctl->not_finite[n & 1] = 0;
+                mbar_arrive(smem_u32(&ctl->wfull[n & 1]));
+            }
+            __syncwarp();
+            if (t < 0) break;
+            if (!DEALT) ok = ok && mbar_wait_warp(smem_u32(&ctl->want), n & 1, abort_flag, status, code + 1);
+            ++n;
+        }
+        if (!ok) break;
+        if (DEALT) {
+            t = t + gridDim.x < tiles ? t + gridDim.x : -1;
+            continue;
+        }
+        if (lane == 0) ask_next(smem_u32(ctl->answer), smem_u32(&ctl->next));
+        // (also where a wait gave up: what the answer takes from the grid nobody else will do)
+        ok = mbar_wait_warp(smem_u32(&ctl->next), asked & 1, abort_flag, status, code + 2);
+        t = ok || mbar_wait_answer(smem_u32(&ctl->next), asked & 1) ? next_of(smem_u32(ctl->answer)) : -1;
+        ++asked;
+        fence_proxy_async_smem();
+        __syncwarp();
+    }
+}
+
 }  // namespace packed
 }  // namespace es
