@@ -75,8 +75,11 @@ def _check_cache(k_cache, v_cache):
 @N.device_guard
 def store_kv(k, v, k_cache, v_cache, slots):
     """Writes k, v [tokens, kv_heads, D] into the cache: token t at slots[t] (page * page_size + offset). Tokens whose slot is
-    -1, or lies outside the cache, are skipped. The slots of a call are distinct: of two tokens with one slot either may be stored."""
+    -1, or lies outside the cache, are skipped. The slots of a call are distinct: of two tokens with one slot either may be stored. No
+    gradients; autograd knows that the cache has changed, and a graph that had saved it says so in its backward."""
     check_tokens(k, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise RuntimeError("store_kv has no backward: call it under torch.no_grad()")
     P, S, Hk, D = _check_cache(k_cache, v_cache)
     if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (Hk, D):
         raise RuntimeError("k and v must be [tokens, kv_heads, D] with the heads of the cache")
@@ -87,6 +90,7 @@ def store_kv(k, v, k_cache, v_cache, slots):
     k, v = rows(k), rows(v)
     _call("es_store_kv", N.ptr(k), N.ptr(v), N.ptr(k_cache), N.ptr(v_cache), N.ptr(slots), k.shape[0], Hk, D, P, S, *strides(k), *strides(v),
           *strides(k_cache), *strides(v_cache), N.stream_ptr())
+    torch.autograd.graph.increment_version([t for t in (k_cache, v_cache) if not t.is_inference()])
 
 
 @N.device_guard

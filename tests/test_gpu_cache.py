@@ -112,6 +112,31 @@ def test_store_kv(T, Hk, D, page, layout, dtype):
     cache.store_kv(fused[:0, 0], fused[:0, 1], kc, vc, slots[:0])
 
 
+def test_store_kv_and_autograd():
+    """Nothing that takes part in a graph is stored without its gradient, and a graph that saved the cache does not use what has replaced it."""
+    from self_trainable_or_free_attn_b200 import cache
+    kc, vc = (torch.ones(2, 16, 2, 64, dtype=BF, device="cuda") for _ in range(2))
+    k, v, slots = kc[0, :3].clone(), vc[0, :3].clone(), ints([1, 20, 7])
+    for leaf in (k, v, kc, vc):
+        leaf.requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            cache.store_kv(k, v, kc, vc, slots)
+        with torch.no_grad():
+            cache.store_kv(k, v, kc, vc, slots)
+        leaf.requires_grad_(False)
+    w = torch.ones(2, 16, 2, 64, dtype=BF, device="cuda", requires_grad=True)
+    for c in (kc, vc):
+        y = (w * c).sum()
+        cache.store_kv(k, v, kc, vc, slots)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        ki, vi = kc.clone(), vc.clone()
+        cache.store_kv(2 * k, 2 * v, ki, vi, slots)
+        cache.store_kv(2 * k, 2 * v, kc, vc, slots)
+        assert torch.equal(ki, kc) and torch.equal(vi, vc) and float(kc.detach()[1, 4, 0, 0]) == 2
+
+
 # ---------------------------------------------------------------------------------------------- attention
 def _prefix_case(B, N, H, Hk, D, page, prefix, own, dtype, seed=0, layout="plain"):
     g = torch.Generator().manual_seed(seed)
