@@ -3,7 +3,8 @@
 Public names of the reference's package root (echosparse/__init__.py:1-5): `EchoSparseAttention`, `PRESETS`, `enable`.
 `offload_blocks` (weight offload for small GPUs) is outside this library: a B200 holds the models the presets name.
 `kernels.sm100` is the kernel-set module the attention processor calls; the CUDA code lives in `csrc/` behind the C ABI
-declared in `include/echosparse_sm100.h`; `vsa` holds the VSA2 entry points.
+declared in `include/echosparse_sm100.h`; `vsa` holds the VSA2 entry points; `packed` and `cache` hold the attention over
+packed sequences and over a paged cache.
 """
 __version__ = "0.2.0"
 __all__ = ["EchoSparseAttention", "PRESETS", "enable"]

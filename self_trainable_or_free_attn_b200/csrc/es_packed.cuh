@@ -37,16 +37,6 @@ struct Batch {
     __device__ __forceinline__ int k_at(int b) const { return min(max(__ldg(cu_k + b), 0), Tk); }
 };
 
-// The sequence that holds token t of a packed batch, -1 for none: the last one that starts at or before t.
-__device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
-    int lo = 0, hi = B;                                      // the first b with cu[b] > t is in lo .. hi + 1
-    while (lo <= hi) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= t) lo = mid + 1; else hi = mid - 1;
-    }
-    return lo == 0 || lo == B + 1 ? -1 : lo - 1;
-}
-
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }

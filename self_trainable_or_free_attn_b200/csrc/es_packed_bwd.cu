@@ -9,11 +9,16 @@
 // pass instead would save two of seven products, S and dP again, and need dQ added with atomics in the order in which CTAs happen to run.)
 //
 //   warps 0-7  P and dS: a thread has row 32 (warp % 4) + lane and 64 columns, those of warps 4-7 the upper half
-//   warp 8     issues the MMAs; warp 9 issues the TMA loads; warp 10 (dK / dV) brings LSE and delta of the walked rows
+//   warp 8     issues the MMAs; warp 9 issues the TMA loads; warp 10 (dK / dV) brings LSE and delta of the walked rows; the next one
+//              finds out what the CTA does next
 //
 // What a mask hides, or what lies in the walked tile behind the sequence, has P = dS = 0, and 0 times NaN or infinity would be NaN: in tiles
 // that a mask cuts, values of the walked tiles that are not finite are set to 0 in shared memory once S and dP are there. dS is NaN already
 // where they are seen; dV alone gets what is not finite in dO at the end, from global memory.
+//
+// Bound by the chain S -> P -> dP -> dS of an iteration, which one set of 128 x 128 tiles cannot hide: accumulators and scores fill tensor memory, the
+// tiles shared memory. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.89 ms =
+// 1,080 TFLOP/s, dK / dV 1.13 ms = 1,134. A CTA that takes tile after tile saves setting up and tearing down: 3 to 10 % of both passes.
 #include "es_packed_tc.cuh"
 
 namespace es {

@@ -12,6 +12,10 @@ per gradient row: reproducible bit for bit).
 
 Tokens of no sequence (behind the last, say) get output 0, LSE -inf and gradient 0, and what they hold reaches no other row; the same
 is true of keys that the causal mask hides.
+
+Forward and backward can be captured into a CUDA graph, by autograd's rule for captures: warm up on a side stream and drop every
+graph that was recorded eagerly from the same leaves before the capture begins (an eager graph that lives on ties its leaves'
+accumulation to another stream, and a capture that reaches into that stream ends with an error).
 """
 import functools
 import math
