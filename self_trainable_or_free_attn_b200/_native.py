@@ -149,7 +149,7 @@ def device_guard(fn):
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
         import torch
-        for a in args if args else kwargs.values():
+        for a in args or kwargs.values():
             if isinstance(a, torch.Tensor):
                 if a.is_cuda and a.get_device() != torch._C._cuda_getDevice():
                     with torch.cuda.device(a.device):

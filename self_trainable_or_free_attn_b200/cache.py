@@ -19,7 +19,7 @@ import torch
 
 from . import _native as N
 from ._native import check_status  # noqa: F401
-from .packed import _DTYPES, _call, _workspace, check_heads, check_ints, check_tokens, rows, softmax_scale, strides, usable
+from .packed import _DTYPES, _call, _workspace, check_heads, check_ints, check_tokens, empty, lay, softmax_scale, strides, usable
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -87,8 +87,9 @@ def store_kv(k, v, k_cache, v_cache, slots):
     slots, = check_ints(k, slots=slots)
     if slots.shape != (k.shape[0],):
         raise RuntimeError("slots must be [tokens]")
-    k, v = rows(k), rows(v)
-    _call("es_store_kv", N.ptr(k), N.ptr(v), N.ptr(k_cache), N.ptr(v_cache), N.ptr(slots), k.shape[0], Hk, D, P, S, *strides(k), *strides(v),
+    k, rk = lay(k, (Hk * D, D))
+    v, rv = lay(v, (Hk * D, D))
+    _call("es_store_kv", k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), k.shape[0], Hk, D, P, S, *rk, *rv,
           *strides(k_cache), *strides(v_cache), N.stream_ptr())
     torch.autograd.graph.increment_version([t for t in (k_cache, v_cache) if not t.is_inference()])
 
@@ -123,7 +124,7 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
     if table.shape[1] * S > 2 ** 31 - 256 or B * T * H >= 2 ** 31:
         raise RuntimeError("at most 2**31 - 256 tokens to a row of table, and fewer than 2**31 query rows")
     q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-    o = torch.empty(B, T, H, D, device=q.device, dtype=q.dtype)
+    o = empty(q)
     lse = torch.empty(B, H, T, device=q.device, dtype=torch.float32)
     ws = _workspace("es_prefix_workspace_bytes", q, (B, T, H, Hk, D, prefix_len, table.shape[1], S))
     _call("es_prefix_attn", N.ptr(q), N.ptr(k_cache), N.ptr(v_cache), N.ptr(o), N.ptr(lse), N.ptr(prefix_pages), prefix_pages.numel(), prefix_len,

@@ -58,6 +58,20 @@ def strides(t):
     return tuple(reversed(out))
 
 
+def lay(t, whole):
+    """t, or a copy where the kernels cannot read it as it lies, and its strides; `whole`: those of a contiguous one."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, whole
+    if usable(t):
+        return t, strides(t)
+    return t.clone(memory_format=torch.contiguous_format), whole
+
+
+def empty(t):
+    """Memory for a contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def softmax_scale(scale, D):
     if scale is None:
         return 1.0 / math.sqrt(D)
@@ -78,12 +92,13 @@ def check_tokens(ref, **tensors):
     """Every tensor on the CUDA device of `ref` and in its dtype, bf16 or fp16."""
     dev, dtype = ref.get_device(), ref.dtype
     for name, t in tensors.items():
+        if t.is_cuda and t.dtype is dtype and dtype in _DTYPES and t.get_device() == dev:
+            continue
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be a CUDA tensor: this operator has no CPU path")
         if t.get_device() != dev:
             raise RuntimeError(f"{name} must be on {ref.device}, got {t.device}")
-        if t.dtype is not dtype or dtype not in _DTYPES:
-            raise RuntimeError("all of them must share the dtype bfloat16 or float16: " + ", ".join(tensors))
+        raise RuntimeError("all of them must share the dtype bfloat16 or float16: " + ", ".join(tensors))
 
 
 def check_ints(ref, **tensors):
@@ -101,7 +116,7 @@ def check_ints(ref, **tensors):
 
 
 def _call(name, *args):
-    rc = getattr(N.load(), name)(*args)
+    rc = getattr(N._lib or N.load(), name)(*args)
     if rc:
         N.check(rc, name)
 
@@ -120,14 +135,16 @@ def _workspace(name, q, sizes):
 def _fwd(q, k, v, cu_q, cu_k, scale, causal, with_rest):
     T, H, D = q.shape
     Tk, Hk, _ = k.shape
-    device, dtype = q.device, q.dtype
-    o = torch.empty(T, H, D, device=device, dtype=dtype)
-    rest = torch.empty(T, H, D, device=device, dtype=dtype) if with_rest else None
-    lse = torch.empty(H, T, device=device, dtype=torch.float32)
+    q, rq = lay(q, (H * D, D))
+    k, rk = lay(k, (Hk * D, D))
+    v, rv = lay(v, (Hk * D, D))
+    o = empty(q)
+    rest = empty(q) if with_rest else None
+    lse = torch.empty(H, T, device=q.device, dtype=torch.float32)
     sizes = (cu_q.shape[0] - 1, T, Tk, H, Hk, D)
     ws = _workspace("es_packed_fwd_workspace_bytes", q, sizes)
     _call("es_packed_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), N.ptr(rest), lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), *sizes,
-          *strides(q), *strides(k), *strides(v), scale, causal, _DTYPES[dtype], N.ptr(ws), N.stream_ptr())
+          *rq, *rk, *rv, scale, causal, _DTYPES[q.dtype], N.ptr(ws), N.stream_ptr())
     return o, rest, lse
 
 
@@ -148,15 +165,15 @@ class _Function(torch.autograd.Function):
         if dout is None:
             return (None,) * 7
         q, k, v, o, rest, lse, cu_q, cu_k = ctx.saved_tensors
-        dout = rows(dout)
-        sizes = (cu_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2])
+        (T, H, D), (Tk, Hk, _) = q.shape, k.shape
+        dout, rdo = lay(dout, (H * D, D))
+        sizes = (cu_q.shape[0] - 1, T, Tk, H, Hk, D)
         need = ctx.needs_input_grad
-        mk = lambda t: torch.empty(t.shape, device=t.device, dtype=t.dtype)
-        dq = mk(q) if need[0] else None
-        dk, dv = (mk(k), mk(v)) if need[1] or need[2] else (None, None)
+        dq = empty(q) if need[0] else None
+        dk, dv = (empty(k), empty(v)) if need[1] or need[2] else (None, None)
         ws = _workspace("es_packed_bwd_workspace_bytes", q, sizes)
         _call("es_packed_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), N.ptr(dq), N.ptr(dk),
-              N.ptr(dv), cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides(q), *strides(k), *strides(v), *strides(dout), ctx.scale, ctx.causal, _DTYPES[q.dtype],
+              N.ptr(dv), cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides(q), *strides(k), *strides(v), *rdo, ctx.scale, ctx.causal, _DTYPES[q.dtype],
               N.ptr(ws), N.stream_ptr())
         return dq, dk, dv, None, None, None, None
 
@@ -192,5 +209,5 @@ def packed_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, retur
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         o, lse = _Function.apply(rows(q), rows(k), rows(v), cu_q, cu_k, scale, causal)
     else:
-        o, _, lse = _fwd(rows(q), rows(k), rows(v), cu_q, cu_k, scale, causal, False)
+        o, _, lse = _fwd(q, k, v, cu_q, cu_k, scale, causal, False)
     return (o, lse) if return_lse else o
