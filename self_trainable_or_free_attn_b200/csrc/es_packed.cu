@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const uint4* o, const uint4*
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / L;
     float s = 0.f;
     int t = 0, h = 0;
+    launch_dependents();                                     // (the next kernel waits for all of this)
     if (row < (int64_t)Tq * H) {
         t = (int)(row / H);
         h = (int)(row % H);

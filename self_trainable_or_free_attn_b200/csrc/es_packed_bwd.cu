@@ -61,6 +61,7 @@ struct BwdArgs {
     float* part;                                             // their sums: [split][dV, dK][key][head][D]
     const void* dout;                                        // for what is not finite
     int64_t slots;                                           // owner tiles, some of them empty
+    int behind_q;                                            // the dK / dV pass runs behind the dQ pass, not behind the row sums
     Rows rdo;
     int* status;
 };
@@ -189,6 +190,8 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     __syncthreads();
     tc_fence_after();
+    if (!a.behind_q) wait_prerequisites();                   // (the row sums; behind the dQ pass they are there)
+    launch_dependents();
     const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     float* row_lse = reinterpret_cast<float*>(smem + C::ROWS);        // [stage][128]: minus LSE in log2; then minus delta
@@ -510,6 +513,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             }
         }
     }
+    wait_prerequisites();                                    // what comes next waits for this kernel, and so for the dQ pass too
 }
 
 // ---------------------------------------------------------------------------------------------- dQ
@@ -579,6 +583,8 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
     __syncthreads();
     tc_fence_after();
+    wait_prerequisites();                                    // the row sums
+    launch_dependents();
     const uint32_t tmem = uniform(ctl->tmem_base);
     const uint32_t full0 = smem_u32(&ctl->full[0]), empty0 = smem_u32(&ctl->empty[0]);
     bool ok = *abort_flag == 0;
@@ -809,6 +815,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 // dK, dV = the sums of their parts in the order of the CTAs; four values a thread.
 template <typename T> __global__ void __launch_bounds__(256) sum_kernel(const float4* part, T* dk, T* dv, int splits, int64_t n4) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    wait_prerequisites();
     if (i >= 2 * n4) return;
     float4 s = part[i];
     for (int p = 1; p < splits; ++p) {
@@ -856,13 +863,18 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
         if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
         a.d0 = kv ? dk : dq;
         a.d1 = dv;
-        kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, tdo, a);
+        a.behind_q = kv && dq;
+        // either pass may set up while the kernel before it ends, and dK / dV start on the SMs that dQ has left
+        const cudaError_t e = launch_dependent(kern, dim3((unsigned)grid), dim3(THREADS), Cfg<D>::BYTES, st, tq, tk, tv, tdo, a);
+        if (e != cudaSuccess) return set_error(-2, cudaGetErrorString(e));
         ES_CHECK_LAUNCH("packed_bwd_kernel");
     }
     if (dk && a.splits > 1) {
         const int64_t n4 = (int64_t)a.b.Tk * a.b.Hk * D / 4, blocks = (2 * n4 + 255) / 256;
         if (blocks > 0x7FFFFFFF) return set_error(-1, "es_packed_attn_bwd: too many rows");
-        sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(reinterpret_cast<const float4*>(a.part), static_cast<T*>(dk), static_cast<T*>(dv), a.splits, n4);
+        const cudaError_t e = launch_dependent(sum_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, reinterpret_cast<const float4*>(a.part), static_cast<T*>(dk),
+                                               static_cast<T*>(dv), a.splits, n4);
+        if (e != cudaSuccess) return set_error(-2, cudaGetErrorString(e));
         ES_CHECK_LAUNCH("sum_kernel");
     }
     return 0;
