@@ -8,6 +8,9 @@
 // P and dS are written over S and dP in tensor memory, as 16-bit pairs, and are the A operands of the second products from there. (One
 // pass instead would save two of seven products, S and dP again, and need dQ added with atomics in the order in which CTAs happen to run.)
 //
+// Tiles with rows that see few keys multiply what these roundings left as well, from the tensor memory that S and dP no longer need: there
+// they do not average out, neither in P and dS nor in the forward's O, which delta is summed from.
+//
 //   warps 0-7  P and dS: a thread has row 32 (warp % 4) + lane and 64 columns, those of warps 4-7 the upper half
 //   warp 8     issues the MMAs; warp 9 issues the TMA loads; warp 10 (dK / dV) brings LSE and delta of the walked rows; the next one
 //              finds out what the CTA does next
@@ -20,6 +23,8 @@
 // tiles shared memory. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.89 ms =
 // 1,080 TFLOP/s, dK / dV 1.13 ms = 1,134. A CTA that takes tile after tile saves setting up and tearing down: 3 to 10 % of both passes.
 #include "es_packed_tc.cuh"
+
+#include <climits>
 
 namespace es {
 namespace packed {
@@ -41,7 +46,7 @@ struct Work {
     int nt;              // walked tiles
     int head, split;     // key head; dQ: first query head
     int from, per, tile0;        // dK / dV: first query that sees one of the keys, tiles from it to the end, the first of them in this split
-    int ones;            // dK / dV: see below
+    int ones, fine;      // see below
 };
 struct Ctl {
     uint64_t yfull, yempty, full[10], empty[10], sfull[2], dpfull, pfull, dsfull, rfull[2], rempty[2], gfull, drain, wfull[2], wempty[2], want, next;
@@ -129,6 +134,9 @@ __device__ __forceinline__ Work kv_work(const BwdArgs& a, int64_t t, int lane) {
     // Rows that see one key: their P is 1 whatever the logit, and dS is 0 and not what rounding leaves of a difference (where it is a number). They
     // are the first columns of the first walked tile in causal attention, all rows (more than TM) where the sequence has one key.
     w.ones = at.length == 1 ? TM + 1 : a.b.causal && at.offset == 0 && w.nw >= at.length ? a.pack : 0;
+    // Walked tiles that start at query `fine` or before have rows that see few keys, all of them in this tile. What rounding their P and dS left is
+    // multiplied as well: such roundings do not average out (es_packed_fwd.cu).
+    w.fine = at.offset > 0 ? -1 : a.b.causal ? FEW - 1 - w.diag : at.length <= FEW ? INT_MAX : -1;
     return w;
 }
 
@@ -210,6 +218,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint32_t issued = 0, owners = 0;
     // walked tile i: query heads head0 .., first token
     auto head_of = [&](const Work& w, int i) { return w.head * a.b.G + (w.tile0 + i) / w.per * a.pack; };
+    auto is_fine = [&](const Work& w, int t0) { return t0 <= w.fine; };
     auto token_of = [&](const Work& w, int i) { return w.from + (w.tile0 + i) % w.per * a.tokens; };
 
     if (warp >= 8) {
@@ -309,7 +318,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 }
                 __syncwarp();
             };
-            auto second_product = [&](int x, uint32_t i, uint32_t more) {        // x = 0: dK += dS^T Q, x = 1: dV += P^T dO
+            auto second_product = [&](int x, uint32_t i, uint32_t more, bool fine) {     // x = 0: dK += dS^T Q, x = 1: dV += P^T dO
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t xb = x_lo + ((base + C::RING + slot_of(2 * i + x) * C::TILE) >> 4), p = tmem + (x ? 0u : DP_COL);
@@ -317,6 +326,10 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     for (int ks = 0; ks < 8; ++ks)
                         umma_ts_lohi(tmem + (x ? DV_COL : DK_COL), p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G,
                                      ks > 0 ? 1u : more);
+                    if (fine)
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            umma_ts_lohi(tmem + (x ? DV_COL : DK_COL), p + 32 + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, 1u);
                     umma_commit(empty0 + 8 * slot_of(2 * i + x));
                 }
                 __syncwarp();
@@ -330,14 +343,18 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 ++tiles;
                 if (ok) first_product(0, done, false);
                 if (ok) first_product(1, done, nt == 1);
+                const int stop = w.from + w.per * a.tokens;
+                int t0 = token_of(w, 0);
                 for (int i = 0; i < nt && ok; ++i, ++done) {
+                    const bool fine = uniform((int)is_fine(w, t0));
+                    t0 = t0 + a.tokens < stop ? t0 + a.tokens : w.from;
                     ok = mbar_wait_warp(smem_u32(&ctl->pfull), done & 1, abort_flag, a.status, 625);
                     if (!ok) break;
-                    second_product(1, done, i > 0);
+                    second_product(1, done, i > 0, fine);
                     if (i + 1 < nt) first_product(0, done + 1, false);           // (over P, which dV has read: MMAs run in their order)
                     ok = ok && mbar_wait_warp(smem_u32(&ctl->dsfull), done & 1, abort_flag, a.status, 626);
                     if (!ok) break;
-                    second_product(0, done, i > 0);
+                    second_product(0, done, i > 0, fine);
                     if (i + 1 < nt) first_product(1, done + 1, i + 2 == nt);
                 }
                 if (ok && elect_one()) umma_commit(smem_u32(&ctl->gfull));
@@ -357,12 +374,12 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         uint32_t done = 0, tiles = 0;                        // walked tiles and owners before this work
         Work w;
         for (int n = 0; enter(n, w); ++n) {
-        const int nt = w.nt, nw = w.nw, diag = w.diag, first = w.from, stop = first + w.per * a.tokens, last = w.n_tok - 1, ones = w.ones;
+        const int nt = w.nt, nw = w.nw, diag = w.diag, first = w.from, stop = first + w.per * a.tokens, last = w.n_tok - 1, ones = w.ones, fine_to = w.fine;
         int t0 = nt > 0 ? token_of(w, 0) : 0;
         for (int i = 0; i < nt && ok; ++i, ++done) {
             const uint32_t stage = done % C::NROW;
             // the first of the tile's tokens sees the fewest keys; the rows behind the last token are of other sequences
-            const bool cut = t0 + diag < last, masked = cut || t0 + a.tokens > nw;
+            const bool cut = t0 + diag < last, masked = cut || t0 + a.tokens > nw, fine = t0 <= fine_to;
             ok = mbar_wait_warp(smem_u32(&ctl->rfull[stage]), (done / C::NROW) & 1, abort_flag, a.status, 628) &&
                  mbar_wait_warp(smem_u32(&ctl->sfull[0]), done & 1, abort_flag, a.status, 629);
             if (!ok) break;
@@ -410,6 +427,18 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             } else {
                 probabilities(std::false_type{});
             }
+            if (fine) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t rest[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float p0 = __uint_as_float(x[32 * h + 2 * j]), p1 = __uint_as_float(x[32 * h + 2 * j + 1]);
+                        rest[j] = rest2<T>(p0, p1, pack2<T>(p0, p1));
+                    }
+                    tmem_st16(scol + 32 + 16 * h, rest);
+                }
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -422,12 +451,39 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             ok = mbar_wait_warp(smem_u32(&ctl->dpfull), done & 1, abort_flag, a.status, 631);
             if (!ok) break;
             tc_fence_after();
+            const float4* rd = reinterpret_cast<const float4*>(row_delta + stage * TM + 64 * ch);
+            if (fine) {
+                // in halves: dS over dP where that has been read
+                uint32_t y[64];
+                tmem_ld32(dpcol, y);
+                tmem_ld32(dpcol + 32, y + 32);
+                tmem_wait_ld_regs(y);
+                tmem_wait_ld_regs(y + 32);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t ds[16], rest[16];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float4 z = rd[8 * h + j / 4];
+                        const float nd = j % 4 == 0 ? z.x : j % 4 == 1 ? z.y : j % 4 == 2 ? z.z : z.w;
+                        const float g = __uint_as_float(x[32 * h + j]) * (__uint_as_float(y[32 * h + j]) + nd);
+                        y[32 * h + j] = 32 * h + j < lim || 32 * h + j >= end ? 0u : __float_as_uint(g);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float g0 = __uint_as_float(y[32 * h + 2 * j]), g1 = __uint_as_float(y[32 * h + 2 * j + 1]);
+                        ds[j] = pack2<T>(g0, g1);
+                        rest[j] = rest2<T>(g0, g1, ds[j]);
+                    }
+                    tmem_st16(dpcol + 16 * h, ds);
+                    tmem_st16(dpcol + 32 + 16 * h, rest);
+                }
+            } else {
             uint32_t y[64];
             tmem_ld32(dpcol, y);
             tmem_ld32(dpcol + 32, y + 32);
             tmem_wait_ld_regs(y);
             tmem_wait_ld_regs(y + 32);
-            const float4* rd = reinterpret_cast<const float4*>(row_delta + stage * TM + 64 * ch);
             auto differences = [&](auto cut_tile) {
                 uint32_t ds[32];
 #pragma unroll
@@ -450,6 +506,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             };
             if (masked) differences(std::true_type{});
             else differences(std::false_type{});
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -531,7 +588,9 @@ __device__ __forceinline__ Work q_work(const BwdArgs& a, int64_t t, int lane) {
     w.nw = max(a.b.k_at(at.seq + 1) - w.w0, 0);
     w.diag = w.nw - at.length + at.offset;
     const int last = at.n - 1;
+    // (rows that see few keys, see kv_work; one walked tile)
     w.nt = ((a.b.causal ? min(max(last + w.diag + 1, 0), w.nw) : w.nw) + TN - 1) / TN;
+    w.fine = w.nt == 1 && (a.b.causal ? w.diag + 1 : w.nw) <= FEW;
     return w;
 }
 
@@ -690,6 +749,10 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks)
                             umma_ts_lohi(tmem + DQ_COL, p + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, (i > 0 || ks > 0) ? 1u : 0u);
+                        if (w.fine)
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                umma_ts_lohi(tmem + DQ_COL, p + 32 + (ks < 4 ? ks * 8 : 64 + (ks - 4) * 8), xb + ((ks * 2048) >> 4), x_hi, ID_G, 1u);
                         umma_commit(empty0 + 8 * slot_of(2 * done));
                         if (i + 1 == nt) umma_commit(smem_u32(&ctl->gfull));
                     }
@@ -752,6 +815,29 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             ok = mbar_wait_warp(smem_u32(&ctl->dpfull), done & 1, abort_flag, a.status, 651);
             if (!ok) break;
             tc_fence_after();
+            if (w.fine) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t y[32], ds[16], rest[16];
+                    tmem_ld32(dpcol + 32 * h, y);
+                    tmem_wait_ld_regs(y);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float g[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int k = 32 * h + 2 * j + e;
+                            g[e] = k >= lim ? 0.f : __uint_as_float(x[k]) * (__uint_as_float(y[2 * j + e]) - delta);
+                        }
+                        // (a row that sees one key: P is 1 whatever the logit, and dS is 0 and not what rounding leaves; NaN stays)
+                        if (h == 0 && j == 0 && vis == 1 && g[0] == g[0]) g[0] = 0.f;
+                        ds[j] = pack2<T>(g[0], g[1]);
+                        rest[j] = rest2<T>(g[0], g[1], ds[j]);
+                    }
+                    tmem_st16(scol + 16 * h, ds);
+                    tmem_st16(scol + 32 + 16 * h, rest);
+                }
+            } else {
             uint32_t y[64];
             tmem_ld32(dpcol, y);
             tmem_ld32(dpcol + 32, y + 32);
@@ -775,6 +861,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             };
             if (masked) differences(std::true_type{});
             else differences(std::false_type{});
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();

@@ -74,6 +74,10 @@ struct FwdArgs {
 };
 
 __device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
+// Whether row tile s is one of training with rows that see few keys (and one tile of keys in all): what rounding P left is multiplied with V as
+// well. delta = rowsum(dO o O) stands against sums over these few keys, where P's roundings do not average out: dQ and dK of short sequences
+// were off by up to 1.7 times what their own rounding is, and are by 1.0 to 1.4 times with it (and with the same of the backward's P and dS).
+__device__ __forceinline__ bool is_fine(const FwdArgs& a, const Work& w, int s) { return w.i0 == 0 && w.end(s) == 1 && seen_by(a, w, s * a.tokens) <= FEW; }
 }  // namespace
 
 // The grid's tile t: split and heads go fastest, and the last tiles of a causal sequence, which see the most keys, first.
@@ -109,7 +113,8 @@ template <bool PAGED> __device__ __forceinline__ Work work_of(const FwdArgs& a, 
     return w;
 }
 
-template <typename T, int D, bool PAGED>
+// FINE: in training.
+template <typename T, int D, bool PAGED, bool FINE>
 __global__ void __launch_bounds__(THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ FwdArgs a) {
@@ -290,6 +295,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                             for (int ks = 0; ks < 8; ++ks)
                                 umma_ts_lohi(tmem + O_COL + s * D, tmem + s * 128 + ks * 8, vb + ((ks * 2048) >> 4), v_hi, ID_PV, (i > 0 || ks > 0) ? 1u : 0u);
+                            if (FINE && is_fine(a, w, s))
+#pragma unroll
+                                for (int ks = 0; ks < 8; ++ks)
+                                    umma_ts_lohi(tmem + O_COL + s * D, tmem + s * 128 + 64 + ks * 8, vb + ((ks * 2048) >> 4), v_hi, ID_PV, 1u);
                             if (left == 1) umma_commit(smem_u32(&ctl->ofull[s]));
                             if (last) umma_commit(empty0 + 8 * slot_of(vseq));
                             if (left > 1) {
@@ -346,6 +355,44 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (!ok) break;
                 ++products;
                 tc_fence_after();
+                if (FINE && is_fine(a, w, s)) {
+                    // the only tile of these rows, in quarters. (Apart from the rest: its registers are all taken.)
+                    const int lim = vis - i * TN;
+                    auto quarter = [&](int h, uint32_t* x) {
+                        tmem_ld32(scol + 32 * h, x);
+                        tmem_wait_ld_regs(x);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * h + j >= lim) x[j] = 0xff800000u;
+                    };
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t x[32];
+                        quarter(h, x);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+                    }
+                    m = top * c;
+                    const float off = m == -INFINITY ? 0.f : -m;
+                    uint32_t p[64];
+                    // from the last to the first: what is left goes where S has been read, P over S when all of it has
+#pragma unroll
+                    for (int h = 3; h >= 0; --h) {
+                        uint32_t x[32], rest[16];
+                        quarter(h, x);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float e0 = ex2_approx(__uint_as_float(x[2 * j]) * c + off), e1 = ex2_approx(__uint_as_float(x[2 * j + 1]) * c + off);
+                            l += e0 + e1;
+                            p[16 * h + j] = pack2<T>(e0, e1);
+                            rest[j] = rest2<T>(e0, e1, p[16 * h + j]);
+                        }
+                        tmem_st16(scol + 64 + 16 * h, rest);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) tmem_st16(scol + 16 * h, p + 16 * h);
+                } else {
                 uint32_t x[128];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) tmem_ld32(scol + 32 * j, x + 32 * j);
@@ -404,6 +451,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                     tmem_st16(scol + 16 * h, p);
                 }
                 l += sum.x + sum.y;
+                }
                 if (i >= whole) {
                     // V rows that some rows of the tile may not see
                     const uint32_t vseq = first + 2 * (i - w.i0) + 1, slot = vseq % C::NSLOT;
@@ -567,7 +615,7 @@ static int launch(const void* q, Rows rq, const void* k, Rows rk, const void* v,
     if (int rc = make_rows_map<T>(&tq, q, D, a.b.H, a.b.Tq, rq, a.pack, a.tokens)) return rc;
     if (int rc = make_rows_map<T>(&tk, k, D, a.b.Hk, tk_rows, rk, 1, TN)) return rc;
     if (int rc = make_rows_map<T>(&tv, v, D, a.b.Hk, tk_rows, rv, 1, TN)) return rc;
-    auto kern = packed_fwd_kernel<T, D, false>;
+    auto kern = a.o_rest ? packed_fwd_kernel<T, D, false, true> : packed_fwd_kernel<T, D, false, false>;
     if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
     a.slots = piece_slots(a.b.Tq, 2 * a.tokens, a.b.B);
     const int64_t grid = (int64_t)a.vheads * a.splits * a.slots;
@@ -636,7 +684,7 @@ static int launch_prefix(const void* q, const void* k, CacheRows rk, const void*
     if (int rc = make_pages_map<T>(&tv, v, D, a.b.Hk, 1 << a.log_page, a.pages, rv, TN)) return rc;
     a.slots = (int64_t)a.vheads * a.splits * ((a.b.Tq + 2 * a.tokens - 1) / (2 * a.tokens));
     const int64_t grid = std::min<int64_t>(a.slots, sm_count());
-    auto kern = packed_fwd_kernel<T, D, true>;
+    auto kern = packed_fwd_kernel<T, D, true, false>;
     if (int rc = opt_in_shared_memory((const void*)kern, (int)Cfg<D>::BYTES)) return rc;
     kern<<<(unsigned)grid, THREADS, Cfg<D>::BYTES, st>>>(tq, tk, tv, a);
     ES_CHECK_LAUNCH("packed_fwd_kernel (paged)");

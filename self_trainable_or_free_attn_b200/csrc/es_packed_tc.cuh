@@ -15,6 +15,7 @@ using vsa::kNaN32;
 constexpr int TM = 128, TN = 128, THREADS = 384;
 // Registers per thread: 168 at launch (three warps to a quarter of the SM), shared out anew: 224 + 224 + 56 = 3 * 168.
 constexpr int REGS_MATH = 224, REGS_REST = 56;
+constexpr int FEW = 32;                                      // keys of a row (see is_fine, es_packed_fwd.cu)
 constexpr uint32_t HALF = TM * 128;                          // 128 rows x 64 d, one swizzled box
 
 // A value that all lanes have, said so: what is computed from it stays in the registers of the whole warp, where the MMA instructions want their
