@@ -20,8 +20,8 @@
 // where they are seen; dV alone gets what is not finite in dO at the end, from global memory.
 //
 // Bound by the chain S -> P -> dP -> dS of an iteration, which one set of 128 x 128 tiles cannot hide: accumulators and scores fill tensor memory, the
-// tiles shared memory. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.89 ms =
-// 1,080 TFLOP/s, dK / dV 1.13 ms = 1,134. A CTA that takes tile after tile saves setting up and tearing down: 3 to 10 % of both passes.
+// tiles shared memory. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.91 ms =
+// 1,060 TFLOP/s, dK / dV 1.18 ms = 1,090. A CTA that takes tile after tile saves setting up and tearing down: 3 to 10 % of both passes.
 #include "es_packed_tc.cuh"
 
 #include <climits>
