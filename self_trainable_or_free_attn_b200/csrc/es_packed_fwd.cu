@@ -16,8 +16,8 @@
 // itself): O, in tensor memory, is then rescaled by the row's own thread.
 //
 // What is hidden must not reach the row, but P = 0 times NaN or infinity is NaN. In the iterations that a mask cuts (the diagonal, the end of the
-// keys) the softmax warps therefore look through V in shared memory; what is not finite is set to 0 there and added at the end, from global
-// memory, to the rows that do see it.
+// keys) the softmax warps of one row tile therefore look through V in shared memory; what is not finite is set to 0 there and added at the end, from
+// global memory, to the rows that do see it.
 //
 // Bound by the exponentials and what surrounds them: an iteration (two tiles, 128 keys) takes 3,430 clocks, of which its MMAs are 2,051. Of a tile's
 // turn, 1,870 are softmax, 300 the way from P to the MMA warp, 1,065 the two products, 195 the way back; polynomial exponentials on the FMA
@@ -452,8 +452,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 l += sum.x + sum.y;
                 }
-                if (i >= whole) {
-                    // V rows that some rows of the tile may not see
+                if (i >= whole && (s == 0 || i >= w.end0)) {
+                    // V rows that some rows of the tile may not see. One owner for both row tiles: tile 0 where it has these keys (it is cut wherever tile 1
+                    // is), and its P is waited for before either product is issued
                     const uint32_t vseq = first + 2 * (i - w.i0) + 1, slot = vseq % C::NSLOT;
                     ok = mbar_wait_warp(full0 + 8 * slot, (vseq / C::NSLOT) & 1, abort_flag, a.status, 608);
                     if (!ok) break;
