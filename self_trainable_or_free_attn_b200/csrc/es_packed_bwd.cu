@@ -53,6 +53,7 @@ struct Ctl {
     alignas(16) uint32_t answer[4];
     uint32_t tmem_base;
     int abort, not_finite[2];
+    volatile uint32_t moved[2];  // see mbar_wait_moving
     Work work[2], held;          // held: the last one taken, which a wait that gave up may have kept from being handed on
 };
 static_assert(sizeof(Ctl) <= 768, "control block");
@@ -169,6 +170,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             ctl->work[i].n_tok = 0;
         }
         ctl->held.n_tok = 0;
+        ctl->moved[0] = ctl->moved[1] = 0;
         mbar_init(smem_u32(&ctl->want), 1);
         mbar_init(smem_u32(&ctl->dpfull), 1);
         mbar_init(smem_u32(&ctl->pfull), 8);
@@ -207,7 +209,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = *abort_flag == 0;
     // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
     auto enter = [&](int n, Work& w) {
-        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        ok = ok && mbar_wait_moving(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, ctl->moved, abort_flag, a.status, 610);
         if (ok) w = ctl->work[n & 1];
         return ok && w.n_tok > 0;
     };
@@ -260,6 +262,7 @@ packed_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         }
                         __syncwarp();
                         ++issued;
+                        if (lane == 0) ctl->moved[0] = issued;
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
                 }
@@ -623,6 +626,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             ctl->work[i].n_tok = 0;
         }
         ctl->held.n_tok = 0;
+        ctl->moved[0] = ctl->moved[1] = 0;
         mbar_init(smem_u32(&ctl->want), 1);
         mbar_init(smem_u32(&ctl->dpfull), 1);
         mbar_init(smem_u32(&ctl->pfull), 8);
@@ -649,7 +653,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     bool ok = *abort_flag == 0;
     // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
     auto enter = [&](int n, Work& w) {
-        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        ok = ok && mbar_wait_moving(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, ctl->moved, abort_flag, a.status, 610);
         if (ok) w = ctl->work[n & 1];
         return ok && w.n_tok > 0;
     };
@@ -698,6 +702,7 @@ packed_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                         }
                         __syncwarp();
                         ++issued;
+                        if (lane == 0) ctl->moved[0] = issued;
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->want));

@@ -51,6 +51,7 @@ struct Ctl {
     alignas(16) uint32_t answer[4];
     uint32_t tmem_base;
     int abort, not_finite[2];
+    volatile uint32_t moved[2];  // see mbar_wait_moving
     Work work[2], held;          // held: the last one taken, which a wait that gave up may have kept from being handed on
 };
 static_assert(sizeof(Ctl) <= 768, "control block");
@@ -147,6 +148,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         mbar_init(smem_u32(&ctl->next), 1);
         mbar_init(smem_u32(&ctl->want), 1);
         ctl->held.n_tok = 0;
+        ctl->moved[0] = ctl->moved[1] = 0;
         ctl->abort = (base & 1023u) || earlier ? 1 : 0;      // the swizzled tiles need a 1024-byte aligned base
         if (base & 1023u) atomicCAS(a.status, 0, 910);
         mbar_fence_init();
@@ -164,7 +166,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool ok = *abort_flag == 0;
     // the CTA's n-th tile, for the warps that work on it; `leave` once they have read all they need of it
     auto enter = [&](int n, Work& w) {
-        ok = ok && mbar_wait_warp(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, abort_flag, a.status, 610);
+        ok = ok && mbar_wait_moving(smem_u32(&ctl->wfull[n & 1]), (n >> 1) & 1, ctl->moved, abort_flag, a.status, 610);
         if (ok) w = ctl->work[n & 1];
         return ok && w.n_tok > 0;
     };
@@ -229,6 +231,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                 tma_load_4d(dst + d * HALF + lane * box * 128, x ? &tmV : &tmK, bar, 64 * d, kh, (i * TN) & ((1 << a.log_page) - 1), page);
                         __syncwarp();
                         ++issued;
+                        if (lane == 0) ctl->moved[0] = issued;
                         if (++slot == C::NSLOT) { slot = 0; par ^= 1; }
                     }
                 }

@@ -157,6 +157,39 @@ template <int N> __device__ __forceinline__ void load_floats(const float* src, f
     }
 }
 
+// The wait of a warp for what may be a whole walk away (a tile's end, or the next tile of the grid that has work; either grows with the input), where
+// those inside a walk are an iteration away. Its limit counts from the last time the CTA got on: moved[0] counts the tiles loaded, moved[1] the
+// grid's tiles looked at.
+__device__ __forceinline__ bool mbar_wait_moving(uint32_t bar, uint32_t parity, volatile uint32_t* moved, volatile int* abort_flag, int* status, int code) {
+    bool there = mbar_test_wait(bar, parity) || mbar_try_wait(bar, parity);
+    if (!there) {
+        uint32_t polls = 0, late = 0, seen = moved[0] + moved[1];
+        int64_t t0 = (int64_t)global_timer_ns();
+        while (!(there = mbar_try_wait(bar, parity))) {
+            if ((++polls & 63u) != 0) continue;
+            if (*abort_flag) break;
+            if (*reinterpret_cast<volatile int*>(status) != 0) {
+                *abort_flag = 1;
+                break;
+            }
+            const uint32_t now = moved[0] + moved[1];
+            if (now != seen) {
+                seen = now;
+                t0 = (int64_t)global_timer_ns();
+                late = 0;
+                continue;
+            }
+            late = (int64_t)global_timer_ns() - t0 > (int64_t)kWaitLimitNs ? late + 1 : 0;       // (two in a row: see mbar_wait)
+            if (late >= 2) {
+                *abort_flag = 1;
+                atomicCAS(status, 0, code + 1000 * (int)(blockIdx.x % 100000));
+                break;
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, there) != 0;
+}
+
 // After a wait has given up, whether an answer on its way to shared memory has come (100 us at most).
 __device__ __forceinline__ bool mbar_wait_answer(uint32_t bar, uint32_t parity) {
     const uint64_t t_end = global_timer_ns() + 100000ull;
@@ -225,12 +258,15 @@ __device__ __forceinline__ int next_of(uint32_t answer) {
 template <bool DEALT, typename C, typename F>
 __device__ __forceinline__ void hand_out(C* ctl, F&& work_of, int64_t tiles, bool ok, int lane, volatile int* abort_flag, int* status, int code) {
     int64_t t = blockIdx.x;
-    uint32_t asked = 0;
+    uint32_t asked = 0, looked = 0;
     for (int n = 0;;) {
         auto w = work_of(t);                                 // (t < 0: none)
-        if (lane == 0) ctl->held = w;
+        if (lane == 0) {
+            ctl->held = w;
+            ctl->moved[1] = ++looked;
+        }
         if (t < 0 || w.n_tok > 0) {
-            ok = ok && mbar_wait_warp(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, abort_flag, status, code);
+            ok = ok && mbar_wait_moving(smem_u32(&ctl->wempty[n & 1]), ((n >> 1) & 1) ^ 1, ctl->moved, abort_flag, status, code);
             if (ok && lane == 0) {
                 ctl->work[n & 1] = w;
                 ctl->not_finite[n & 1] = 0;
@@ -238,7 +274,7 @@ __device__ __forceinline__ void hand_out(C* ctl, F&& work_of, int64_t tiles, boo
             }
             __syncwarp();
             if (t < 0) break;
-            if (!DEALT) ok = ok && mbar_wait_warp(smem_u32(&ctl->want), n & 1, abort_flag, status, code + 1);
+            if (!DEALT) ok = ok && mbar_wait_moving(smem_u32(&ctl->want), n & 1, ctl->moved, abort_flag, status, code + 1);
             ++n;
         }
         if (!ok) break;

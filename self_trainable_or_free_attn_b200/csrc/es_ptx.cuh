@@ -60,8 +60,8 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Wait limit of every barrier wait in this library: far above any legitimate wait (a CTA lives for well under a
-// second), short enough that a stuck pipeline returns quickly.
+// Wait limit of every barrier wait in this library: far above any legitimate wait (a stage of a pipeline, microseconds; what may be a whole walk
+// away is waited for by mbar_wait_moving, es_packed_tc.cuh), short enough that a stuck pipeline returns quickly.
 constexpr uint64_t kWaitLimitNs = 500000000ull;
 
 // Bounded wait. `abort_flag` (shared memory) is set by the first wait of the CTA that gives up; later waits return at
