@@ -179,6 +179,8 @@ extern "C" int es_extend_tables(const int32_t* lengths, const int32_t* new_token
     if (!cu_new || !taken || (batch && (!lengths || !new_tokens || !lengths_out)) || (batch && table_width && !table) || (n_free && !free_pages) ||
         (total && (!slots || !positions)))
         return set_error(-1, "es_extend_tables: null pointer");
+    if (!aligned(4, lengths, new_tokens, table, free_pages, slots, positions, cu_new, lengths_out, taken))
+        return set_error(-1, "es_extend_tables: the int32 arrays must be 4-byte aligned");
     const PlanArgs a{lengths, new_tokens, free_pages, table, slots, positions, cu_new, lengths_out, taken, n_free, batch, table_width, page_size, total};
     const unsigned grid = (unsigned)std::max<int64_t>(1, ((int64_t)total + PLAN_TOKENS - 1) / PLAN_TOKENS);
     extend_tables_kernel<<<grid, PLAN_THREADS, 0, (cudaStream_t)stream>>>(a);
@@ -193,7 +195,7 @@ extern "C" int es_store_kv(const void* k, const void* v, void* k_cache, void* v_
     if (pages < 0 || page_size < 1 || (int64_t)pages * page_size > 0x7FFFFFFF) return set_error(-1, "es_store_kv: sizes out of range");
     if (total == 0 || pages == 0) return 0;
     if (!k || !v || !k_cache || !v_cache || !slots) return set_error(-1, "es_store_kv: null pointer");
-    if (!aligned(16, k, v, k_cache, v_cache)) return set_error(-1, "es_store_kv: k, v, k_cache, v_cache must be 16-byte aligned");
+    if (!aligned(16, k, v, k_cache, v_cache) || !aligned(4, slots)) return set_error(-1, "es_store_kv: k, v, k_cache, v_cache must be 16-byte, slots 4-byte aligned");
     if (!whole_chunks(k_token, k_head, v_token, v_head, kc_page, kc_token, kc_head, vc_page, vc_token, vc_head))
         return set_error(-1, "es_store_kv: strides must be multiples of 8 elements");
     const StoreArgs a{(const uint4*)k, (const uint4*)v, (uint4*)k_cache, (uint4*)v_cache, slots, {k_token / 8, k_head / 8}, {v_token / 8, v_head / 8},

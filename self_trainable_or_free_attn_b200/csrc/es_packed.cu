@@ -70,8 +70,8 @@ extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, v
     if (total_q == 0) return 0;
     if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v)) || (!workspace && packed_fwd_workspace(batch, total_q, total_k, heads, kv_heads, D)))
         return set_error(-1, "es_packed_attn_fwd: null pointer");
-    if (!aligned(16, q, k, v) || !aligned(32, o, o_rest, workspace))
-        return set_error(-1, "es_packed_attn_fwd: q, k, v must be 16-byte, o, o_rest and the workspace 32-byte aligned");
+    if (!aligned(16, q, k, v) || !aligned(32, o, o_rest, workspace) || !aligned(4, lse, cu_q, cu_k))
+        return set_error(-1, "es_packed_attn_fwd: q, k, v must be 16-byte, o, o_rest and the workspace 32-byte, lse, cu_q, cu_k 4-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head)) return set_error(-1, "es_packed_attn_fwd: strides must be multiples of 8 elements");
     const Batch b{cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, heads / kv_heads, scale, causal};
     return packed_fwd_tc(q, {q_token, q_head}, k, {k_token, k_head}, v, {v_token, v_head}, o, o_rest, lse, b, D, dtype, workspace, (cudaStream_t)stream);
@@ -98,8 +98,8 @@ extern "C" int es_packed_attn_bwd(const void* q, const void* k, const void* v, c
     if (!cu_q || !cu_k || (total_q && (!q || !o || !dout || !lse || !workspace)) || (total_k && (!k || !v)) ||
         (!workspace && packed_bwd_workspace(batch, total_q, total_k, heads, kv_heads, D)))
         return set_error(-1, "es_packed_attn_bwd: null pointer");
-    if (!aligned(16, q, k, v, o, o_rest, dout) || !aligned(32, dq, dk, dv, workspace))
-        return set_error(-1, "es_packed_attn_bwd: q, k, v, o, o_rest, dout must be 16-byte, dq, dk, dv and the workspace 32-byte aligned");
+    if (!aligned(16, q, k, v, o, o_rest, dout) || !aligned(32, dq, dk, dv, workspace) || !aligned(4, lse, cu_q, cu_k))
+        return set_error(-1, "es_packed_attn_bwd: q, k, v, o, o_rest, dout must be 16-byte, dq, dk, dv and the workspace 32-byte, lse, cu_q, cu_k 4-byte aligned");
     if (!whole_chunks(q_token, q_head, k_token, k_head, v_token, v_head, do_token, do_head))
         return set_error(-1, "es_packed_attn_bwd: strides must be multiples of 8 elements");
     const cudaStream_t st = (cudaStream_t)stream;

@@ -657,7 +657,8 @@ extern "C" int es_prefix_attn(const void* q, const void* k_cache, const void* v_
     if (batch == 0 || tokens == 0) return 0;
     if (!q || !o || !lse || !lengths || (prefix_len && !prefix_pages) || (table_width && !table) || (pages && (!k_cache || !v_cache)))
         return set_error(-1, "es_prefix_attn: null pointer");
-    if (!aligned(16, q, k_cache, v_cache, o, workspace)) return set_error(-1, "es_prefix_attn: q, k_cache, v_cache, o, workspace must be 16-byte aligned");
+    if (!aligned(16, q, k_cache, v_cache, o) || !aligned(32, workspace) || !aligned(4, lse, prefix_pages, table, lengths))
+        return set_error(-1, "es_prefix_attn: q, k_cache, v_cache, o must be 16-byte, the workspace 32-byte, lse and the int32 arrays 4-byte aligned");
     if (!whole_chunks(k_page, k_token, k_head, v_page, v_token, v_head)) return set_error(-1, "es_prefix_attn: strides must be multiples of 8 elements");
     if (pages == 0) prefix_len = table_width = 0;             // no key can be attended to
     const Plan p = make_plan(batch, tokens, heads, kv_heads, D, prefix_len, table_width);
