@@ -21,6 +21,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -89,7 +90,12 @@ def check_heads(q_heads, kv_heads, D):
 
 
 def check_tokens(ref, **tensors):
-    """Every tensor on the CUDA device of `ref` and in its dtype, bf16 or fp16."""
+    """Every tensor on the CUDA device of `ref` and in its dtype, bf16 or fp16, and none with a tangent: the kernels compute no forward-mode
+    derivatives, and would take a dual tensor for its value."""
+    if forward_ad._current_level >= 0:                       # (inside torch.autograd.forward_ad.dual_level)
+        for name, t in tensors.items():
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} carries a tangent: this operator has no forward-mode derivative")
     dev, dtype = ref.get_device(), ref.dtype
     for name, t in tensors.items():
         if t.is_cuda and t.dtype is dtype and dtype in _DTYPES and t.get_device() == dev:
