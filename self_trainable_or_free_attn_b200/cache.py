@@ -51,8 +51,8 @@ def extend_tables(lengths, new_tokens, table, free_pages, page_size, *, total):
     if lengths.shape != (B,) or new_tokens.shape != (B,) or free_pages.dim() != 1:
         raise RuntimeError("lengths and new_tokens must be [batch] like the rows of table, free_pages [pages]")
     page_size, total = int(page_size), int(total)
-    if page_size < 1:
-        raise ValueError(f"page_size must be at least 1, got {page_size}")
+    if not 1 <= page_size < 2 ** 31:
+        raise ValueError(f"page_size must be at least 1 and below 2**31, got {page_size}")
     if not 0 <= total < 2 ** 31:
         raise ValueError(f"total must be 0 or more, got {total}")
     plan = CachePlan(*torch.empty(2 * total + 2 * B + 3, device=table.device, dtype=torch.int32).split_with_sizes((total, total, B + 1, B, 2)))
@@ -121,6 +121,8 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
     prefix_len = int(prefix_len)
     if not 0 <= prefix_len <= prefix_pages.numel() * S:
         raise ValueError(f"prefix_len = {prefix_len}: the {prefix_pages.numel()} prefix pages hold 0 to {prefix_pages.numel() * S} tokens")
+    if prefix_len >= 2 ** 31 - 256:
+        raise ValueError(f"at most 2**31 - 257 prefix tokens, got {prefix_len}")
     if table.shape[1] * S > 2 ** 31 - 256 or B * T * H >= 2 ** 31:
         raise RuntimeError("at most 2**31 - 256 tokens to a row of table, and fewer than 2**31 query rows")
     q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)

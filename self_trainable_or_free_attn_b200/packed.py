@@ -108,7 +108,7 @@ def check_tokens(ref, **tensors):
 
 
 def check_ints(ref, **tensors):
-    """Device tensors of whole numbers as int32, contiguous."""
+    """Device tensors of whole numbers as int32, contiguous. int64 is narrowed to the nearest 32 bits hold: outside a bound stays outside."""
     out, dev = [], ref.get_device()
     for name, t in tensors.items():
         if t.get_device() != dev:
@@ -116,6 +116,8 @@ def check_ints(ref, **tensors):
         if t.dtype is not torch.int32 or not t.is_contiguous():
             if t.dtype not in (torch.int32, torch.int64):
                 raise RuntimeError(f"{name} must be int32, got {t.dtype}")
+            if t.dtype is torch.int64:
+                t = t.clamp(-2 ** 31, 2 ** 31 - 1)
             t = t.to(torch.int32).contiguous()
         out.append(t)
     return out
