@@ -6,6 +6,7 @@
  *   - D = 64 or 128, dtype 0 = bf16, 1 = fp16; heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads);
  *   - strides are in elements, multiples of 8; the last dimension is contiguous; pointers are 16-byte aligned (workspaces, and the outputs
  *     of the packed operators, 32-byte; lse and int32 arrays 4-byte);
+ *   - scale, the factor of the logits, is from 2^-126 to 2^126;
  *   - lse is the natural-log LSE in fp32, -inf for rows without a key, whose output is 0;
  *   - every wait inside the kernels is bounded; outputs of a tile whose wait gave up are NaN, and so is what later calls of the
  *     device return until es_device_status (echosparse_sm100.h) has read and cleared the word.

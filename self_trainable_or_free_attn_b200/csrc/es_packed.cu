@@ -67,6 +67,7 @@ extern "C" int es_packed_attn_fwd(const void* q, const void* k, const void* v, v
                                   int64_t q_token, int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
                                   float scale, int32_t causal, int32_t dtype, void* workspace, void* stream) {
     if (int rc = check_sizes("es_packed_attn_fwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
+    if (int rc = check_scale("es_packed_attn_fwd", scale)) return rc;
     if (total_q == 0) return 0;
     if (!q || !o || !lse || !cu_q || !cu_k || (total_k && (!k || !v)) || (!workspace && packed_fwd_workspace(batch, total_q, total_k, heads, kv_heads, D)))
         return set_error(-1, "es_packed_attn_fwd: null pointer");
@@ -91,6 +92,7 @@ extern "C" int es_packed_attn_bwd(const void* q, const void* k, const void* v, c
                                   int64_t v_token, int64_t v_head, int64_t do_token, int64_t do_head, float scale, int32_t causal, int32_t dtype,
                                   void* workspace, void* stream) {
     if (int rc = check_sizes("es_packed_attn_bwd", batch, total_q, total_k, heads, kv_heads, D, dtype)) return rc;
+    if (int rc = check_scale("es_packed_attn_bwd", scale)) return rc;
     if (!total_q) dq = nullptr;
     if (!total_k) dk = dv = nullptr;
     if (!dq && !dk && !dv) return 0;

@@ -55,6 +55,11 @@ inline int check_sizes(const char* name, int B, int Tq, int Tk, int H, int Hk, i
     return what ? set_error(-1, (std::string(name) + what).c_str()) : 0;
 }
 
+// A factor of the logits: a normal number, as is its product with log2(e). (0 times the -inf of a masked logit is NaN, and so is infinity times 0.)
+inline int check_scale(const char* name, float scale) {
+    return scale >= 0x1p-126f && scale <= 0x1p126f ? 0 : set_error(-1, (std::string(name) + ": scale must be from 2^-126 to 2^126").c_str());
+}
+
 inline int sm_count() {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;

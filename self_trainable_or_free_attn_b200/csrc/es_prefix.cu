@@ -649,6 +649,7 @@ extern "C" int es_prefix_attn(const void* q, const void* k_cache, const void* v_
                               int64_t k_page, int64_t k_token, int64_t k_head, int64_t v_page, int64_t v_token, int64_t v_head, float scale,
                               int32_t dtype, void* workspace, void* stream) {
     if (int rc = check_sizes("es_prefix_attn", batch, tokens, prefix_len, heads, kv_heads, D, dtype)) return rc;
+    if (int rc = check_scale("es_prefix_attn", scale)) return rc;
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
         return set_error(-1, "es_prefix_attn: page_size must be 16, 32, 64, 128 or 256");
     if (pages < 0 || table_width < 0 || n_prefix_pages < 0 || (int64_t)table_width * page_size > 0x7FFFFF00 || (int64_t)pages * page_size > 0x7FFFFFFF ||

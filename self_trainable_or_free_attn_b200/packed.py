@@ -77,8 +77,8 @@ def softmax_scale(scale, D):
     if scale is None:
         return 1.0 / math.sqrt(D)
     scale = float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"scale must be a finite number above 0, got {scale}")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:               # a normal number of 32 bits, as is its product with log2(e)
+        raise ValueError(f"scale must be above 0 and from 2**-126 to 2**126, got {scale}")
     return scale
 
 
