@@ -50,7 +50,7 @@ int es_packed_attn_bwd(const void* q, const void* k, const void* v, const void* 
  * [batch, heads, tokens]. prefix_pages [n_prefix_pages]: the pages of the prefix, of which the first prefix_len tokens count; table
  * [batch, table_width]: the pages of each request's own tokens, of which lengths[b] count, the queries' own keys the last of them: query i
  * sees the whole prefix and own tokens 0 .. lengths[b] - tokens + i. Keys in pages outside 0 .. pages - 1 are not attended to.
- * page_size 16, 32, 64, 128 or 256. workspace: es_prefix_workspace_bytes bytes, may be NULL where that is 0. */
+ * page_size 16, 32, 64, 128 or 256; at most 2^23 requests. workspace: es_prefix_workspace_bytes bytes, may be NULL where that is 0. */
 long long es_prefix_workspace_bytes(int32_t batch, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t D, int32_t prefix_len,
                                     int32_t table_width, int32_t page_size);
 int es_prefix_attn(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse, const int32_t* prefix_pages,

@@ -123,8 +123,8 @@ def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengt
         raise ValueError(f"prefix_len = {prefix_len}: the {prefix_pages.numel()} prefix pages hold 0 to {prefix_pages.numel() * S} tokens")
     if prefix_len >= 2 ** 31 - 256:
         raise ValueError(f"at most 2**31 - 257 prefix tokens, got {prefix_len}")
-    if table.shape[1] * S > 2 ** 31 - 256 or B * T * H >= 2 ** 31:
-        raise RuntimeError("at most 2**31 - 256 tokens to a row of table, and fewer than 2**31 query rows")
+    if table.shape[1] * S > 2 ** 31 - 256 or B * T * H >= 2 ** 31 or B > 2 ** 23:
+        raise RuntimeError("at most 2**31 - 256 tokens to a row of table, fewer than 2**31 query rows and at most 2**23 requests")
     q = q.contiguous() if q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
     o = empty(q)
     lse = torch.empty(B, H, T, device=q.device, dtype=torch.float32)
