@@ -11,7 +11,8 @@ A step of a decoding loop, all of it on the GPU and nothing synchronising, so th
     store_kv(k, v, k_cache, v_cache, plan.slots)                                         # per layer
     out = prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, plan.lengths)
 
-A prompt enters the same way, its own attention by `packed.packed_attention` with `plan.cu_new`.
+A prompt enters the same way; its own attention is `packed.packed_attention` with `plan.cu_new`, which reads no pages: behind a shared prefix each prompt
+brings the prefix's keys and values in front of its own (`cu_k`, as the prompt's next chunk does).
 """
 from dataclasses import dataclass
 
@@ -97,7 +98,8 @@ def store_kv(k, v, k_cache, v_cache, slots):
 @N.device_guard
 def prefix_attention(q, k_cache, v_cache, prefix_pages, prefix_len, table, lengths, *, scale=None, return_lse=False):
     """Attention of the newest tokens of a batch of requests, q [batch, tokens, heads, D], to a prefix that all of them share and to
-    their own tokens: [batch, tokens, heads, D], and with return_lse the natural-log LSE [batch, heads, tokens] in fp32.
+    their own tokens: [batch, tokens, heads, D], and with return_lse the natural-log LSE [batch, heads, tokens] in fp32. At most 2**23 requests. Softmax
+    statistics and sums are fp32, the weights are rounded to the inputs' type before they are multiplied with the values.
 
     The prefix is the first `prefix_len` tokens (an int; 0 for none) of the pages `prefix_pages` (int32); its keys and values are read once for
     the whole batch. The queries' own keys are the last of a request's `lengths[b]` tokens (what `extend_tables` returns), and query i

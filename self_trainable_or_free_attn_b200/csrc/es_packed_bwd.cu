@@ -8,8 +8,9 @@
 // P and dS are written over S and dP in tensor memory, as 16-bit pairs, and are the A operands of the second products from there. (One
 // pass instead would save two of seven products, S and dP again, and need dQ added with atomics in the order in which CTAs happen to run.)
 //
-// Tiles with rows that see few keys multiply what these roundings left as well, from the tensor memory that S and dP no longer need: there
-// they do not average out, neither in P and dS nor in the forward's O, which delta is summed from.
+// What rounding P and dS to 16 bits leaves is off by u at most per pair, as often up as down: dQ, dK and dV of long rows are off by 1.3 to 1.5 times what
+// their own rounding to the type is. Tiles with rows that see few keys multiply what these roundings left as well, from the tensor memory that S and dP no
+// longer need: there they do not average out, neither in P and dS nor in the forward's O, which delta is summed from.
 //
 //   warps 0-7  P and dS: a thread has row 32 (warp % 4) + lane and 64 columns, those of warps 4-7 the upper half
 //   warp 8     issues the MMAs; warp 9 issues the TMA loads; warp 10 (dK / dV) brings LSE and delta of the walked rows; the next one
@@ -19,8 +20,9 @@
 // that a mask cuts, values of the walked tiles that are not finite are set to 0 in shared memory once S and dP are there. dS is NaN already
 // where they are seen; dV alone gets what is not finite in dO at the end, from global memory.
 //
-// Bound by the chain S -> P -> dP -> dS of an iteration, which one set of 128 x 128 tiles cannot hide: accumulators and scores fill tensor memory, the
-// tiles shared memory. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.91 ms =
+// Bound by the chain S -> P -> dP -> dS of an iteration, which one set of 128 x 128 tiles cannot hide (tensor pipe 56 % busy, exponentials 22 to 28 %). At
+// D = 128 accumulators and scores fill tensor memory, the tiles shared memory; at D = 64 (tensor pipe 30 and 34 %) the dK / dV pass leaves 128 columns free,
+// the dQ pass 64, and nothing uses them. (Sixteen math warps instead of eight were no faster.) bf16, causal, 32,768 tokens in 8 sequences, 12 heads: dQ 0.91 ms =
 // 1,060 TFLOP/s, dK / dV 1.18 ms = 1,090. A CTA that takes tile after tile saves setting up and tearing down: 3 to 10 % of both passes.
 #include "es_packed_tc.cuh"
 

@@ -76,8 +76,9 @@ struct FwdArgs {
 
 __device__ __forceinline__ int seen_by(const FwdArgs& a, const Work& w, int t) { return a.b.causal ? min(max(w.base + t + 1, 0), w.nk) : w.nk; }
 // Whether row tile s is one of training with rows that see few keys (and one tile of keys in all): what rounding P left is multiplied with V as
-// well. delta = rowsum(dO o O) stands against sums over these few keys, where P's roundings do not average out: dQ and dK of short sequences
-// were off by up to 1.7 times what their own rounding is, and are by 1.0 to 1.4 times with it (and with the same of the backward's P and dS).
+// well. delta = rowsum(dO o O) stands against sums over these few keys, where P's roundings do not average out: dQ and dK of sequences of up to
+// 32 tokens were off by 1.5 to 1.7 times what their own rounding is (in the norm), and are by 1.00 times with it (and with the same of the backward's P
+// and dS). Longer rows go without: full attention 1.41 to 1.47 times from 33 keys on, causal 1.01 at 33, 1.20 at 64, 1.40 at 1,500.
 __device__ __forceinline__ bool is_fine(const FwdArgs& a, const Work& w, int s) { return w.i0 == 0 && w.end(s) == 1 && seen_by(a, w, s * a.tokens) <= FEW; }
 }  // namespace
 
@@ -449,6 +450,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[32 * h + 2 * j]), __uint_as_float(x[32 * h + 2 * j + 1])), cc, oo);
                         const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
                         sum = __fadd2_rn(sum, e);
+                        // the product takes 16 bits; the sum is of what was not rounded. Each key's weight is off by u at most and as often up as down: O is off by
+                        // 1.06 (4 keys) to 1.40 times (1,500) what its own rounding to the type is
                         p[j] = pack2<T>(e.x, e.y);
                     }
                     tmem_st16(scol + 16 * h, p);

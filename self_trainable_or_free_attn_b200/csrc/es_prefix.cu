@@ -374,6 +374,7 @@ own_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUte
                 __syncwarp();
                 fence_proxy_async_smem();
             }
+            // (P in 16 bits, the sum of what was not rounded: see es_packed_fwd.cu)
             const uint32_t vb = base + C::RING + slot * C::TILE;
 #pragma unroll
             for (int j = 0; j < KW / 16; ++j) {

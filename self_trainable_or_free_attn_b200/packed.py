@@ -2,8 +2,12 @@
 
 `packed_attention` is exact softmax attention of every sequence to its own keys, with gradients: causal or full, with as many
 query heads to a key head as the model has, from sequences of one token to long ones. It stands beside the block-sparse operators of
-`vsa`, which take sequences of one length: the same kernels' conventions (bf16 or fp16, head dim 64 or 128, fp32 softmax and LSE, one owner
-per gradient row: reproducible bit for bit).
+`vsa`, which take sequences of one length: the same kernels' conventions (bf16 or fp16, head dim 64 or 128, one owner per gradient row:
+reproducible bit for bit). Scores, softmax statistics, LSE and sums are fp32; the weights P and, in the backward, dS are rounded to the inputs' type
+before they are multiplied with V, dO, Q and K, which leaves an output off by 1.1 to 1.5 times its own rounding. Where rows see up to 32 keys the training
+path multiplies what these roundings left as well, and the outputs are off by their own rounding alone.
+
+Memory: a call that records a graph keeps, beside q, k, v, the output and its LSE, what rounding the output left, a second tensor of the output's size.
 
   q        [tokens, heads, D]; k, v [tokens, kv_heads, D], heads a multiple of kv_heads; any token and head strides (the thirds
            of a fused projection, say); what the kernels' loads cannot take (a last dimension with a stride, rows off 16 bytes) is copied
